@@ -18,7 +18,9 @@ SOURCES = ["common.hip", "index.hip", "encoder.hip", "gemm_bf16.hip"]
 HEADERS = ["otter_common.h", "otter_device.h", "otter_gemm.h", os.path.join("..", "..", "include", "otter_hip.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-pthread", "-Wall", "-Wno-unused-function",
-         "-Rpass-analysis=kernel-resource-usage"]
+         "-Rpass-analysis=kernel-resource-usage",
+         # no packed float32 instructions: some of their forms have given wrong results on this hardware
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # Kernels that load into REGISTERS from inline asm and wait for them by hand (counted vmcnt): the register allocator
 # does not know the destination is still in flight, so a spill there is not just slow -- it may reuse a register an
 # asynchronous load is still going to write (seen once as a GPU memory fault).  The build fails if one needs scratch.
