@@ -212,6 +212,23 @@ int otter_sharded_search(otter_index* const* shards, int G, const void* q, int64
 int otter_inbatch_scores(int device, const float* q, const float* c, const float* neg_c, int B, int d,
                          float* product, int32_t* rank, void* stream);
 
+/* The loss of the fine-tuning script over that matrix and its gradient (reference retrieval/criterions.py:10-27:
+ * cross entropy of [q c^T | q . neg_c] against the diagonal, mean over the batch), float32 throughout:
+ *   S = [q c^T | q . neg_c],  lse_i = log sum_j exp S_ij,  *loss = mean_i (lse_i - S_ii)
+ *   G = (exp(S - lse) - 1[j = i]) * *dloss / B,  dq = G c + G_neg neg_c,  dc = G^T q,  dneg = G_neg q
+ * All pointers are device pointers: q, c, neg_c (may be NULL) float32 [B, d]; scores float32 [B, ld] with
+ * ld >= B + (neg_c != NULL) -- the forward pass fills the first B (+ 1) columns, the backward pass reads them;
+ * lse float32 [B]; loss, dloss float32 [1].  1 <= B <= 65536.  The forward pass needs a workspace of
+ * otter_inbatch_loss_workspace(B, d) bytes for the time of the call (stream order).  Both calls only enqueue;
+ * the same inputs give the same bits (no atomics). */
+int64_t otter_inbatch_loss_workspace(int B, int d);
+int otter_inbatch_loss_forward(int device, const float* q, const float* c, const float* neg_c, int B, int d,
+                               float* scores, int ld, float* lse, float* loss, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+int otter_inbatch_loss_backward(int device, const float* dloss, const float* q, const float* c, const float* neg_c,
+                                int B, int d, const float* scores, int ld, const float* lse, float* dq, float* dc,
+                                float* dneg, void* stream);
+
 /* ---------------------------------------------------------------- encoder */
 
 typedef struct otter_encoder otter_encoder;
@@ -320,6 +337,77 @@ int otter_ln_stats(int device, const void* part, int P, int64_t M, int N, float 
 
 int  otter_encoder_out_dim(const otter_encoder* enc);
 void otter_encoder_destroy(otter_encoder* enc);
+
+/* --------------------------------------------------------------- training */
+
+/* Layer operators of a fine-tuning step (the reference trains the encoder of retrieval/models/tb_retriever.py with
+ * torch autograd, scripts/train_1hop_tb_retrieval.py:196-262).  dtype = element type of the activations and their
+ * gradients: OTTER_F32 or OTTER_BF16; sums, statistics and probabilities are float32.  Every call only enqueues,
+ * allocates nothing and uses no atomics: the same inputs give the same bits.
+ *
+ * Dropout: value e is dropped where its 16-bit draw is below T = round(65536 p), kept values are scaled by
+ * 65536 / (65536 - T); 0 <= p < 1.  The draws are Philox4x32 with 7 rounds under the 64-bit key *seed (DEVICE
+ * pointer, so that a captured graph can be given a new one; may be NULL when T = 0), eight to a counter:
+ *   rows       counter (col >> 3, row, 0xFFFFFFFF, call), draw of col: word (col & 7) >> 1, low half first
+ *   attention  counter (j >> 2, i >> 1, b * heads + h, call), draw of query i, key j of sequence b: word j & 3,
+ *              low half for even i (i, j count within their sequence, dense or packed)
+ * `call` tells apart the calls that share a seed; a backward call gets the seed and `call` of its forward call.
+ * No mask is stored. */
+
+/* y = dropout(x), [rows, cols] contiguous; the backward pass is the same call on dy. x == y is allowed. */
+int otter_dropout(int device, int dtype, const void* x, void* y, int64_t rows, int64_t cols, float p,
+                  const int64_t* seed, uint32_t call, void* stream);
+
+/* y = layer_norm(dropout(x) + residual), torch.nn.LayerNorm over the last dimension (reached in the reference through
+ * HF's BertSelfOutput / BertOutput from tb_retriever.py:180-185).  x, residual (may be NULL), y: [rows, cols]
+ * contiguous; weight, bias: [cols] of type wdtype; mean, rstd: float32 [rows], kept for the backward pass.
+ * 1 <= cols <= 8192, rows < 2^32. */
+int otter_layernorm_forward(int device, int dtype, int wdtype, const void* x, const void* residual, const void* weight,
+                            const void* bias, int64_t rows, int cols, float eps, float p, const int64_t* seed,
+                            uint32_t call, void* y, float* mean, float* rstd, void* stream);
+/* dx, dresidual [rows, cols], dweight, dbias [cols] (wdtype).  With p = 0 dresidual equals dx and may be NULL.
+ * rows = 0 gives zero dweight and dbias. */
+int64_t otter_layernorm_backward_workspace(int64_t rows, int cols);
+int otter_layernorm_backward(int device, int dtype, int wdtype, const void* dy, const void* x, const void* residual,
+                             const void* weight, const float* mean, const float* rstd, int64_t rows, int cols, float p,
+                             const int64_t* seed, uint32_t call, void* dx, void* dresidual, void* dweight, void* dbias,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/* softmax(scale q k^T) v with dropout on the probabilities, bidirectional, head dimension 64 (HF's BertSelfAttention,
+ * reached from tb_retriever.py:180-185), and its gradients with the probabilities made again from lse.
+ *
+ * A tensor is given as an otter_view: element strides of its batch, token and head dimension, the 64 elements of a head
+ * contiguous.  Data pointers and strides are multiples of 16 bytes.
+ *   dense   cu_seqlens NULL: [batch, tokens, heads, 64]; mask int64 [batch, tokens] (non-zero = attend, as input_mask of
+ *           the encoder) or NULL for every key.  Keys left out reach nothing, whatever they hold.  A sequence whose mask
+ *           leaves nothing attends to all its keys evenly, as in the encoder; no gradient reaches its q and k.
+ *   packed  cu_seqlens int32 [batch + 1], non-decreasing: sequence b is rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of
+ *           [total, heads, 64] tensors (stride_batch unused); tokens = the longest sequence (sizes the launch; a
+ *           longer one is still computed).  Rows of no sequence are set to zero in the outputs.
+ * lse: float32 [batch, heads, tokens] / [heads, total], log sum_j exp(scale q k^T), written by the forward pass. */
+typedef struct otter_view {
+    void* data;
+    int64_t stride_batch, stride_token, stride_head;
+} otter_view;
+
+typedef struct otter_attention_args {
+    int32_t dtype, batch, tokens, heads, head_dim;
+    uint32_t call;
+    float scale, dropout_p;
+    int64_t total;                    /* packed: rows of the tensors */
+    const int64_t* mask;
+    const int32_t* cu_seqlens;
+    const int64_t* seed;
+    otter_view q, k, v, out;
+    float* lse;
+    otter_view dout, dq, dk, dv;      /* backward only */
+    void* workspace;                  /* backward only: otter_attention_backward_workspace() bytes */
+    int64_t workspace_bytes;
+} otter_attention_args;
+
+int otter_attention_forward(int device, const otter_attention_args* args, void* stream);
+int64_t otter_attention_backward_workspace(const otter_attention_args* args);
+int otter_attention_backward(int device, const otter_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -34,6 +34,18 @@ class EncoderCfg(ctypes.Structure):
                 ("layer_norm_eps", ctypes.c_float)]
 
 
+class View(ctypes.Structure):
+    _fields_ = [("data", c_vp), ("stride_batch", c_i64), ("stride_token", c_i64), ("stride_head", c_i64)]
+
+
+class AttentionArgs(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("tokens", ctypes.c_int32), ("heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("call", ctypes.c_uint32), ("scale", ctypes.c_float),
+                ("dropout_p", ctypes.c_float), ("total", c_i64), ("mask", c_vp), ("cu_seqlens", c_vp), ("seed", c_vp),
+                ("q", View), ("k", View), ("v", View), ("out", View), ("lse", c_vp), ("dout", View), ("dq", View),
+                ("dk", View), ("dv", View), ("workspace", c_vp), ("workspace_bytes", c_i64)]
+
+
 # name -> (restype, argtypes); every symbol include/otter_hip.h declares
 SIGNATURES = {
     "otter_last_error": (ctypes.c_char_p, []),
@@ -69,6 +81,19 @@ SIGNATURES = {
     "otter_gemm_bf16_ln": (c_int, [c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64,
                                    c_int, c_int, c_vp]),
     "otter_ln_stats": (c_int, [c_int, c_vp, c_int, c_i64, c_int, ctypes.c_float, c_vp, c_vp]),
+    "otter_inbatch_loss_workspace": (c_i64, [c_int, c_int]),
+    "otter_inbatch_loss_forward": (c_int, [c_int, c_vp, c_vp, c_vp, c_int, c_int, c_vp, c_int, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "otter_inbatch_loss_backward": (c_int, [c_int, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_vp, c_int, c_vp, c_vp, c_vp, c_vp,
+                                            c_vp]),
+    "otter_dropout": (c_int, [c_int, c_int, c_vp, c_vp, c_i64, c_i64, ctypes.c_float, c_vp, ctypes.c_uint32, c_vp]),
+    "otter_layernorm_forward": (c_int, [c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_int, ctypes.c_float,
+                                        ctypes.c_float, c_vp, ctypes.c_uint32, c_vp, c_vp, c_vp, c_vp]),
+    "otter_layernorm_backward_workspace": (c_i64, [c_i64, c_int]),
+    "otter_layernorm_backward": (c_int, [c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_int,
+                                         ctypes.c_float, c_vp, ctypes.c_uint32, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "otter_attention_forward": (c_int, [c_int, ctypes.POINTER(AttentionArgs), c_vp]),
+    "otter_attention_backward_workspace": (c_i64, [ctypes.POINTER(AttentionArgs)]),
+    "otter_attention_backward": (c_int, [c_int, ctypes.POINTER(AttentionArgs), c_vp]),
     "otter_encoder_out_dim": (c_int, [c_vp]),
     "otter_encoder_destroy": (None, [c_vp]),
 }

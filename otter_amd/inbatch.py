@@ -7,6 +7,9 @@ each row's target come from one HIP kernel (otter_inbatch_scores, include/otter_
 passes that produce q / c / neg_c are the HIP encoder's (RobertaSingleRetrieverThreeCatPool.forward,
 retrieval/models/tb_retriever.py:235-239, restated in `retriever_outputs`).
 
+The loss over that matrix, with its gradient, is `inbatch_loss` (otter_inbatch_loss_forward / _backward); the layer
+operators of the same fine-tuning step are in otter_amd.training.
+
 Ties: torch's argsort leaves the order of equal scores unspecified; here an equal score in a lower column
 sorts first (argmax's first-index rule), so `rank == 0` is exactly `argmax == target`.
 """
@@ -14,6 +17,7 @@ import ctypes
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -41,6 +45,85 @@ def inbatch_scores(q, c, neg_c=None):
         ctypes.c_void_p(neg_c.data_ptr()) if neg_c is not None else None, B, d,
         ctypes.c_void_p(product.data_ptr()), ctypes.c_void_p(rank.data_ptr()), stream), "otter_inbatch_scores")
     return product, rank
+
+
+def _loss_operands(what, q, c, neg_c):
+    if not (torch.is_tensor(q) and q.is_cuda):
+        raise ValueError("%s: q must be a tensor on a GPU (the HIP path has no CPU fallback)" % what)
+    if q.dim() != 2 or c.shape != q.shape or (neg_c is not None and neg_c.shape != q.shape):
+        raise ValueError("%s: q, c and neg_c must all be [B, d]; got %s %s %s" % (
+            what, tuple(q.shape), tuple(c.shape), None if neg_c is None else tuple(neg_c.shape)))
+    if c.device != q.device or (neg_c is not None and neg_c.device != q.device):
+        raise ValueError("%s: q, c and neg_c must be on one GPU" % what)
+    return [None if t is None else t.to(torch.float32).contiguous() for t in (q, c, neg_c)]
+
+
+def inbatch_loss_forward(q, c, neg_c=None):
+    """loss_single (retrieval/criterions.py:10-27): cross entropy of the in-batch scores against their diagonal, mean over the
+    batch.  Returns (loss, product, lse): float32 scalar, the scores [B, B + (neg_c is not None)] and their row-wise
+    logsumexp [B]; the backward pass needs the last two.  B <= 65536."""
+    lib = _lib.load()
+    q, c, neg_c = _loss_operands("inbatch_loss", q, c, neg_c)
+    dev = q.device
+    B, d = q.shape
+    ncol = B + (neg_c is not None)
+    ld = (ncol + 3) // 4 * 4                  # rows of whole 16-byte pieces
+    nbytes = lib.otter_inbatch_loss_workspace(B, d)
+    if nbytes < 0:
+        _lib.check(int(nbytes), "otter_inbatch_loss_workspace")
+    buf = torch.empty((B, ld), dtype=torch.float32, device=dev)
+    lse = torch.empty((B,), dtype=torch.float32, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    _lib.check(lib.otter_inbatch_loss_forward(
+        dev.index, q.data_ptr(), c.data_ptr(), None if neg_c is None else neg_c.data_ptr(), B, d, buf.data_ptr(), ld,
+        lse.data_ptr(), loss.data_ptr(), ws.data_ptr(), nbytes, torch.cuda.current_stream(dev).cuda_stream),
+        "otter_inbatch_loss_forward")
+    return loss, buf[:, :ncol], lse
+
+
+def inbatch_loss_backward(dloss, q, c, neg_c, product, lse):
+    """Gradients (dq, dc, dneg_c or None), float32 [B, d], of inbatch_loss_forward for dloss, the gradient of the loss
+    (float32, one element on the GPU)."""
+    lib = _lib.load()
+    q, c, neg_c = _loss_operands("inbatch_loss_backward", q, c, neg_c)
+    dev = q.device
+    B, d = q.shape
+    ncol = B + (neg_c is not None)
+    if (tuple(product.shape) != (B, ncol) or product.dtype != torch.float32 or product.device != dev
+            or (ncol > 1 and product.stride(1) != 1) or tuple(lse.shape) != (B,) or lse.dtype != torch.float32
+            or lse.device != dev or not lse.is_contiguous()):
+        raise ValueError("inbatch_loss_backward: product and lse must be what inbatch_loss_forward returned")
+    if dloss.numel() != 1 or dloss.dtype != torch.float32 or dloss.device != dev:
+        raise ValueError("inbatch_loss_backward: dloss must be one float32 element on %s" % dev)
+    ld = product.stride(0) if B > 1 else ncol
+    dq, dc = torch.empty_like(q), torch.empty_like(c)
+    dneg = None if neg_c is None else torch.empty_like(neg_c)
+    _lib.check(lib.otter_inbatch_loss_backward(
+        dev.index, dloss.data_ptr(), q.data_ptr(), c.data_ptr(), None if neg_c is None else neg_c.data_ptr(), B, d,
+        product.data_ptr(), ld, lse.data_ptr(), dq.data_ptr(), dc.data_ptr(), None if dneg is None else dneg.data_ptr(),
+        torch.cuda.current_stream(dev).cuda_stream), "otter_inbatch_loss_backward")
+    return dq, dc, dneg
+
+
+class _InbatchLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, c, neg_c):
+        loss, product, lse = inbatch_loss_forward(q, c, neg_c)
+        ctx.save_for_backward(q, c, neg_c, product, lse)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        q, c, neg_c, product, lse = ctx.saved_tensors
+        dq, dc, dneg = inbatch_loss_backward(dloss.contiguous(), q, c, neg_c, product, lse)
+        return dq.to(q.dtype), dc.to(c.dtype), None if dneg is None else dneg.to(neg_c.dtype)
+
+
+def inbatch_loss(q, c, neg_c=None):
+    """Differentiable in-batch loss (inbatch_loss_forward)."""
+    return _InbatchLoss.apply(q, c, neg_c)
 
 
 def mrr_accuracy(ranks):
