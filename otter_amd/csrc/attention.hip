@@ -24,6 +24,14 @@ using namespace otter;
 
 constexpr int DH = 64;         // head dimension
 constexpr int TR = 64;         // rows of a streamed tile
+#ifndef SUBU
+#define SUBU 1
+#endif
+#ifndef W_FWD
+#define W_FWD 2
+#define W_DQ 2
+#define W_DKV 2
+#endif
 constexpr int OWN = 128;       // rows a workgroup owns: 4 waves x 32
 
 struct View {                  // element strides of a [batch, token, head, 64] tensor (batch stride unused when packed)
@@ -88,31 +96,56 @@ __device__ __forceinline__ void zero_outside(const AttnTrainArgs& a, int h, cons
 }
 
 // ------------------------------------------------------------------ tiles
+// A tile in LDS: 64 rows of 64 elements, 16 bytes of padding a row.  With that pitch (36 / 68 words) neither the 16-byte
+// reads down a column of rows nor the transposed 8-byte reads conflict, and every address is one of two lane constants plus
+// an immediate (an XOR swizzle needs a register for each of its chunks: 60 more, one wave less a SIMD).
 template <typename T>
 struct Tile {
-    static constexpr int ROWB = DH * (int)sizeof(T);   // bytes a row
-    static constexpr int CH = ROWB / 16;               // 16-byte chunks a row
-    static constexpr int NF = CH / 2;                  // fragment chunks a lane
+    static constexpr int PITCH = DH * (int)sizeof(T) + 16;
+    static constexpr int CH = DH * (int)sizeof(T) / 16;   // 16-byte chunks a row
+    static constexpr int NF = CH / 2;                     // fragment chunks a lane: 2 j + lane half
     static constexpr int EPC = 16 / (int)sizeof(T);
-    static constexpr int BYTES = TR * ROWB;
-    // chunk c of row r lies at chunk c ^ swz(r): the 32 rows a fragment read touches spread over the banks
-    static __device__ __forceinline__ int swz(int r) { return CH == 16 ? (r & 15) : ((r >> 1) & 7); }
-    static __device__ __forceinline__ float4 frag(const char* t, int row, int c) {
-        return *reinterpret_cast<const float4*>(t + row * ROWB + ((c ^ swz(row)) << 4));
+    static constexpr int BYTES = TR * PITCH;
+};
+
+struct Lane {
+    int lane, wave, h, l31;
+    __device__ __forceinline__ Lane() : lane(threadIdx.x & 63), wave(threadIdx.x >> 6), h((threadIdx.x >> 5) & 1), l31(threadIdx.x & 31) {}
+    template <typename T>
+    __device__ __forceinline__ int frag() const { return l31 * Tile<T>::PITCH + h * 16; }
+    // bf16: the corner of this lane's 4 x 16 block for the transposed reads; float: row 4 h, column l31
+    template <typename T>
+    __device__ __forceinline__ int col() const {
+        return sizeof(T) == 2 ? (4 * h + ((lane & 15) >> 2)) * Tile<T>::PITCH + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2
+                              : 4 * h * Tile<T>::PITCH + l31 * 4;
     }
 };
 
-// rows row0 .. row0 + 63 into LDS; rows that `keep` leaves out (bit per row) become zeros and are not read
+// A tile on its way: 64 rows through the registers of the workgroup's 256 threads, loaded while the tile before it is
+// multiplied.  Rows that `keep` leaves out (a bit per row) become zeros and are not read.
 template <typename T>
-__device__ __forceinline__ void stage(char* lds, const T* base, long long st, int row0, u64 keep) {
+struct Stage {
     using X = Tile<T>;
-    for (int c = threadIdx.x; c < TR * X::CH; c += blockDim.x) {
-        const int r = c / X::CH, p = c % X::CH;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if ((keep >> r) & 1) v = *reinterpret_cast<const float4*>(base + (long long)(row0 + r) * st + p * X::EPC);
-        *reinterpret_cast<float4*>(lds + r * X::ROWB + ((p ^ X::swz(r)) << 4)) = v;
+    static constexpr int N = TR * X::CH / 256, STEP = 256 / X::CH;   // loads a thread, rows between them
+    float4 v[N];
+    const T* p;                 // this thread's first chunk of the next tile
+    long long st;
+    __device__ __forceinline__ Stage(const T* base, long long stride) : p(base + (threadIdx.x / X::CH) * stride + (threadIdx.x % X::CH) * X::EPC), st(stride) {}
+    __device__ __forceinline__ void load(u64 keep) {
+        const u64 mine = keep >> (threadIdx.x / X::CH);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if ((mine >> (i * STEP)) & 1) v[i] = *reinterpret_cast<const float4*>(p + i * STEP * st);
+        }
+        p += TR * st;
     }
-}
+    __device__ __forceinline__ void store(char* lds) const {
+        char* d = lds + (threadIdx.x / X::CH) * X::PITCH + (threadIdx.x % X::CH) * 16;
+#pragma unroll
+        for (int i = 0; i < N; ++i) *reinterpret_cast<float4*>(d + i * STEP * X::PITCH) = v[i];
+    }
+};
 
 template <typename T>
 __device__ __forceinline__ void mma(f32x16& acc, const float4& a, const float4& b) {
@@ -133,54 +166,45 @@ __device__ __forceinline__ f32x16 zero16() {
 }
 
 // row of a 32 x 32 accumulator tile that register r of lane half h holds
-__device__ __forceinline__ int acc_row(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
+__device__ __forceinline__ constexpr int acc_row(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
 
-// acc[rows of the tile][own rows on the lane] = tile rows (row0 .. row0 + 31) x own fragments
+// acc[rows of the tile][own rows on the lane] = tile rows (32 from t on) x own fragments; t: the tile + Lane::frag
 template <typename T>
-__device__ __forceinline__ f32x16 row_product(const char* t, int row0, const float4 (&own)[Tile<T>::NF], int l31, int h) {
+__device__ __forceinline__ f32x16 row_product(const char* t, const float4 (&own)[Tile<T>::NF]) {
     f32x16 acc = zero16();
 #pragma unroll
-    for (int j = 0; j < Tile<T>::NF; ++j) mma<T>(acc, Tile<T>::frag(t, row0 + l31, 2 * j + h), own[j]);
+    for (int j = 0; j < Tile<T>::NF; ++j) mma<T>(acc, *reinterpret_cast<const float4*>(t + j * 32), own[j]);
     return acc;
 }
 
-// o[d half] += X^T w: X = tile rows row0 .. row0 + 31, w = an accumulator tile with X's row on the registers.
-// bf16: w is rounded here, the one rounding between the two products (2^-9 of each weight; sums stay in float32).
+// o[d half] += X^T w: X = tile rows (32 from t on), w = an accumulator tile with X's row on the registers; t: the tile +
+// Lane::col.  bf16: w is rounded here, the one rounding between the two products (2^-8 of each weight at most; the sums
+// stay in float32).
 template <typename T>
-__device__ __forceinline__ void col_product(f32x16 (&o)[2], const char* t, int row0, const f32x16& w, int lane) {
-    using X = Tile<T>;
-    const int h = lane >> 5, l31 = lane & 31;
+__device__ __forceinline__ void col_product(f32x16 (&o)[2], const char* t, const f32x16& w) {
+    constexpr int P = Tile<T>::PITCH;
     if constexpr (sizeof(T) == 2) {
-        const int i16 = lane & 15, qq = i16 >> 2, pp = i16 & 3, g = (lane >> 4) & 1;
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
             bf16x8 wb;
 #pragma unroll
             for (int j = 0; j < 8; ++j) wb[j] = (__bf16)w[8 * s2 + j];
-            const int r0 = row0 + s2 * 16 + 4 * h + qq;
 #pragma unroll
             for (int d = 0; d < 2; ++d) {
                 // X^T[d][row], rows 16 s2 + 8 (j >> 2) + 4 h + (j & 3): two transposed reads of 4 rows x 16 columns
-                const int byte = (d * 32 + 16 * g + 4 * pp) * 2, c = byte >> 4, in = byte & 15;
-                const char* p0 = t + r0 * X::ROWB + ((c ^ X::swz(r0)) << 4) + in;
-                const char* p1 = t + (r0 + 8) * X::ROWB + ((c ^ X::swz(r0 + 8)) << 4) + in;
+                const char* p0 = t + s2 * 16 * P + d * 64;
                 const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)p0);
-                const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)p1);
+                const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)(p0 + 8 * P));
                 const short va[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, va), wb, o[d], 0, 0, 0);
             }
         }
     } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int row = row0 + acc_row(r, h);
+        for (int r = 0; r < 16; ++r)
 #pragma unroll
-            for (int d = 0; d < 2; ++d) {
-                const int col = d * 32 + l31;
-                const float x = *reinterpret_cast<const float*>(t + row * X::ROWB + (((col >> 2) ^ X::swz(row)) << 4) + (col & 3) * 4);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, w[r], o[d], 0, 0, 0);
-            }
-        }
+            for (int d = 0; d < 2; ++d)
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(t + acc_row(r, 0) * P + d * 128), w[r], o[d], 0, 0, 0);
     }
 }
 
@@ -190,6 +214,17 @@ __device__ __forceinline__ void load_own(float4 (&f)[Tile<T>::NF], const T* base
 #pragma unroll
     for (int j = 0; j < Tile<T>::NF; ++j)
         f[j] = *reinterpret_cast<const float4*>(base + (long long)row * st + (2 * j + h) * Tile<T>::EPC);
+}
+
+template <typename T>
+__device__ __forceinline__ void negate(float4 (&f)[Tile<T>::NF]) {
+    constexpr u32 sign = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
+#pragma unroll
+    for (int j = 0; j < Tile<T>::NF; ++j) {
+        u32* w = reinterpret_cast<u32*>(&f[j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] ^= sign;
+    }
 }
 
 // store o[2] (head dimension on the registers, row on the lane) times f
@@ -225,54 +260,103 @@ __device__ __forceinline__ int key_end(const AttnTrainArgs& a, const Seq& s, boo
     return s.len;
 }
 
-// bit r: key j0 + r counts
-__device__ __forceinline__ u64 key_bits(const AttnTrainArgs& a, const Seq& s, int j0, bool even) {
-    const int j = j0 + (threadIdx.x & 63);
-    return __ballot(j < s.len && (even || !a.mask || a.mask[(long long)s.b * a.L + j] != 0));
-}
+// bit r: key j0 + r counts.  The mask's value of this lane's key is loaded a tile before it is needed.
+struct KeyBits {
+    const long long* m;        // the sequence's mask, or null: every key below len counts
+    int len;
+    long long v;
+    __device__ __forceinline__ KeyBits(const AttnTrainArgs& a, const Seq& s, bool even)
+        : m(a.mask && !even ? a.mask + (long long)s.b * a.L : nullptr), len(s.len), v(1) {}
+    __device__ __forceinline__ void fetch(int j0) {
+        const int j = j0 + (threadIdx.x & 63);
+        if (m && j < len) v = m[j];
+    }
+    __device__ __forceinline__ u64 bits(int j0) const { return __ballot(j0 + (int)(threadIdx.x & 63) < len && v != 0); }
+};
 
 // bits of rows j0 .. j0 + 63 below n
 __device__ __forceinline__ u64 row_bits(int j0, int n) { return n - j0 >= 64 ? ~0ull : (1ull << max(n - j0, 0)) - 1ull; }
 
 // ------------------------------------------------------------------ draws
-// bit r: the value in register r is kept.  QL: the query is on the lane (row i) and keys j0 + acc_row(r, h) on the
-// registers; otherwise the key is on the lane (row j) and queries i0 + acc_row(r, h) on the registers.
-template <bool QL>
-__device__ __forceinline__ u32 keep16(const DropArgs& d, u32 k0, u32 k1, u32 bh, int own, int t0, int h) {
-    u32 keep = 0;
-    if constexpr (QL) {
+template <int CTRL>
+__device__ __forceinline__ u32 quad(u32 x) { return (u32)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xF, 0xF, true); }
+
+// Draws of a 32 x 32 score tile.  x[8]: two draws of 16 bits each; kept(r) tests the one of register r.
+// A counter's eight draws (2 queries x 4 keys) belong to a pair of lanes where the query is on the lane and to four lanes
+// where the key is; each of them makes its share of the counters and they hand the words around inside the quad (DPP), so no
+// draw is made twice: two counters a lane for sixteen values.
+struct Draws {
+    u32 x[8];
+    u32 thr, thrhi;
+    // query on the lane: keys j0 + acc_row(r, h) of query i.  The even query's lane makes groups 0 and 1 of four keys, the
+    // odd one's 2 and 3; of every word the even query takes the low half, the odd one the high half.
+    __device__ __forceinline__ void queries(const DropArgs& d, u32 k0, u32 k1, u32 bh, int i, int j0, int h) {
+        thr = d.thr;
+        thrhi = d.thr << 16;
+        const u32 odd = (u32)i & 1u, sel = odd ? 0x03020706u : 0x05040100u;     // bytes 0-3: own word, 4-7: the partner's
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const Philox4 w = philox7((u32)(t0 + 8 * g + 4 * h) >> 2, (u32)own >> 1, bh, d.call, k0, k1);
+        for (int g = 0; g < 2; ++g) {
+            const Philox4 w = philox7((u32)((j0 + 4 * h) >> 2) + 2 * g + 4 * odd, (u32)i >> 1, bh, d.call, k0, k1);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const u32 draw = own & 1 ? w.w[e] >> 16 : w.w[e] & 0xFFFFu;
-                keep |= (u32)(draw >= d.thr) << (4 * g + e);
-            }
+            for (int e = 0; e < 4; ++e) x[4 * g + e] = __builtin_amdgcn_perm(quad<0xB1>(w.w[e]), w.w[e], sel);
         }
-    } else {
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const Philox4 w = philox7((u32)own >> 2, (u32)(t0 + 8 * g + 4 * h + 2 * e) >> 1, bh, d.call, k0, k1);
-                const u32 x = own & 2 ? (own & 1 ? w.w[3] : w.w[2]) : (own & 1 ? w.w[1] : w.w[0]);
-                keep |= (u32)((x & 0xFFFFu) >= d.thr) << (4 * g + 2 * e);
-                keep |= (u32)((x >> 16) >= d.thr) << (4 * g + 2 * e + 1);
-            }
     }
-    return keep;
-}
+    // low half of x[4 g + e]: group g, high half: group g + 2
+    __device__ __forceinline__ bool kept_q(int r) const {
+        return r < 8 ? (unsigned short)x[r] >= (unsigned short)thr : x[r - 8] >= thrhi;
+    }
+    // key on the lane: queries i0 + acc_row(r, h) of key j.  Lane t of the quad makes the counters of query pairs t and t + 4
+    // (of the eight pairs its half holds) and takes word t of every counter: a 4 x 4 transpose of words, twice.
+    __device__ __forceinline__ void keys(const DropArgs& d, u32 k0, u32 k1, u32 bh, int j, int i0, int h) {
+        thr = d.thr;
+        thrhi = d.thr << 16;
+        const u32 t = (u32)j & 3u;
+        const bool o1 = t & 1u, o2 = t & 2u;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            // pair p = 2 g + e: queries i0 + 8 g + 4 h + 2 e and the next; here p = t + 4 c
+            const Philox4 w = philox7((u32)j >> 2, (u32)(i0 >> 1) + 8 * c + 4 * (t >> 1) + 2 * h + (t & 1u), bh, d.call, k0, k1);
+            // every lane runs every move: a move inside a conditional's arm would read lanes that are switched off
+            const u32 n0 = quad<0xB1>(w.w[0]), n1 = quad<0xB1>(w.w[1]), n2 = quad<0xB1>(w.w[2]), n3 = quad<0xB1>(w.w[3]);
+            const u32 a0 = o1 ? n1 : w.w[0], a1 = o1 ? w.w[1] : n0, a2 = o1 ? n3 : w.w[2], a3 = o1 ? w.w[3] : n2;
+            const u32 m0 = quad<0x4E>(a0), m1 = quad<0x4E>(a1), m2 = quad<0x4E>(a2), m3 = quad<0x4E>(a3);
+            x[4 * c] = o2 ? m2 : a0;
+            x[4 * c + 1] = o2 ? m3 : a1;
+            x[4 * c + 2] = o2 ? a2 : m0;
+            x[4 * c + 3] = o2 ? a3 : m1;
+        }
+    }
+    // x[p]: low half query 2 p of the half's, high half the next
+    __device__ __forceinline__ bool kept_k(int r) const {
+        return r & 1 ? x[r >> 1] >= thrhi : (unsigned short)x[r >> 1] >= (unsigned short)thr;
+    }
+};
+
+struct Key2 {
+    u32 k0 = 0, k1 = 0;
+    __device__ __forceinline__ explicit Key2(const DropArgs& d) {
+        if (d.thr) {
+            const u64 seed = (u64)*d.seed;
+            k0 = (u32)seed;
+            k1 = (u32)(seed >> 32);
+        }
+    }
+};
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ------------------------------------------------------------------ forward
-template <typename T>
-__global__ __launch_bounds__(256) void attn_fwd_kernel(AttnTrainArgs a) {
+// A workgroup owns 128 queries, a wave 32 (one on each lane of a half), and streams the keys in tiles of 64.
+// The running maximum is let stand while no score passes it by more than 2^8 (in base 2 exponents: the sums and the
+// probabilities then stay below 2^8 times their final size, harmless in float32 and for bfloat16's relative rounding), so
+// that the accumulators are rescaled once or twice a row and not at every tile.
+template <typename T, bool DROP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? W_FWD : 2) void attn_fwd_kernel(AttnTrainArgs a) {
     using X = Tile<T>;
-    __shared__ __attribute__((aligned(16))) char sK[X::BYTES];
-    __shared__ __attribute__((aligned(16))) char sV[X::BYTES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, l31 = lane & 31;
+    __shared__ __attribute__((aligned(16))) char sK[2][X::BYTES];
+    __shared__ __attribute__((aligned(16))) char sV[2][X::BYTES];
+    const Lane ln;
+    const int h = ln.h, l31 = ln.l31, wave = ln.wave;
     const int items = a.nblk * a.heads * a.B;
     if ((int)blockIdx.x >= items) return zero_outside<T>(a, blockIdx.x - items, a.o, a.lse);
     const Seq s = find_seq(a, xcd_remap(blockIdx.x, items));
@@ -281,76 +365,94 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(AttnTrainArgs a) {
     const T *Q = head_ptr<T>(a, a.q, s), *K = head_ptr<T>(a, a.k, s), *V = head_ptr<T>(a, a.v, s);
     T* O = head_ptr<T>(a, a.o, s);
     const u32 bh = (u32)(s.b * a.heads + s.h);
-    u32 k0 = 0, k1 = 0;
-    if (a.drop.thr) {
-        const u64 seed = (u64)*a.drop.seed;
-        k0 = (u32)seed;
-        k1 = (u32)(seed >> 32);
-    }
+    const Key2 key(a.drop);
+    const float c2 = fmaxf(fabsf(a.c2), 1e-30f);   // not 0: a left-out key's -inf has to stay one
     for (int q0 = s.blk * OWN; q0 < s.len; q0 += a.nblk * OWN) {
         const int i = q0 + wave * 32 + l31;
         float4 qf[X::NF];
         load_own<T>(qf, Q, a.q.st, min(i, s.len - 1), h);
+        if (a.c2 < 0.0f) negate<T>(qf);
         f32x16 o[2] = {zero16(), zero16()};
-        float m = -INFINITY, l = 0.0f;
-        for (int j0 = 0; j0 < kend; j0 += TR) {
-            const u64 bits = key_bits(a, s, j0, even);
+        float m = -INFINITY, base = 0.0f, l = 0.0f;   // base: m, or 0 while no score is above -inf
+        KeyBits kb(a, s, even);
+        Stage<T> rk(K, a.k.st), rv(V, a.v.st);
+        kb.fetch(0);
+        u64 next = kb.bits(0);
+        rk.load(next);
+        rv.load(next);
+        kb.fetch(TR);
+        for (int j0 = 0, buf = 0; j0 < kend; j0 += TR, buf ^= 1) {
+            const u64 bits = next;
+            rk.store(sK[buf]);
+            rv.store(sV[buf]);
+            __syncthreads();               // everyone is done with the other buffer, too
+            if (j0 + TR < kend) {
+                next = kb.bits(j0 + TR);
+                rk.load(next);
+                rv.load(next);
+                kb.fetch(j0 + 2 * TR);
+            }
             if (bits == 0) continue;
-            __syncthreads();
-            stage<T>(sK, K, a.k.st, j0, bits);
-            stage<T>(sV, V, a.v.st, j0, bits);
-            __syncthreads();
             f32x16 sc[2];
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub) sc[sub] = even ? zero16() : row_product<T>(sK[buf] + sub * 32 * X::PITCH + ln.frag<T>(), qf);
+            if (~bits != 0) {
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub) {
+                    const u32 kb32 = (u32)(bits >> (32 * sub)) >> (4 * h);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sc[sub][r] = (kb32 >> acc_row(r, 0)) & 1u ? sc[sub][r] : -INFINITY;
+                }
+            }
             float mx = -INFINITY;
 #pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fmaxf(sc[0][r], sc[1][r]));
+            mx = fmaxf(mx, __shfl_xor(mx, 32)) * c2;
+            // mx > m + 8 or a NaN: move the maximum
+            if (__any(!(mx <= m + 8.0f))) {
+                const float mnew = fmaxf(m, mx);
+                base = mnew == -INFINITY ? 0.0f : mnew;
+                const float alpha = exp2_(m - base);
+                m = mnew;
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < 2; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+            }
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
-                sc[sub] = row_product<T>(sK, sub * 32, qf, l31, h);
-                const u32 kb = (u32)(bits >> (32 * sub)) >> (4 * h);
+                Draws w;
+                if constexpr (DROP) w.queries(a.drop, key.k0, key.k1, bh, i, j0 + 32 * sub, h);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    float v = even ? 0.0f : sc[sub][r] * a.c2;
-                    v = (kb >> acc_row(r, 0)) & 1u ? v : -INFINITY;
-                    sc[sub][r] = v;
-                    mx = fmaxf(mx, v);
+                    const float p = exp2_(fmaf(sc[sub][r], c2, -base));
+                    sum[r & 1] += p;                                 // the softmax's sum is over all keys, dropped or not
+                    sc[sub][r] = !DROP || w.kept_q(r) ? p : 0.0f;
                 }
+                col_product<T>(o, sV[buf] + sub * 32 * X::PITCH + ln.col<T>(), sc[sub]);
             }
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float mnew = fmaxf(m, mx), base = mnew == -INFINITY ? 0.0f : mnew;
-            const float alpha = exp2_(m - base);
-            m = mnew;
-            float sum = 0.0f;
-#pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-                const u32 keep = a.drop.thr ? keep16<true>(a.drop, k0, k1, bh, i, j0 + 32 * sub, h) : 0xFFFFu;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float p = exp2_(sc[sub][r] - base);
-                    sum += p;                                        // the softmax's sum is over all keys, dropped or not
-                    sc[sub][r] = (keep >> r) & 1u ? p : 0.0f;
-                }
-            }
-            l = l * alpha + sum + __shfl_xor(sum, 32);
-#pragma unroll
-            for (int d = 0; d < 2; ++d)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
-#pragma unroll
-            for (int sub = 0; sub < 2; ++sub) col_product<T>(o, sV, sub * 32, sc[sub], lane);
+            l += sum[0] + sum[1];
         }
+        l += __shfl_xor(l, 32);
         if (i < s.len) {
             store_own<T>(O + (long long)i * a.o.st, o, a.drop.scale / l, h);
-            if (h == 0) a.lse[s.stat + i] = (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+            if (h == 0) a.lse[s.stat + i] = (base + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
         }
+        __syncthreads();                   // the buffers are free for the next rows
     }
 }
 
 // ------------------------------------------------------------------ backward: dQ (and D)
-template <typename T>
-__global__ __launch_bounds__(256) void attn_dq_kernel(AttnTrainArgs a) {
+// The forward kernel's walk again: queries on the lanes, dS^T is the right operand of dQ^T = K^T dS^T.
+template <typename T, bool DROP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? W_DQ : 2) void attn_dq_kernel(AttnTrainArgs a) {
     using X = Tile<T>;
-    __shared__ __attribute__((aligned(16))) char sK[X::BYTES];
-    __shared__ __attribute__((aligned(16))) char sV[X::BYTES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, l31 = lane & 31;
+    __shared__ __attribute__((aligned(16))) char sK[2][X::BYTES];
+    __shared__ __attribute__((aligned(16))) char sV[2][X::BYTES];
+    const Lane ln;
+    const int h = ln.h, l31 = ln.l31, wave = ln.wave;
     const int items = a.nblk * a.heads * a.B;
     if ((int)blockIdx.x >= items) return zero_outside<T>(a, blockIdx.x - items, a.dq, nullptr);
     const Seq s = find_seq(a, xcd_remap(blockIdx.x, items));
@@ -360,12 +462,7 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(AttnTrainArgs a) {
     const T *O = head_ptr<T>(a, a.o, s), *dO = head_ptr<T>(a, a.dout, s);
     T* dQ = head_ptr<T>(a, a.dq, s);
     const u32 bh = (u32)(s.b * a.heads + s.h);
-    u32 k0 = 0, k1 = 0;
-    if (a.drop.thr) {
-        const u64 seed = (u64)*a.drop.seed;
-        k0 = (u32)seed;
-        k1 = (u32)(seed >> 32);
-    }
+    const Key2 key(a.drop);
     for (int q0 = s.blk * OWN; q0 < s.len; q0 += a.nblk * OWN) {
         const int i = q0 + wave * 32 + l31, ic = min(i, s.len - 1);
         float4 qf[X::NF], df[X::NF];
@@ -383,41 +480,62 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(AttnTrainArgs a) {
         load_own<T>(qf, Q, a.q.st, ic, h);
         const float lse2 = a.lse[s.stat + ic] * 1.4426950408889634f;
         f32x16 o[2] = {zero16(), zero16()};
-        if (!even)                                  // even: dS = 0
-            for (int j0 = 0; j0 < kend; j0 += TR) {
-                const u64 bits = key_bits(a, s, j0, even);
+        if (!even) {                                // even: dS = 0
+            KeyBits kb(a, s, even);
+            Stage<T> rk(K, a.k.st), rv(V, a.v.st);
+            kb.fetch(0);
+            u64 next = kb.bits(0);
+            rk.load(next);
+            rv.load(next);
+            kb.fetch(TR);
+            for (int j0 = 0, buf = 0; j0 < kend; j0 += TR, buf ^= 1) {
+                const u64 bits = next;
+                rk.store(sK[buf]);
+                rv.store(sV[buf]);
+                __syncthreads();
+                if (j0 + TR < kend) {
+                    next = kb.bits(j0 + TR);
+                    rk.load(next);
+                    rv.load(next);
+                    kb.fetch(j0 + 2 * TR);
+                }
                 if (bits == 0) continue;
-                __syncthreads();
-                stage<T>(sK, K, a.k.st, j0, bits);
-                stage<T>(sV, V, a.v.st, j0, bits);
-                __syncthreads();
-#pragma unroll
+#pragma unroll SUBU
                 for (int sub = 0; sub < 2; ++sub) {
-                    f32x16 sc = row_product<T>(sK, sub * 32, qf, l31, h);
-                    const f32x16 dp = row_product<T>(sV, sub * 32, df, l31, h);
-                    const u32 kb = (u32)(bits >> (32 * sub)) >> (4 * h);
-                    const u32 keep = a.drop.thr ? keep16<true>(a.drop, k0, k1, bh, i, j0 + 32 * sub, h) : 0xFFFFu;
+                    f32x16 sc = row_product<T>(sK[buf] + sub * 32 * X::PITCH + ln.frag<T>(), qf);
+                    const f32x16 dp = row_product<T>(sV[buf] + sub * 32 * X::PITCH + ln.frag<T>(), df);
+                    Draws w;
+                    if constexpr (DROP) w.queries(a.drop, key.k0, key.k1, bh, i, j0 + 32 * sub, h);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const float p = exp2_(fmaf(sc[r], a.c2, -lse2));
-                        const float g = ((keep >> r) & 1u ? dp[r] * a.drop.scale : 0.0f) - D;
-                        sc[r] = (kb >> acc_row(r, 0)) & 1u ? p * g : 0.0f;
+                        const float g = !DROP ? dp[r] - D : fmaf(w.kept_q(r) ? dp[r] : 0.0f, a.drop.scale, -D);
+                        sc[r] = p * g;
                     }
-                    col_product<T>(o, sK, sub * 32, sc, lane);
+                    if (~bits != 0) {
+                        const u32 kb32 = (u32)(bits >> (32 * sub)) >> (4 * h);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) sc[r] = (kb32 >> acc_row(r, 0)) & 1u ? sc[r] : 0.0f;
+                    }
+                    col_product<T>(o, sK[buf] + sub * 32 * X::PITCH + ln.col<T>(), sc);
                 }
             }
+            __syncthreads();
+        }
         if (i < s.len) store_own<T>(dQ + (long long)i * a.dq.st, o, a.scale, h);
     }
 }
 
 // ------------------------------------------------------------------ backward: dK, dV
-template <typename T>
-__global__ __launch_bounds__(256) void attn_dkv_kernel(AttnTrainArgs a) {
+// A workgroup owns 128 keys, a wave 32 (one on each lane of a half), and streams the queries in tiles of 64.
+template <typename T, bool DROP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? W_DKV : 2) void attn_dkv_kernel(AttnTrainArgs a) {
     using X = Tile<T>;
-    __shared__ __attribute__((aligned(16))) char sQ[X::BYTES];
-    __shared__ __attribute__((aligned(16))) char sO[X::BYTES];
-    __shared__ float sL[TR], sD[TR];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, l31 = lane & 31;
+    __shared__ __attribute__((aligned(16))) char sQ[2][X::BYTES];
+    __shared__ __attribute__((aligned(16))) char sO[2][X::BYTES];
+    __shared__ __attribute__((aligned(16))) float sL[2][TR], sD[2][TR];
+    const Lane ln;
+    const int h = ln.h, l31 = ln.l31, wave = ln.wave;
     const int items = a.nblk * a.heads * a.B;
     if ((int)blockIdx.x >= items) {
         zero_outside<T>(a, blockIdx.x - items, a.dk, nullptr);
@@ -430,51 +548,73 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(AttnTrainArgs a) {
     const T* dO = head_ptr<T>(a, a.dout, s);
     T *dK = head_ptr<T>(a, a.dk, s), *dV = head_ptr<T>(a, a.dv, s);
     const u32 bh = (u32)(s.b * a.heads + s.h);
-    u32 k0 = 0, k1 = 0;
-    if (a.drop.thr) {
-        const u64 seed = (u64)*a.drop.seed;
-        k0 = (u32)seed;
-        k1 = (u32)(seed >> 32);
-    }
+    const Key2 key(a.drop);
     for (int n0 = s.blk * OWN; n0 < s.len; n0 += a.nblk * OWN) {
         const int j = n0 + wave * 32 + l31, jc = min(j, s.len - 1);
         const bool counts = j < kend && (even || !a.mask || a.mask[(long long)s.b * a.L + jc] != 0);
-        float4 kf[X::NF], vf[X::NF];
-        load_own<T>(kf, K, a.k.st, jc, h);
-        load_own<T>(vf, V, a.v.st, jc, h);
+        const bool all = __all(counts);
         f32x16 ok[2] = {zero16(), zero16()}, ov[2] = {zero16(), zero16()};
-        if (n0 < kend)
-            for (int i0 = 0; i0 < s.len; i0 += TR) {
-                const u64 bits = row_bits(i0, s.len);
-                __syncthreads();
-                stage<T>(sQ, Q, a.q.st, i0, bits);
-                stage<T>(sO, dO, a.dout.st, i0, bits);
+        if (n0 < kend) {
+            float4 kf[X::NF], vf[X::NF];
+            load_own<T>(kf, K, a.k.st, jc, h);
+            load_own<T>(vf, V, a.v.st, jc, h);
+            Stage<T> rq(Q, a.q.st), ro(dO, a.dout.st);
+            float rl = 0.0f, rd = 0.0f;
+            auto fetch = [&](int i0) {
+                const u64 rows = row_bits(i0, s.len);
+                rq.load(rows);
+                ro.load(rows);
                 if (threadIdx.x < TR) {
-                    const int i = i0 + threadIdx.x;
+                    const int i = i0 + (int)threadIdx.x;
                     // rows past the end: exp2(0 - inf) = 0
-                    sL[threadIdx.x] = i < s.len ? a.lse[s.stat + i] * 1.4426950408889634f : INFINITY;
-                    sD[threadIdx.x] = i < s.len ? a.delta[s.stat + i] : 0.0f;
+                    rl = i < s.len ? a.lse[s.stat + i] * 1.4426950408889634f : INFINITY;
+                    rd = i < s.len ? a.delta[s.stat + i] : 0.0f;
+                }
+            };
+            fetch(0);
+            for (int i0 = 0, buf = 0; i0 < s.len; i0 += TR, buf ^= 1) {
+                rq.store(sQ[buf]);
+                ro.store(sO[buf]);
+                if (threadIdx.x < TR) {
+                    sL[buf][threadIdx.x] = rl;
+                    sD[buf][threadIdx.x] = rd;
                 }
                 __syncthreads();
-#pragma unroll
+                if (i0 + TR < s.len) fetch(i0 + TR);
+#pragma unroll SUBU
                 for (int sub = 0; sub < 2; ++sub) {
-                    f32x16 sc = row_product<T>(sQ, sub * 32, kf, l31, h);
-                    f32x16 dp = row_product<T>(sO, sub * 32, vf, l31, h);
-                    const u32 keep = a.drop.thr ? keep16<false>(a.drop, k0, k1, bh, j, i0 + 32 * sub, h) : 0xFFFFu;
+                    f32x16 sc = even ? zero16() : row_product<T>(sQ[buf] + sub * 32 * X::PITCH + ln.frag<T>(), kf);
+                    f32x16 dp = row_product<T>(sO[buf] + sub * 32 * X::PITCH + ln.frag<T>(), vf);
+                    Draws w;
+                    if constexpr (DROP) w.keys(a.drop, key.k0, key.k1, bh, j, i0 + 32 * sub, h);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int row = sub * 32 + acc_row(r, h);
-                        float p = exp2_((even ? 0.0f : sc[r] * a.c2) - sL[row]);
-                        p = counts ? p : 0.0f;
-                        const bool kept = (keep >> r) & 1u;
-                        const float g = (kept ? dp[r] * a.drop.scale : 0.0f) - sD[row];
-                        sc[r] = kept ? p : 0.0f;
-                        dp[r] = counts && !even ? p * g : 0.0f;
+                    for (int g = 0; g < 4; ++g) {
+                        const float4 L4 = *reinterpret_cast<const float4*>(&sL[buf][sub * 32 + 8 * g + 4 * h]);
+                        const float4 D4 = *reinterpret_cast<const float4*>(&sD[buf][sub * 32 + 8 * g + 4 * h]);
+                        const float lv[4] = {L4.x, L4.y, L4.z, L4.w}, dv[4] = {D4.x, D4.y, D4.z, D4.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int r = 4 * g + e;
+                            const float p = exp2_(fmaf(sc[r], a.c2, -lv[e]));
+                            const bool kept = !DROP || w.kept_k(r);
+                            const float gr = !DROP ? dp[r] - dv[e] : fmaf(kept ? dp[r] : 0.0f, a.drop.scale, -dv[e]);
+                            sc[r] = kept ? p : 0.0f;
+                            dp[r] = p * gr;
+                        }
                     }
-                    col_product<T>(ov, sO, sub * 32, sc, lane);
-                    col_product<T>(ok, sQ, sub * 32, dp, lane);
+                    if (!all || even) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            sc[r] = counts ? sc[r] : 0.0f;
+                            dp[r] = counts && !even ? dp[r] : 0.0f;
+                        }
+                    }
+                    col_product<T>(ov, sO[buf] + sub * 32 * X::PITCH + ln.col<T>(), sc);
+                    col_product<T>(ok, sQ[buf] + sub * 32 * X::PITCH + ln.col<T>(), dp);
                 }
             }
+            __syncthreads();
+        }
         if (j < s.len) {
             store_own<T>(dK + (long long)j * a.dk.st, ok, a.scale, h);
             store_own<T>(dV + (long long)j * a.dv.st, ov, a.drop.scale, h);
@@ -523,6 +663,25 @@ int fill(const char* what, const otter_attention_args* x, AttnTrainArgs* a, long
     return OTTER_OK;
 }
 
+template <typename T>
+void launch_fwd(const AttnTrainArgs& a, int grid, hipStream_t st) {
+    if (a.drop.thr)
+        attn_fwd_kernel<T, true><<<grid, 256, 0, st>>>(a);
+    else
+        attn_fwd_kernel<T, false><<<grid, 256, 0, st>>>(a);
+}
+
+template <typename T>
+void launch_bwd(const AttnTrainArgs& a, int grid, hipStream_t st) {
+    if (a.drop.thr) {
+        attn_dq_kernel<T, true><<<grid, 256, 0, st>>>(a);
+        attn_dkv_kernel<T, true><<<grid, 256, 0, st>>>(a);
+    } else {
+        attn_dq_kernel<T, false><<<grid, 256, 0, st>>>(a);
+        attn_dkv_kernel<T, false><<<grid, 256, 0, st>>>(a);
+    }
+}
+
 }  // namespace
 
 extern "C" {
@@ -543,9 +702,9 @@ int otter_attention_forward(int device, const otter_attention_args* x, void* str
     const int grid = a.nblk * a.heads * a.B + (a.cu ? a.heads : 0);
     hipStream_t st = (hipStream_t)stream;
     if (size == 2)
-        attn_fwd_kernel<bf16_t><<<grid, 256, 0, st>>>(a);
+        launch_fwd<bf16_t>(a, grid, st);
     else
-        attn_fwd_kernel<float><<<grid, 256, 0, st>>>(a);
+        launch_fwd<float>(a, grid, st);
     OTTER_HIP_TRY(hipGetLastError());
     return OTTER_OK;
 }
@@ -583,13 +742,10 @@ int otter_attention_backward(int device, const otter_attention_args* x, void* st
     if (!g.ok) return set_err(OTTER_EHIP, "attention_backward: hipSetDevice(%d) failed", device);
     const int grid = a.nblk * a.heads * a.B + (a.cu ? a.heads : 0);
     hipStream_t st = (hipStream_t)stream;
-    if (size == 2) {
-        attn_dq_kernel<bf16_t><<<grid, 256, 0, st>>>(a);
-        attn_dkv_kernel<bf16_t><<<grid, 256, 0, st>>>(a);
-    } else {
-        attn_dq_kernel<float><<<grid, 256, 0, st>>>(a);
-        attn_dkv_kernel<float><<<grid, 256, 0, st>>>(a);
-    }
+    if (size == 2)
+        launch_bwd<bf16_t>(a, grid, st);
+    else
+        launch_bwd<float>(a, grid, st);
     OTTER_HIP_TRY(hipGetLastError());
     return OTTER_OK;
 }

@@ -15,13 +15,15 @@ struct Philox4 {
     u32 w[4];
 };
 
+__device__ __forceinline__ u32 xor3(u32 a, u32 b, u32 c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
+
 __device__ __forceinline__ Philox4 philox7(u32 c0, u32 c1, u32 c2, u32 c3, u32 k0, u32 k1) {
 #pragma unroll
     for (int r = 0; r < 7; ++r) {
         const u64 p0 = (u64)c0 * 0xD2511F53u, p1 = (u64)c2 * 0xCD9E8D57u;
-        c0 = (u32)(p1 >> 32) ^ c1 ^ k0;
+        c0 = xor3((u32)(p1 >> 32), c1, k0);
         c1 = (u32)p1;
-        c2 = (u32)(p0 >> 32) ^ c3 ^ k1;
+        c2 = xor3((u32)(p0 >> 32), c3, k1);
         c3 = (u32)p0;
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;
