@@ -132,11 +132,16 @@ struct Stage {
     long long st;
     __device__ __forceinline__ Stage(const T* base, long long stride) : p(base + (threadIdx.x / X::CH) * stride + (threadIdx.x % X::CH) * X::EPC), st(stride) {}
     __device__ __forceinline__ void load(u64 keep) {
-        const u64 mine = keep >> (threadIdx.x / X::CH);
+        if (~keep == 0) {                     // the usual tile: no lane is switched off
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if ((mine >> (i * STEP)) & 1) v[i] = *reinterpret_cast<const float4*>(p + i * STEP * st);
+            for (int i = 0; i < N; ++i) v[i] = *reinterpret_cast<const float4*>(p + i * STEP * st);
+        } else {
+            const u64 mine = keep >> (threadIdx.x / X::CH);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if ((mine >> (i * STEP)) & 1) v[i] = *reinterpret_cast<const float4*>(p + i * STEP * st);
+            }
         }
         p += TR * st;
     }
@@ -193,10 +198,9 @@ __device__ __forceinline__ void col_product(f32x16 (&o)[2], const char* t, const
             for (int d = 0; d < 2; ++d) {
                 // X^T[d][row], rows 16 s2 + 8 (j >> 2) + 4 h + (j & 3): two transposed reads of 4 rows x 16 columns
                 const char* p0 = t + s2 * 16 * P + d * 64;
-                const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)p0);
-                const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)(p0 + 8 * P));
-                const short va[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, va), wb, o[d], 0, 0, 0);
+                const s16x4 v[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)p0),
+                                    __builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)(p0 + 8 * P))};
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), wb, o[d], 0, 0, 0);
             }
         }
     } else {
@@ -225,6 +229,12 @@ __device__ __forceinline__ void negate(float4 (&f)[Tile<T>::NF]) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] ^= sign;
     }
+}
+
+template <typename T>
+__device__ __forceinline__ void zero_frags(float4 (&f)[Tile<T>::NF]) {
+#pragma unroll
+    for (int j = 0; j < Tile<T>::NF; ++j) f[j] = make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 // store o[2] (head dimension on the registers, row on the lane) times f
@@ -343,6 +353,8 @@ struct Key2 {
     }
 };
 
+// the larger one, a NaN if there is one (fmaxf would first quiet both operands, two instructions more)
+__device__ __forceinline__ float max_(float x, float y) { return __builtin_elementwise_maximum(x, y); }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ------------------------------------------------------------------ forward
@@ -372,13 +384,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? W_FWD : 2) void attn_fwd_kern
         float4 qf[X::NF];
         load_own<T>(qf, Q, a.q.st, min(i, s.len - 1), h);
         if (a.c2 < 0.0f) negate<T>(qf);
+        if (even) zero_frags<T>(qf);       // and zero keys below: every score is 0
         f32x16 o[2] = {zero16(), zero16()};
         float m = -INFINITY, base = 0.0f, l = 0.0f;   // base: m, or 0 while no score is above -inf
         KeyBits kb(a, s, even);
         Stage<T> rk(K, a.k.st), rv(V, a.v.st);
         kb.fetch(0);
         u64 next = kb.bits(0);
-        rk.load(next);
+        rk.load(even ? 0 : next);
         rv.load(next);
         kb.fetch(TR);
         for (int j0 = 0, buf = 0; j0 < kend; j0 += TR, buf ^= 1) {
@@ -388,14 +401,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? W_FWD : 2) void attn_fwd_kern
             __syncthreads();               // everyone is done with the other buffer, too
             if (j0 + TR < kend) {
                 next = kb.bits(j0 + TR);
-                rk.load(next);
+                rk.load(even ? 0 : next);
                 rv.load(next);
                 kb.fetch(j0 + 2 * TR);
             }
             if (bits == 0) continue;
             f32x16 sc[2];
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub) sc[sub] = even ? zero16() : row_product<T>(sK[buf] + sub * 32 * X::PITCH + ln.frag<T>(), qf);
+            for (int sub = 0; sub < 2; ++sub) sc[sub] = row_product<T>(sK[buf] + sub * 32 * X::PITCH + ln.frag<T>(), qf);
             if (~bits != 0) {
 #pragma unroll
                 for (int sub = 0; sub < 2; ++sub) {
@@ -404,13 +417,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? W_FWD : 2) void attn_fwd_kern
                     for (int r = 0; r < 16; ++r) sc[sub][r] = (kb32 >> acc_row(r, 0)) & 1u ? sc[sub][r] : -INFINITY;
                 }
             }
-            float mx = -INFINITY;
+            float mx = max_(sc[0][0], sc[1][0]);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fmaxf(sc[0][r], sc[1][r]));
-            mx = fmaxf(mx, __shfl_xor(mx, 32)) * c2;
+            for (int r = 1; r < 16; ++r) mx = max_(max_(sc[0][r], sc[1][r]), mx);
+            mx = max_(mx, __shfl_xor(mx, 32)) * c2;
             // mx > m + 8 or a NaN: move the maximum
             if (__any(!(mx <= m + 8.0f))) {
-                const float mnew = fmaxf(m, mx);
+                const float mnew = max_(m, mx);
                 base = mnew == -INFINITY ? 0.0f : mnew;
                 const float alpha = exp2_(m - base);
                 m = mnew;
@@ -558,11 +571,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? W_DKV : 2) void attn_dkv_kern
             float4 kf[X::NF], vf[X::NF];
             load_own<T>(kf, K, a.k.st, jc, h);
             load_own<T>(vf, V, a.v.st, jc, h);
+            if (even) zero_frags<T>(kf);       // and zero queries below: every score is 0
             Stage<T> rq(Q, a.q.st), ro(dO, a.dout.st);
             float rl = 0.0f, rd = 0.0f;
             auto fetch = [&](int i0) {
                 const u64 rows = row_bits(i0, s.len);
-                rq.load(rows);
+                rq.load(even ? 0 : rows);
                 ro.load(rows);
                 if (threadIdx.x < TR) {
                     const int i = i0 + (int)threadIdx.x;
@@ -583,7 +597,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? W_DKV : 2) void attn_dkv_kern
                 if (i0 + TR < s.len) fetch(i0 + TR);
 #pragma unroll SUBU
                 for (int sub = 0; sub < 2; ++sub) {
-                    f32x16 sc = even ? zero16() : row_product<T>(sQ[buf] + sub * 32 * X::PITCH + ln.frag<T>(), kf);
+                    f32x16 sc = row_product<T>(sQ[buf] + sub * 32 * X::PITCH + ln.frag<T>(), kf);
                     f32x16 dp = row_product<T>(sO[buf] + sub * 32 * X::PITCH + ln.frag<T>(), vf);
                     Draws w;
                     if constexpr (DROP) w.keys(a.drop, key.k0, key.k1, bh, j, i0 + 32 * sub, h);
