@@ -91,9 +91,9 @@ SIGNATURES = {
     "otter_layernorm_backward_workspace": (c_i64, [c_i64, c_int]),
     "otter_layernorm_backward": (c_int, [c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_int,
                                          ctypes.c_float, c_vp, ctypes.c_uint32, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
-    "otter_attention_forward": (c_int, [c_int, ctypes.POINTER(AttentionArgs), c_vp]),
-    "otter_attention_backward_workspace": (c_i64, [ctypes.POINTER(AttentionArgs)]),
-    "otter_attention_backward": (c_int, [c_int, ctypes.POINTER(AttentionArgs), c_vp]),
+    "otter_attention_forward": (c_int, [c_int, c_vp, c_vp]),
+    "otter_attention_backward_workspace": (c_i64, [c_vp]),
+    "otter_attention_backward": (c_int, [c_int, c_vp, c_vp]),
     "otter_encoder_out_dim": (c_int, [c_vp]),
     "otter_encoder_destroy": (None, [c_vp]),
 }

@@ -24,14 +24,6 @@ using namespace otter;
 
 constexpr int DH = 64;         // head dimension
 constexpr int TR = 64;         // rows of a streamed tile
-#ifndef SUBU
-#define SUBU 1
-#endif
-#ifndef W_FWD
-#define W_FWD 2
-#define W_DQ 2
-#define W_DKV 2
-#endif
 constexpr int OWN = 128;       // rows a workgroup owns: 4 waves x 32
 
 struct View {                  // element strides of a [batch, token, head, 64] tensor (batch stride unused when packed)
@@ -122,30 +114,33 @@ struct Lane {
 };
 
 // A tile on its way: 64 rows through the registers of the workgroup's 256 threads, loaded while the tile before it is
-// multiplied.  Rows that `keep` leaves out (a bit per row) become zeros and are not read.
+// multiplied.  Rows that `keep` leaves out (a bit per row) become zeros.
 template <typename T>
 struct Stage {
     using X = Tile<T>;
     static constexpr int N = TR * X::CH / 256, STEP = 256 / X::CH;   // loads a thread, rows between them
     float4 v[N];
-    const T* p;                 // this thread's first chunk of the next tile
+    u64 keep;
+    const T* p;                 // this thread's chunk of row 0
     long long st;
-    __device__ __forceinline__ Stage(const T* base, long long stride) : p(base + (threadIdx.x / X::CH) * stride + (threadIdx.x % X::CH) * X::EPC), st(stride) {}
-    __device__ __forceinline__ void load(u64 keep) {
-        if (~keep == 0) {                     // the usual tile: no lane is switched off
+    int row, last;              // this thread's first row of the next tile, the sequence's last row
+    __device__ __forceinline__ Stage(const T* base, long long stride, int len)
+        : p(base + (threadIdx.x % X::CH) * X::EPC), st(stride), row(threadIdx.x / X::CH), last(len - 1) {}
+    // No lane is switched off (a load inside a branch makes the compiler wait for the ones before it): rows past the end
+    // are read from the last one, and what `keep` leaves out is cleared on its way to LDS.
+    __device__ __forceinline__ void load(u64 bits) {
+        keep = bits;
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = *reinterpret_cast<const float4*>(p + i * STEP * st);
-        } else {
+        for (int i = 0; i < N; ++i) v[i] = *reinterpret_cast<const float4*>(p + min(row + i * STEP, last) * st);
+        row += TR;
+    }
+    __device__ __forceinline__ void store(char* lds) {
+        if (~keep != 0) {
             const u64 mine = keep >> (threadIdx.x / X::CH);
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if ((mine >> (i * STEP)) & 1) v[i] = *reinterpret_cast<const float4*>(p + i * STEP * st);
-            }
+            for (int i = 0; i < N; ++i)
+                if (!((mine >> (i * STEP)) & 1)) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        p += TR * st;
-    }
-    __device__ __forceinline__ void store(char* lds) const {
         char* d = lds + (threadIdx.x / X::CH) * X::PITCH + (threadIdx.x % X::CH) * 16;
 #pragma unroll
         for (int i = 0; i < N; ++i) *reinterpret_cast<float4*>(d + i * STEP * X::PITCH) = v[i];
@@ -363,7 +358,7 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 // probabilities then stay below 2^8 times their final size, harmless in float32 and for bfloat16's relative rounding), so
 // that the accumulators are rescaled once or twice a row and not at every tile.
 template <typename T, bool DROP>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? W_FWD : 2) void attn_fwd_kernel(AttnTrainArgs a) {
+__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnTrainArgs a) {
     using X = Tile<T>;
     __shared__ __attribute__((aligned(16))) char sK[2][X::BYTES];
     __shared__ __attribute__((aligned(16))) char sV[2][X::BYTES];
@@ -388,7 +383,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? W_FWD : 2) void attn_fwd_kern
         f32x16 o[2] = {zero16(), zero16()};
         float m = -INFINITY, base = 0.0f, l = 0.0f;   // base: m, or 0 while no score is above -inf
         KeyBits kb(a, s, even);
-        Stage<T> rk(K, a.k.st), rv(V, a.v.st);
+        Stage<T> rk(K, a.k.st, s.len), rv(V, a.v.st, s.len);
         kb.fetch(0);
         u64 next = kb.bits(0);
         rk.load(even ? 0 : next);
@@ -460,7 +455,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? W_FWD : 2) void attn_fwd_kern
 // ------------------------------------------------------------------ backward: dQ (and D)
 // The forward kernel's walk again: queries on the lanes, dS^T is the right operand of dQ^T = K^T dS^T.
 template <typename T, bool DROP>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? W_DQ : 2) void attn_dq_kernel(AttnTrainArgs a) {
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
     using X = Tile<T>;
     __shared__ __attribute__((aligned(16))) char sK[2][X::BYTES];
     __shared__ __attribute__((aligned(16))) char sV[2][X::BYTES];
@@ -495,7 +490,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? W_DQ : 2) void attn_dq_kernel
         f32x16 o[2] = {zero16(), zero16()};
         if (!even) {                                // even: dS = 0
             KeyBits kb(a, s, even);
-            Stage<T> rk(K, a.k.st), rv(V, a.v.st);
+            Stage<T> rk(K, a.k.st, s.len), rv(V, a.v.st, s.len);
             kb.fetch(0);
             u64 next = kb.bits(0);
             rk.load(next);
@@ -513,7 +508,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? W_DQ : 2) void attn_dq_kernel
                     kb.fetch(j0 + 2 * TR);
                 }
                 if (bits == 0) continue;
-#pragma unroll SUBU
+#pragma unroll (DROP ? 2 : 1)
                 for (int sub = 0; sub < 2; ++sub) {
                     f32x16 sc = row_product<T>(sK[buf] + sub * 32 * X::PITCH + ln.frag<T>(), qf);
                     const f32x16 dp = row_product<T>(sV[buf] + sub * 32 * X::PITCH + ln.frag<T>(), df);
@@ -542,7 +537,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? W_DQ : 2) void attn_dq_kernel
 // ------------------------------------------------------------------ backward: dK, dV
 // A workgroup owns 128 keys, a wave 32 (one on each lane of a half), and streams the queries in tiles of 64.
 template <typename T, bool DROP>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? W_DKV : 2) void attn_dkv_kernel(AttnTrainArgs a) {
+__global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
     using X = Tile<T>;
     __shared__ __attribute__((aligned(16))) char sQ[2][X::BYTES];
     __shared__ __attribute__((aligned(16))) char sO[2][X::BYTES];
@@ -572,30 +567,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? W_DKV : 2) void attn_dkv_kern
             load_own<T>(kf, K, a.k.st, jc, h);
             load_own<T>(vf, V, a.v.st, jc, h);
             if (even) zero_frags<T>(kf);       // and zero queries below: every score is 0
-            Stage<T> rq(Q, a.q.st), ro(dO, a.dout.st);
-            float rl = 0.0f, rd = 0.0f;
+            Stage<T> rq(Q, a.q.st, s.len), ro(dO, a.dout.st, s.len);
+            float rl, rd;
+            int ri;
             auto fetch = [&](int i0) {
                 const u64 rows = row_bits(i0, s.len);
                 rq.load(even ? 0 : rows);
                 ro.load(rows);
-                if (threadIdx.x < TR) {
-                    const int i = i0 + (int)threadIdx.x;
-                    // rows past the end: exp2(0 - inf) = 0
-                    rl = i < s.len ? a.lse[s.stat + i] * 1.4426950408889634f : INFINITY;
-                    rd = i < s.len ? a.delta[s.stat + i] : 0.0f;
-                }
+                ri = i0 + (int)threadIdx.x % TR;
+                rl = a.lse[s.stat + min(ri, s.len - 1)];
+                rd = a.delta[s.stat + min(ri, s.len - 1)];
             };
             fetch(0);
             for (int i0 = 0, buf = 0; i0 < s.len; i0 += TR, buf ^= 1) {
                 rq.store(sQ[buf]);
                 ro.store(sO[buf]);
-                if (threadIdx.x < TR) {
-                    sL[buf][threadIdx.x] = rl;
-                    sD[buf][threadIdx.x] = rd;
+                if (threadIdx.x < TR) {        // rows past the end: exp2(0 - inf) = 0
+                    sL[buf][threadIdx.x] = ri < s.len ? rl * 1.4426950408889634f : INFINITY;
+                    sD[buf][threadIdx.x] = ri < s.len ? rd : 0.0f;
                 }
                 __syncthreads();
                 if (i0 + TR < s.len) fetch(i0 + TR);
-#pragma unroll SUBU
+#pragma unroll (DROP ? 2 : 1)
                 for (int sub = 0; sub < 2; ++sub) {
                     f32x16 sc = row_product<T>(sQ[buf] + sub * 32 * X::PITCH + ln.frag<T>(), kf);
                     f32x16 dp = row_product<T>(sO[buf] + sub * 32 * X::PITCH + ln.frag<T>(), vf);

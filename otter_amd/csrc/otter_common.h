@@ -28,7 +28,12 @@ struct DeviceGuard {
     bool ok = false;
     explicit DeviceGuard(int device) {
         if (hipGetDevice(&prev) != hipSuccess) prev = -1;
-        ok = hipSetDevice(device) == hipSuccess;
+        if (prev == device) {             // the usual call: nothing to switch or to restore
+            prev = -1;
+            ok = true;
+        } else {
+            ok = hipSetDevice(device) == hipSuccess;
+        }
     }
     ~DeviceGuard() {
         if (prev >= 0) (void)hipSetDevice(prev);

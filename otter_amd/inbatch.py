@@ -21,6 +21,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 
+_stream = torch._C._cuda_getCurrentRawStream     # a device's current stream, without an object around it
+
 
 def inbatch_scores(q, c, neg_c=None):
     """q, c, neg_c: float32 [B, d] tensors on one GPU.  Returns (product float32 [B, B + (neg_c is not None)],
@@ -55,7 +57,8 @@ def _loss_operands(what, q, c, neg_c):
             what, tuple(q.shape), tuple(c.shape), None if neg_c is None else tuple(neg_c.shape)))
     if c.device != q.device or (neg_c is not None and neg_c.device != q.device):
         raise ValueError("%s: q, c and neg_c must be on one GPU" % what)
-    return [None if t is None else t.to(torch.float32).contiguous() for t in (q, c, neg_c)]
+    f32 = torch.float32
+    return [t if t is None or (t.dtype == f32 and t.is_contiguous()) else t.to(f32).contiguous() for t in (q, c, neg_c)]
 
 
 def inbatch_loss_forward(q, c, neg_c=None):
@@ -77,7 +80,7 @@ def inbatch_loss_forward(q, c, neg_c=None):
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
     _lib.check(lib.otter_inbatch_loss_forward(
         dev.index, q.data_ptr(), c.data_ptr(), None if neg_c is None else neg_c.data_ptr(), B, d, buf.data_ptr(), ld,
-        lse.data_ptr(), loss.data_ptr(), ws.data_ptr(), nbytes, torch.cuda.current_stream(dev).cuda_stream),
+        lse.data_ptr(), loss.data_ptr(), ws.data_ptr(), nbytes, _stream(dev.index)),
         "otter_inbatch_loss_forward")
     return loss, buf[:, :ncol], lse
 
@@ -102,7 +105,7 @@ def inbatch_loss_backward(dloss, q, c, neg_c, product, lse):
     _lib.check(lib.otter_inbatch_loss_backward(
         dev.index, dloss.data_ptr(), q.data_ptr(), c.data_ptr(), None if neg_c is None else neg_c.data_ptr(), B, d,
         product.data_ptr(), ld, lse.data_ptr(), dq.data_ptr(), dc.data_ptr(), None if dneg is None else dneg.data_ptr(),
-        torch.cuda.current_stream(dev).cuda_stream), "otter_inbatch_loss_backward")
+        _stream(dev.index)), "otter_inbatch_loss_backward")
     return dq, dc, dneg
 
 

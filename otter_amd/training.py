@@ -17,8 +17,8 @@ dropout of a step its own `call`, every step a new seed, and a backward call tho
 Under graph capture use the *_forward / *_backward calls.  (torch's own autograd engine ends the process when a backward
 pass is captured while an eager graph over the same leaves is alive; that is not particular to these operators.)
 """
-import ctypes
 import math
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -34,21 +34,21 @@ def new_seed(device=None, generator=None):
     return torch.randint(0, 2 ** 62, (1,), dtype=torch.int64, device=dev, generator=generator)
 
 
-def _on_gpu(what, **tensors):
-    """Every tensor on one GPU and of one supported dtype; returns (device, dtype code)."""
-    first = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not (torch.is_tensor(t) and t.is_cuda):
-            raise ValueError("%s: %s must be a tensor on a GPU (the HIP path has no CPU fallback)" % (what, name))
-        if first is None:
-            first = t
-            if t.dtype not in _DTYPES:
-                raise ValueError("%s: %s must be float32 or bfloat16, got %s" % (what, name, t.dtype))
-        elif t.device != first.device or t.dtype != first.dtype:
-            raise ValueError("%s: %s is %s on %s, expected %s on %s" % (what, name, t.dtype, t.device, first.dtype, first.device))
-    return first.device, _DTYPES[first.dtype]
+def _on_gpu(what, name, t):
+    """The tensor is on a GPU and of a supported dtype; returns (device, dtype code)."""
+    if not (torch.is_tensor(t) and t.is_cuda):
+        raise ValueError("%s: %s must be a tensor on a GPU (the HIP path has no CPU fallback)" % (what, name))
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError("%s: %s must be float32 or bfloat16, got %s" % (what, name, t.dtype))
+    return t.device, code
+
+
+def _like(what, name, t, first):
+    """t has the first tensor's shape, dtype and device."""
+    if not torch.is_tensor(t) or t.dtype != first.dtype or t.device != first.device or t.shape != first.shape:
+        raise ValueError("%s: %s must be like the first operand: expected %s %r on %s" % (
+            what, name, first.dtype, tuple(first.shape), first.device))
 
 
 def _seed_ptr(what, seed, dropout_p, dev):
@@ -68,18 +68,20 @@ def _call_id(what, call):
     return call
 
 
-def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+# The handle of a device's current stream; torch.cuda.current_stream() builds an object around it, which takes as long as a
+# small kernel.
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 # ------------------------------------------------------------------------------------------------------------ dropout
 def _dropout(what, x, p, seed, call, out=None):
     lib = _lib.load()
-    dev, dt = _on_gpu(what, x=x)
+    dev, dt = _on_gpu(what, "x", x)
     ptr = _seed_ptr(what, seed, p, dev)
     if p == 0.0:
         return x.clone() if out is None else out.copy_(x)
-    x = x.contiguous()
+    if not x.is_contiguous():
+        x = x.contiguous()
     cols = x.shape[-1] if x.dim() else 1
     rows = x.numel() // cols if cols else 0
     if out is None:
@@ -87,7 +89,7 @@ def _dropout(what, x, p, seed, call, out=None):
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError("%s: out must be a contiguous %s tensor of shape %r on %s" % (what, x.dtype, tuple(x.shape), dev))
     _lib.check(lib.otter_dropout(dev.index, dt, x.data_ptr(), out.data_ptr(), rows, cols, p, ptr, _call_id(what, call),
-                                 _stream(dev)), "otter_dropout")
+                                 _stream(dev.index)), "otter_dropout")
     return out
 
 
@@ -122,10 +124,11 @@ def dropout(x, p, seed, call=0):
 
 # --------------------------------------------------------------------------------------------------------- layer norm
 def _norm_args(what, x, weight, residual, dropout_p, seed, call):
-    dev, dt = _on_gpu(what, x=x, residual=residual)
-    if x.dim() < 1 or (residual is not None and residual.shape != x.shape):
-        raise ValueError("%s: x %r and residual %r must have one shape" % (
-            what, tuple(x.shape), None if residual is None else tuple(residual.shape)))
+    dev, dt = _on_gpu(what, "x", x)
+    if x.dim() < 1:
+        raise ValueError("%s: x has no dimension to normalise over" % what)
+    if residual is not None:
+        _like(what, "residual", residual, x)
     cols = x.shape[-1]
     if not (torch.is_tensor(weight) and weight.device == dev and weight.dtype in _DTYPES and tuple(weight.shape) == (cols,)):
         raise ValueError("%s: weight must be a float32 or bfloat16 tensor [%d] on %s" % (what, cols, dev))
@@ -139,8 +142,7 @@ def layer_norm_forward(x, weight, bias, eps=1e-5, residual=None, dropout_p=0.0, 
     lib = _lib.load()
     what = "layer_norm"
     dev, dt, wdt, rows, cols, ptr, call = _norm_args(what, x, weight, residual, dropout_p, seed, call)
-    if not (torch.is_tensor(bias) and bias.shape == weight.shape and bias.dtype == weight.dtype and bias.device == dev):
-        raise ValueError("%s: bias must be like weight" % what)
+    _like(what, "bias", bias, weight)
     x, weight, bias = x.contiguous(), weight.contiguous(), bias.contiguous()
     residual = None if residual is None else residual.contiguous()
     y = torch.empty_like(x)
@@ -148,7 +150,7 @@ def layer_norm_forward(x, weight, bias, eps=1e-5, residual=None, dropout_p=0.0, 
     rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
     _lib.check(lib.otter_layernorm_forward(
         dev.index, dt, wdt, x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(),
-        bias.data_ptr(), rows, cols, eps, dropout_p, ptr, call, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _stream(dev)),
+        bias.data_ptr(), rows, cols, eps, dropout_p, ptr, call, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _stream(dev.index)),
         "otter_layernorm_forward")
     return y, mean, rstd
 
@@ -159,8 +161,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd, residual=None, dropout_p=0.0,
     lib = _lib.load()
     what = "layer_norm_backward"
     dev, dt, wdt, rows, cols, ptr, call = _norm_args(what, x, weight, residual, dropout_p, seed, call)
-    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != dev:
-        raise ValueError("%s: dy must be like x" % what)
+    _like(what, "dy", dy, x)
     for name, t in (("mean", mean), ("rstd", rstd)):
         if t.dtype != torch.float32 or t.device != dev or t.numel() != rows or not t.is_contiguous():
             raise ValueError("%s: %s must be what layer_norm_forward returned for x" % (what, name))
@@ -168,7 +169,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd, residual=None, dropout_p=0.0,
     residual = None if residual is None else residual.contiguous()
     dx = torch.empty_like(x)
     dres = torch.empty_like(x) if residual is not None and dropout_p > 0.0 else None
-    dw, db = torch.empty_like(weight), torch.empty_like(weight)
+    dw, db = torch.empty((2, cols), dtype=weight.dtype, device=dev).unbind(0)
     nbytes = lib.otter_layernorm_backward_workspace(rows, cols)
     if nbytes < 0:
         _lib.check(int(nbytes), "otter_layernorm_backward_workspace")
@@ -176,7 +177,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd, residual=None, dropout_p=0.0,
     _lib.check(lib.otter_layernorm_backward(
         dev.index, dt, wdt, dy.data_ptr(), x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(),
         mean.data_ptr(), rstd.data_ptr(), rows, cols, dropout_p, ptr, call, dx.data_ptr(),
-        None if dres is None else dres.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), nbytes, _stream(dev)),
+        None if dres is None else dres.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), nbytes, _stream(dev.index)),
         "otter_layernorm_backward")
     return dx, (dx if dres is None and residual is not None else dres), dw, db
 
@@ -203,56 +204,64 @@ def layer_norm(x, weight, bias, eps=1e-5, residual=None, dropout_p=0.0, seed=Non
 
 
 # ---------------------------------------------------------------------------------------------------------- attention
+# otter_attention_args of include/otter_hip.h: the head, q k v out, lse, dout dq dk dv, workspace and its size
+_HEAD = struct.Struct("=5iI2fqQQQ")
+_VIEWS = struct.Struct("=16q")
+_TAIL = struct.Struct("=Qq")
+_NO_VIEWS = _VIEWS.pack(*(0,) * 16)
+
+
 def _aligned(t):
     """t itself if the kernels can read it in place: heads of 64 contiguous elements, 16-byte aligned data and strides."""
-    step = 16 // t.element_size()
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % step == 0 for s in t.stride()[:-1])
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    mask = 15 // t.element_size()
+    *outer, inner = t.stride()
+    bad = t.data_ptr() & 15
+    for x in outer:
+        bad |= x & mask
+    return t.clone(memory_format=torch.contiguous_format) if bad or inner != 1 else t
 
 
 def _view(t):
     s = t.stride()
-    return _lib.View(t.data_ptr(), s[0] if t.dim() == 4 else 0, s[-3], s[-2])
+    return (t.data_ptr(), s[0], s[1], s[2]) if len(s) == 4 else (t.data_ptr(), 0, s[0], s[1])
 
 
 def _attention_args(what, q, k, v, mask, cu_seqlens, max_seqlen, dropout_p, seed, call, scale):
-    """(ctypes arguments without the outputs, tensors to keep alive, lse shape)."""
-    dev, dt = _on_gpu(what, q=q, k=k, v=v)
+    """(packed head of the arguments, q, k, v as they are read, tensors to keep alive, device, lse shape)."""
+    dev, dt = _on_gpu(what, "q", q)
     packed = cu_seqlens is not None
-    if q.dim() != (3 if packed else 4) or k.shape != q.shape or v.shape != q.shape:
+    shape = q.shape
+    if len(shape) != (3 if packed else 4) or k.shape != shape or v.shape != shape:
         raise ValueError("%s: q, k and v must all be [%s, heads, 64]; got %r %r %r" % (
-            what, "total" if packed else "batch, tokens", tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    if q.shape[-2] < 1:
+            what, "total" if packed else "batch, tokens", tuple(shape), tuple(k.shape), tuple(v.shape)))
+    _like(what, "k", k, q)
+    _like(what, "v", v, q)
+    heads, dim = shape[-2], shape[-1]
+    if heads < 1:
         raise ValueError("%s: no heads" % what)
     if packed and mask is not None:
         raise ValueError("%s: a key mask and packed sequences exclude each other" % what)
-    keep = [_aligned(q), _aligned(k), _aligned(v)]
-    a = _lib.AttentionArgs()
-    a.dtype, a.heads, a.head_dim = dt, q.shape[-2], q.shape[-1]
-    a.call, a.dropout_p = _call_id(what, call), dropout_p
-    a.scale = 1.0 / math.sqrt(max(1, q.shape[-1])) if scale is None else scale
-    a.seed = _seed_ptr(what, seed, dropout_p, dev)
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    seed_ptr, call = _seed_ptr(what, seed, dropout_p, dev) or 0, _call_id(what, call)
+    if scale is None:
+        scale = 1.0 / math.sqrt(max(1, dim))
     if packed:
         if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.device != dev:
             raise ValueError("%s: cu_seqlens must be int32 [batch + 1] on %s" % (what, dev))
         cu_seqlens = cu_seqlens.contiguous()
-        keep.append(cu_seqlens)
         if max_seqlen is None:
             max_seqlen = int(cu_seqlens.diff().max()) if cu_seqlens.numel() > 1 else 0
-        a.batch, a.tokens, a.total = cu_seqlens.numel() - 1, max(0, int(max_seqlen)), q.shape[0]
-        a.cu_seqlens = cu_seqlens.data_ptr()
-        lse_shape = (q.shape[1], q.shape[0])
-    else:
-        a.batch, a.tokens = q.shape[0], q.shape[1]
-        if mask is not None:
-            if not torch.is_tensor(mask) or tuple(mask.shape) != (q.shape[0], q.shape[1]) or mask.device != dev:
-                raise ValueError("%s: mask must be [%d, %d] on %s" % (what, q.shape[0], q.shape[1], dev))
-            mask = (mask if mask.dtype == torch.int64 else (mask != 0).to(torch.int64)).contiguous()
-            keep.append(mask)
-            a.mask = mask.data_ptr()
-        lse_shape = (q.shape[0], q.shape[2], q.shape[1])
-    a.q, a.k, a.v = _view(keep[0]), _view(keep[1]), _view(keep[2])
-    return a, keep, dev, lse_shape
+        head = _HEAD.pack(dt, cu_seqlens.numel() - 1, max(0, int(max_seqlen)), heads, dim, call, scale, dropout_p, shape[0], 0,
+                          cu_seqlens.data_ptr(), seed_ptr)
+        return head, q, k, v, cu_seqlens, dev, (heads, shape[0])
+    mask_ptr = 0
+    if mask is not None:
+        if not torch.is_tensor(mask) or mask.shape != shape[:2] or mask.device != dev:
+            raise ValueError("%s: mask must be [%d, %d] on %s" % (what, shape[0], shape[1], dev))
+        mask = (mask if mask.dtype == torch.int64 else (mask != 0).to(torch.int64)).contiguous()
+        mask_ptr = mask.data_ptr()
+    head = _HEAD.pack(dt, shape[0], shape[1], heads, dim, call, scale, dropout_p, 0, mask_ptr, 0, seed_ptr)
+    return head, q, k, v, mask, dev, (shape[0], heads, shape[1])
 
 
 def attention_forward(q, k, v, mask=None, cu_seqlens=None, max_seqlen=None, dropout_p=0.0, seed=None, call=0, scale=None):
@@ -265,11 +274,13 @@ def attention_forward(q, k, v, mask=None, cu_seqlens=None, max_seqlen=None, drop
     Views of a fused projection, qkv.unbind(-3), are read in place.  scale: 1 / 8 by default.
     lse (float32 [batch, heads, tokens] / [heads, total]) is what the backward pass needs."""
     lib = _lib.load()
-    a, keep, dev, lse_shape = _attention_args("attention", q, k, v, mask, cu_seqlens, max_seqlen, dropout_p, seed, call, scale)
+    head, q, k, v, keep, dev, lse_shape = _attention_args("attention", q, k, v, mask, cu_seqlens, max_seqlen, dropout_p, seed,
+                                                          call, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty(lse_shape, dtype=torch.float32, device=dev)
-    a.out, a.lse = _view(out), lse.data_ptr()
-    _lib.check(lib.otter_attention_forward(dev.index, ctypes.byref(a), _stream(dev)), "otter_attention_forward")
+    args = b"".join((head, _VIEWS.pack(*_view(q), *_view(k), *_view(v), *_view(out)), lse.data_ptr().to_bytes(8, "little"),
+                     _NO_VIEWS, _TAIL.pack(0, 0)))
+    _lib.check(lib.otter_attention_forward(dev.index, args, _stream(dev.index)), "otter_attention_forward")
     return out, lse
 
 
@@ -279,28 +290,30 @@ def attention_backward(dout, q, k, v, out, lse, mask=None, cu_seqlens=None, max_
     write them to, for instance the views dqkv.unbind(-3) of one buffer."""
     lib = _lib.load()
     what = "attention_backward"
-    a, keep, dev, lse_shape = _attention_args(what, q, k, v, mask, cu_seqlens, max_seqlen, dropout_p, seed, call, scale)
-    for name, t in (("dout", dout), ("out", out)):
-        if t.shape != q.shape or t.dtype != q.dtype or t.device != dev:
-            raise ValueError("%s: %s must be like q" % (what, name))
-    if tuple(lse.shape) != lse_shape or lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous():
+    head, q, k, v, keep, dev, lse_shape = _attention_args(what, q, k, v, mask, cu_seqlens, max_seqlen, dropout_p, seed, call,
+                                                          scale)
+    _like(what, "dout", dout, q)
+    _like(what, "out", out, q)
+    if lse.shape != lse_shape or lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous():
         raise ValueError("%s: lse must be what attention_forward returned" % what)
     dout, out = _aligned(dout), _aligned(out)
     if grads is None:
-        grads = tuple(torch.empty(q.shape, dtype=q.dtype, device=dev) for _ in range(3))
+        grads = torch.empty((3,) + q.shape, dtype=q.dtype, device=dev).unbind(0)
     else:
         for t in grads:
             if t.shape != q.shape or t.dtype != q.dtype or t.device != dev or _aligned(t) is not t:
                 raise ValueError("%s: grads must be like q, their heads contiguous, data and strides multiples of 16 bytes" % what)
-    a.out, a.lse, a.dout = _view(out), lse.data_ptr(), _view(dout)
-    a.dq, a.dk, a.dv = (_view(t) for t in grads)
-    nbytes = lib.otter_attention_backward_workspace(ctypes.byref(a))
+    dq, dk, dv = grads
+    views = _VIEWS.pack(*_view(q), *_view(k), *_view(v), *_view(out))
+    lse_ptr = lse.data_ptr().to_bytes(8, "little")
+    nbytes = lib.otter_attention_backward_workspace(b"".join((head, views, lse_ptr, _NO_VIEWS, _TAIL.pack(0, 0))))
     if nbytes < 0:
         _lib.check(int(nbytes), "otter_attention_backward_workspace")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    _lib.check(lib.otter_attention_backward(dev.index, ctypes.byref(a), _stream(dev)), "otter_attention_backward")
-    return tuple(grads)
+    args = b"".join((head, views, lse_ptr, _VIEWS.pack(*_view(dout), *_view(dq), *_view(dk), *_view(dv)),
+                     _TAIL.pack(ws.data_ptr(), nbytes)))
+    _lib.check(lib.otter_attention_backward(dev.index, args, _stream(dev.index)), "otter_attention_backward")
+    return dq, dk, dv
 
 
 class _Attention(torch.autograd.Function):
