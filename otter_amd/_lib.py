@@ -83,8 +83,9 @@ SIGNATURES = {
     "otter_ln_stats": (c_int, [c_int, c_vp, c_int, c_i64, c_int, ctypes.c_float, c_vp, c_vp]),
     "otter_inbatch_loss_workspace": (c_i64, [c_int, c_int]),
     "otter_inbatch_loss_forward": (c_int, [c_int, c_vp, c_vp, c_vp, c_int, c_int, c_vp, c_int, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "otter_inbatch_loss_backward_workspace": (c_i64, [c_int, c_int]),
     "otter_inbatch_loss_backward": (c_int, [c_int, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_vp, c_int, c_vp, c_vp, c_vp, c_vp,
-                                            c_vp]),
+                                            c_vp, c_i64, c_vp]),
     "otter_dropout": (c_int, [c_int, c_int, c_vp, c_vp, c_i64, c_i64, ctypes.c_float, c_vp, ctypes.c_uint32, c_vp]),
     "otter_layernorm_forward": (c_int, [c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_int, ctypes.c_float,
                                         ctypes.c_float, c_vp, ctypes.c_uint32, c_vp, c_vp, c_vp, c_vp]),

@@ -4,9 +4,11 @@
 //   S = [q c^T | q . neg]  (B x B | B x 1),  lse_i = log sum_j exp S_ij,  loss = mean_i (lse_i - S_ii)
 //   G = (exp(S - lse) - 1[j = i]) dloss / B,  dq = G c + G_neg neg,  dc = G^T q,  dneg = G_neg q
 //
-// All three products are float32 products on v_mfma_f32_32x32x2_f32 (an fma chain: no operand is rounded).  S is kept
-// (4 B^2 bytes, read twice) instead of multiplied out again in the backward pass (2 B^2 d flops); G is never stored, it is
-// made from S and lse where a product's tile is loaded.
+// Small batches: the three products run on v_mfma_f32_32x32x2_f32 (an fma chain: no operand is rounded), G is made from S and
+// lse where a product's tile is loaded.  Large ones: every operand is split into two float16 planes, x = (hi + lo) 2^-e with
+// hi + lo good to 22 bits, and hi hi' + hi lo' + lo hi' run on v_mfma_f32_32x32x16_f16, sixteen times float32's rate for
+// three times its products.  What that leaves out is at most 3 2^-22 of each |term|, less than the float32 sums' own rounding
+// over a row of 64 and more.  S is kept (4 B^2 bytes) instead of multiplied out again in the backward pass (2 B^2 d flops).
 #include "otter_common.h"
 #include "otter_device.h"
 
@@ -202,25 +204,37 @@ __device__ __forceinline__ void online(float& m, float& l, float m2, float l2) {
     m = n;
 }
 
-// one workgroup a row: the pieces of S summed in order, the hard negative's score, lse and the row's loss
+// one workgroup a row: the pieces of S summed in order (PIECES), the hard negative's score, lse and the row's loss
+template <bool PIECES>
 __global__ __launch_bounds__(256) void loss_rows_kernel(LossArgs a) {
     __shared__ float sm[4], sl[4], sd[4];
     const int i = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float* row = a.scores + (long long)i * a.ld;
     float m = -INFINITY, l = 0.0f;
-    for (int j = threadIdx.x; j < a.B; j += 256) {
-        float s;
-        if (a.splits > 1) {
-            s = 0.0f;
+    if constexpr (PIECES) {
+        for (int j = threadIdx.x; j < a.B; j += 256) {
+            float s = 0.0f;
+#pragma unroll 12
             for (int p = 0; p < a.splits; ++p) s += a.part[((size_t)p * a.B + i) * a.B + j];
             row[j] = s;
-        } else {
-            s = row[j];
+            online(m, l, s, 1.0f);
         }
-        online(m, l, s, 1.0f);
+    } else {
+        // four scores a load: one exponential each and one for the four's maximum
+#pragma unroll 2
+        for (int j = threadIdx.x * 4; j < a.B; j += 1024) {
+            f4u v = load4(row, 0, 1, a.B, 0, j);
+#pragma unroll
+            for (int e = 1; e < 4; ++e)
+                if (j + e >= a.B) v[e] = -INFINITY;
+            const float top = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), n = fmaxf(m, top), base = n == -INFINITY ? 0.0f : n;
+            l = l * __expf(m - base) + ((__expf(v[0] - base) + __expf(v[1] - base)) + (__expf(v[2] - base) + __expf(v[3] - base)));
+            m = n;
+        }
     }
     float dot = 0.0f;
     if (a.neg)
+#pragma unroll 4
         for (int e = threadIdx.x; e < a.d; e += 256) dot = fmaf(a.q[(long long)i * a.d + e], a.neg[(long long)i * a.d + e], dot);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -294,6 +308,270 @@ __global__ __launch_bounds__(256) void loss_grad_kernel(LossArgs a) {
     }
 }
 
+// ------------------------------------------------------------------ two float16 planes
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef u32 u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int SB = 32;             // contraction depth of a staged tile
+constexpr int NMAX = 256;          // workgroups of the pass for the largest element
+
+struct SplitArgs {
+    const float *q, *c;            // [B][d]
+    unsigned short* plane[4];      // q hi, q lo, c hi, c lo: [Bp][dp], zeros outside [B][d]
+    float *qs, *cs;                // [Bp]: what a row of the planes is to be multiplied by (forward)
+    float* top;                    // [2][NMAX] largest elements (backward: one scale a matrix)
+    int B, d, Bp, dp;
+};
+
+// 2^(14 - exponent of top): the largest element then lies in [2^14, 2^15), the smallest half step of a float16 (2^-25) is
+// 2^-39 of it.  Exact in both directions.
+__device__ __forceinline__ float plane_scale(float top) {
+    const int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+    return top > 0.0f && e < 128 ? __uint_as_float((u32)(min(max(14 - e, -126), 126) + 127) << 23) : 1.0f;
+}
+
+__device__ __forceinline__ void split1(float x, unsigned short& hi, unsigned short& lo) {
+    const _Float16 h = (_Float16)x;
+    const _Float16 l = (_Float16)(x - (float)h);
+    hi = __builtin_bit_cast(unsigned short, h);
+    lo = __builtin_bit_cast(unsigned short, l);
+}
+
+__global__ __launch_bounds__(256) void loss_top_kernel(SplitArgs a) {
+    __shared__ float red[4];
+    const float* x = blockIdx.y ? a.c : a.q;
+    const long long n = (long long)a.B * a.d;
+    float t = 0.0f;
+    // four elements a load, four loads in flight; the last n % 4 by the first threads
+    const long long n4 = n / 4, step = (long long)gridDim.x * 256;
+    const long long first = (long long)blockIdx.x * 256 + threadIdx.x;
+#pragma unroll 4
+    for (long long i = first; i < n4; i += step) {
+        const f4u v = *reinterpret_cast<const f4u*>(x + 4 * i);
+        t = fmaxf(t, fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+    }
+    if (4 * n4 + first < n) t = fmaxf(t, fabsf(x[4 * n4 + first]));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = t;
+    __syncthreads();
+    if (threadIdx.x == 0) a.top[blockIdx.y * NMAX + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// one wave a row of one matrix; WHOLE: the scale of the whole matrix, otherwise the row's own
+template <bool WHOLE>
+__global__ __launch_bounds__(256) void loss_split_kernel(SplitArgs a) {
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, m = blockIdx.y;
+    if (row >= a.Bp) return;
+    const float* x = (m ? a.c : a.q) + (long long)row * a.d;
+    float t = 0.0f;
+    if (WHOLE) {
+        for (int i = lane; i < NMAX; i += 64) t = fmaxf(t, a.top[m * NMAX + i]);
+    } else if (row < a.B) {
+        for (int i = lane; i < a.d; i += 64) t = fmaxf(t, fabsf(x[i]));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o));
+    const float f = plane_scale(t);
+    unsigned short *hi = a.plane[2 * m] + (long long)row * a.dp, *lo = a.plane[2 * m + 1] + (long long)row * a.dp;
+    for (int i = lane; i < a.dp / 4; i += 64) {
+        const f4u v = load4(m ? a.c : a.q, a.d, a.B, a.d, row, 4 * i);
+        unsigned short h[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split1(v[e] * f, h[e], l[e]);
+        __builtin_memcpy(hi + 4 * i, h, 8);
+        __builtin_memcpy(lo + 4 * i, l, 8);
+    }
+    if (lane == 0 && !WHOLE) (m ? a.cs : a.qs)[row] = 1.0f / f;
+}
+
+// G 2^14 as two planes [Bp][Bp], zeros outside [B][B]
+__global__ __launch_bounds__(256) void loss_gplanes_kernel(LossArgs a, unsigned short* hi, unsigned short* lo, int Bp) {
+    const int i = blockIdx.y, j = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (j >= Bp) return;
+    const Grad G{a.scores, a.lse, a.ld, a.B, 16384.0f};
+    const f4u v = G(i, j);
+    unsigned short h[4], l[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split1(v[e], h[e], l[e]);
+    __builtin_memcpy(hi + (long long)i * Bp + j, h, 8);
+    __builtin_memcpy(lo + (long long)i * Bp + j, l, 8);
+}
+
+// A tile of one operand, both planes, on its way to LDS.  KC: SB contiguous k of W rows (80 bytes a row in LDS); otherwise W
+// contiguous elements of SB k-rows (32 bytes of padding a row).  Neither the straight nor the transposed reads conflict.
+template <int W, bool KC>
+struct Planes {
+    static constexpr int PITCH = KC ? SB * 2 + 16 : W * 2 + 32;
+    static constexpr int BYTES = (KC ? W : SB) * PITCH;          // one plane
+    static constexpr int N = W * SB * 2 / 16 / 256;              // 16-byte chunks a thread and plane
+    static constexpr int CH = KC ? SB / 8 : W / 8;               // chunks a row
+    u32x4 v[2][N];
+    __device__ __forceinline__ void load(const unsigned short* hi, const unsigned short* lo, long long ld, int w0, int k0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int t = threadIdx.x + 256 * i, r = t / CH, c = t % CH;
+            const long long at = (long long)(KC ? w0 + r : k0 + r) * ld + (KC ? k0 : w0) + 8 * c;
+            v[0][i] = *reinterpret_cast<const u32x4*>(hi + at);
+            v[1][i] = *reinterpret_cast<const u32x4*>(lo + at);
+        }
+    }
+    __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int t = threadIdx.x + 256 * i;
+                *reinterpret_cast<u32x4*>(lds + p * BYTES + (t / CH) * PITCH + (t % CH) * 16) = v[p][i];
+            }
+    }
+    // 8 values of k for row w0 + (lane & 31): k = 16 s + 8 h + (0 .. 7) where both operands are KC, otherwise the order of the
+    // transposed reads, k = 16 s + 4 h + (0 .. 3) and 8 more
+    template <bool BOTH>
+    static __device__ __forceinline__ f16x8 frag(const char* plane, int w0, int s, int lane) {
+        const int h = lane >> 5, l31 = lane & 31;
+        if constexpr (KC) {
+            const char* p = plane + (w0 + l31) * PITCH + s * 32;
+            if constexpr (BOTH) return *reinterpret_cast<const f16x8*>(p + h * 16);
+            const s16x4 x[2] = {*reinterpret_cast<const s16x4*>(p + h * 8), *reinterpret_cast<const s16x4*>(p + 16 + h * 8)};
+            return __builtin_bit_cast(f16x8, x);
+        } else {
+            const int i16 = lane & 15;
+            const char* p = plane + (16 * s + 4 * h + (i16 >> 2)) * PITCH + (w0 + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3)) * 2;
+            const s16x4 x[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)p),
+                                __builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)(p + 8 * PITCH))};
+            return __builtin_bit_cast(f16x8, x);
+        }
+    }
+};
+
+// acc += A B^T over k in [0, K): 4 waves as 2 x 2, a wave 64 x (BN / 2); lds: both operands' planes, one stage (two stages
+// would halve the workgroups of a CU, which are what hides the loads)
+template <int BN, bool AKC, bool BKC>
+__device__ __forceinline__ void product16(f32x16 (&acc)[2][BN / 64], const unsigned short* Ahi, const unsigned short* Alo,
+                                          long long lda, const unsigned short* Bhi, const unsigned short* Blo, long long ldb, int m0,
+                                          int n0, int K, char* lds) {
+    constexpr int NB = BN / 64;
+    constexpr bool BOTH = AKC && BKC;
+    typedef Planes<128, AKC> PA;
+    typedef Planes<BN, BKC> PB;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = (wave >> 1) * 64, wn = (wave & 1) * (BN / 2);
+    char* sA = lds;
+    char* sB = lds + 2 * PA::BYTES;
+    PA ra;
+    PB rb;
+    ra.load(Ahi, Alo, lda, m0, 0);
+    rb.load(Bhi, Blo, ldb, n0, 0);
+    for (int k0 = 0; k0 < K; k0 += SB) {
+        __syncthreads();
+        ra.store(sA);
+        rb.store(sB);
+        __syncthreads();
+        if (k0 + SB < K) {
+            ra.load(Ahi, Alo, lda, m0, k0 + SB);
+            rb.load(Bhi, Blo, ldb, n0, k0 + SB);
+        }
+#pragma unroll
+        for (int s = 0; s < SB / 16; ++s) {
+            f16x8 ah[2], al[2], bh[NB], bl[NB];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                ah[i] = PA::template frag<BOTH>(sA, wm + 32 * i, s, lane);
+                al[i] = PA::template frag<BOTH>(sA + PA::BYTES, wm + 32 * i, s, lane);
+            }
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                bh[n] = PB::template frag<BOTH>(sB, wn + 32 * n, s, lane);
+                bl[n] = PB::template frag<BOTH>(sB + PB::BYTES, wn + 32 * n, s, lane);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int n = 0; n < NB; ++n) acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[n], acc[i][n], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int n = 0; n < NB; ++n) acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[n], acc[i][n], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int n = 0; n < NB; ++n) acc[i][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[n], acc[i][n], 0, 0, 0);
+        }
+    }
+}
+
+template <int BN, typename F>
+__device__ __forceinline__ void each16(const f32x16 (&acc)[2][BN / 64], int m0, int n0, const F& out) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, l31 = lane & 31;
+    const int wm = (wave >> 1) * 64, wn = (wave & 1) * (BN / 2);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int n = 0; n < BN / 64; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                out(m0 + wm + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * h, n0 + wn + 32 * n + l31, acc[i][n][r]);
+}
+
+template <int NB>
+__device__ __forceinline__ void clear16(f32x16 (&acc)[2][NB]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][n][r] = 0.0f;
+}
+
+__global__ __launch_bounds__(256, 2) void loss_scores16_kernel(LossArgs a, SplitArgs s) {
+    __shared__ __attribute__((aligned(16))) char lds[4 * Planes<128, true>::BYTES];
+    const int nt = s.Bp / 128, t = xcd_remap(blockIdx.x, gridDim.x);
+    const int m0 = (t / nt) * 128, n0 = (t % nt) * 128;
+    f32x16 acc[2][2];
+    clear16<2>(acc);
+    product16<128, true, true>(acc, s.plane[0], s.plane[1], s.dp, s.plane[2], s.plane[3], s.dp, m0, n0, s.dp, lds);
+    each16<128>(acc, m0, n0, [&](int i, int j, float v) {
+        if (i < a.B && j < a.B) a.scores[(long long)i * a.ld + j] = v * s.qs[i] * s.cs[j];
+    });
+}
+
+// dq and dc, half the grid each
+__global__ __launch_bounds__(256, 2) void loss_grad16_kernel(LossArgs a, SplitArgs s, const unsigned short* ghi, const unsigned short* glo) {
+    constexpr int LDS1 = 2 * Planes<128, true>::BYTES, LDS2 = 2 * Planes<128, false>::BYTES;
+    __shared__ __attribute__((aligned(16))) char lds[(LDS1 > LDS2 ? LDS1 : LDS2) + 2 * Planes<64, false>::BYTES];
+    const int nt = (a.d + 63) / 64, half = gridDim.x / 2, id = xcd_remap(blockIdx.x, gridDim.x);
+    const bool second = id >= half;
+    const int t = second ? id - half : id, m0 = (t / nt) * 128, n0 = (t % nt) * 64;
+    float top = 0.0f;
+    for (int i = threadIdx.x & 63; i < NMAX; i += 64) top = fmaxf(top, s.top[(second ? 0 : NMAX) + i]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float g = *a.dloss / (float)a.B, back = 1.0f / plane_scale(top), gback = g / 16384.0f;
+    f32x16 acc[2][1];
+    clear16<1>(acc);
+    if (second) {
+        product16<64, false, false>(acc, ghi, glo, s.Bp, s.plane[0], s.plane[1], s.dp, m0, n0, s.Bp, lds);
+        each16<64>(acc, m0, n0, [&](int j, int n, float v) {
+            if (j < a.B && n < a.d) a.dc[(long long)j * a.d + n] = v * back * gback;
+        });
+    } else {
+        product16<64, true, false>(acc, ghi, glo, s.Bp, s.plane[2], s.plane[3], s.dp, m0, n0, s.Bp, lds);
+        each16<64>(acc, m0, n0, [&](int i, int n, float v) {
+            if (i >= a.B || n >= a.d) return;
+            const long long at = (long long)i * a.d + n;
+            v *= back;
+            v *= gback;
+            if (a.neg) {
+                const float gn = __expf(a.scores[(long long)i * a.ld + a.B] - a.lse[i]) * g;
+                v = fmaf(gn, a.neg[at], v);
+                a.dneg[at] = gn * a.q[at];
+            }
+            a.dq[at] = v;
+        });
+    }
+}
+
 // ------------------------------------------------------------------ host side
 int check_loss(const char* what, int B, int d, int ld, int ncol) {
     if (B < 1 || d < 1) return set_err(OTTER_EINVAL, "%s: bad B=%d d=%d (the mean over no rows is undefined)", what, B, d);
@@ -303,14 +581,72 @@ int check_loss(const char* what, int B, int d, int ld, int ncol) {
 }
 
 // pieces of d so that a small batch still has work for the chip: at least 64 of d each
-int loss_splits(int B, int d, int bm) {
-    const long long tiles = (long long)((B + bm - 1) / bm) * ((B + bm - 1) / bm);
-    int s = (int)(tiles < 256 ? 256 / tiles : 1);
-    const int most = (d + 63) / 64;
-    return s < most ? (s < 1 ? 1 : s) : most;
+int loss_splits(int B, int d) {
+    const long long tiles = (long long)((B + 63) / 64) * ((B + 63) / 64);
+    const int s = (int)(tiles < 256 ? 256 / tiles : 1), most = (d + 63) / 64;
+    return s < most ? s : most;
 }
 
-int loss_tile(int B) { return B > 512 ? 128 : 64; }
+// Two float16 planes or float32: the planes cost two passes over the operands, and over G in the backward pass.
+bool loss_planes(int B, int d) { return B > 512 && d >= 64; }
+
+int64_t align16(int64_t x) { return (x + 15) / 16 * 16; }
+
+struct Take {                      // pieces of a workspace, 16-byte aligned
+    char* p;
+    int64_t used = 0;
+    template <typename X>
+    X* operator()(int64_t n) {
+        X* r = reinterpret_cast<X*>(p + used);
+        used += align16(n * (int64_t)sizeof(X));
+        return r;
+    }
+};
+
+void take_planes(Take& t, SplitArgs& s) {
+    for (auto& x : s.plane) x = t.template operator()<unsigned short>((int64_t)s.Bp * s.dp);
+}
+
+SplitArgs split_args(const float* q, const float* c, int B, int d) {
+    SplitArgs s = {};
+    s.q = q;
+    s.c = c;
+    s.B = B;
+    s.d = d;
+    s.Bp = round_up(B, 128);
+    s.dp = round_up(d, 64);
+    return s;
+}
+
+// the pieces of either workspace, and its size
+int64_t lay_forward(void* ws, LossArgs& a, SplitArgs& s) {
+    Take t{(char*)ws};
+    a.rowloss = t.template operator()<float>(a.B);
+    if (loss_planes(a.B, a.d)) {
+        s.qs = t.template operator()<float>(s.Bp);
+        s.cs = t.template operator()<float>(s.Bp);
+        take_planes(t, s);
+    } else if (a.splits > 1) {
+        a.part = t.template operator()<float>((int64_t)a.splits * a.B * a.B);
+    }
+    return t.used;
+}
+
+int64_t lay_backward(void* ws, SplitArgs& s, unsigned short** g) {
+    Take t{(char*)ws};
+    if (!loss_planes(s.B, s.d)) return 0;
+    s.top = t.template operator()<float>(2 * NMAX);
+    take_planes(t, s);
+    g[0] = t.template operator()<unsigned short>((int64_t)s.Bp * s.Bp);
+    g[1] = t.template operator()<unsigned short>((int64_t)s.Bp * s.Bp);
+    return t.used;
+}
+
+int check_workspace(const char* what, const void* ws, int64_t have, int64_t need) {
+    if (need > 0 && (!ws || have < need || ((uintptr_t)ws & 15)))
+        return set_err(OTTER_EINVAL, "%s: workspace of %lld bytes, needs %lld, 16-byte aligned", what, (long long)have, (long long)need);
+    return OTTER_OK;
+}
 
 }  // namespace
 
@@ -319,19 +655,20 @@ extern "C" {
 int64_t otter_inbatch_loss_workspace(int B, int d) {
     const int rc = check_loss("inbatch_loss_workspace", B, d, 0, 0);
     if (rc) return rc;
-    const int s = loss_splits(B, d, loss_tile(B));
-    return (int64_t)sizeof(float) * (B + (s > 1 ? (int64_t)s * B * B : 0));
+    LossArgs a = {};
+    a.B = B;
+    a.d = d;
+    a.splits = loss_splits(B, d);
+    SplitArgs s = split_args(nullptr, nullptr, B, d);
+    return lay_forward(nullptr, a, s);
 }
 
 int otter_inbatch_loss_forward(int device, const float* q, const float* c, const float* neg_c, int B, int d, float* scores,
                                int ld, float* lse, float* loss, void* workspace, int64_t workspace_bytes, void* stream) {
     int rc = check_loss("inbatch_loss_forward", B, d, ld, B + (neg_c ? 1 : 0));
     if (rc) return rc;
-    if (!q || !c || !scores || !lse || !loss || !workspace) return set_err(OTTER_EINVAL, "inbatch_loss_forward: NULL buffer");
-    const int64_t need = otter_inbatch_loss_workspace(B, d);
-    if (workspace_bytes < need)
-        return set_err(OTTER_EINVAL, "inbatch_loss_forward: workspace of %lld bytes, needs %lld", (long long)workspace_bytes,
-                       (long long)need);
+    if (!q || !c || !scores || !lse || !loss) return set_err(OTTER_EINVAL, "inbatch_loss_forward: NULL buffer");
+    if ((rc = check_workspace("inbatch_loss_forward", workspace, workspace_bytes, otter_inbatch_loss_workspace(B, d)))) return rc;
     DeviceGuard g(device);
     if (!g.ok) return set_err(OTTER_EHIP, "inbatch_loss_forward: hipSetDevice(%d) failed", device);
     LossArgs a = {};
@@ -341,32 +678,49 @@ int otter_inbatch_loss_forward(int device, const float* q, const float* c, const
     a.scores = scores;
     a.lse = lse;
     a.loss = loss;
-    a.rowloss = (float*)workspace;
-    a.part = a.rowloss + B;
     a.B = B;
     a.d = d;
     a.ld = ld;
-    const int bm = loss_tile(B), nt = (B + bm - 1) / bm;
-    a.splits = loss_splits(B, d, bm);
-    a.kchunk = ((d + a.splits - 1) / a.splits + KB - 1) / KB * KB;
+    a.splits = loss_splits(B, d);
+    a.kchunk = round_up((d + a.splits - 1) / a.splits, KB);
+    SplitArgs s = split_args(q, c, B, d);
+    lay_forward(workspace, a, s);
     hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)nt * nt, (unsigned)a.splits);
-    if (bm == 128)
-        loss_scores_kernel<128><<<grid, 256, 0, st>>>(a);
+    if (loss_planes(B, d)) {
+        a.splits = 1;
+        loss_split_kernel<false><<<dim3((unsigned)(s.Bp / 4), 2), 256, 0, st>>>(s);
+        loss_scores16_kernel<<<(unsigned)((s.Bp / 128) * (s.Bp / 128)), 256, 0, st>>>(a, s);
+    } else {
+        const unsigned nt = (unsigned)(B + 63) / 64;
+        loss_scores_kernel<64><<<dim3(nt * nt, (unsigned)a.splits), 256, 0, st>>>(a);
+    }
+    if (a.splits > 1)
+        loss_rows_kernel<true><<<B, 256, 0, st>>>(a);
     else
-        loss_scores_kernel<64><<<grid, 256, 0, st>>>(a);
-    loss_rows_kernel<<<B, 256, 0, st>>>(a);
+        loss_rows_kernel<false><<<B, 256, 0, st>>>(a);
     loss_mean_kernel<<<1, 1024, 0, st>>>(a);
     OTTER_HIP_TRY(hipGetLastError());
     return OTTER_OK;
 }
 
+int64_t otter_inbatch_loss_backward_workspace(int B, int d) {
+    const int rc = check_loss("inbatch_loss_backward_workspace", B, d, 0, 0);
+    if (rc) return rc;
+    SplitArgs s = split_args(nullptr, nullptr, B, d);
+    unsigned short* g[2];
+    return lay_backward(nullptr, s, g);
+}
+
 int otter_inbatch_loss_backward(int device, const float* dloss, const float* q, const float* c, const float* neg_c, int B, int d,
-                                const float* scores, int ld, const float* lse, float* dq, float* dc, float* dneg, void* stream) {
+                                const float* scores, int ld, const float* lse, float* dq, float* dc, float* dneg, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
     int rc = check_loss("inbatch_loss_backward", B, d, ld, B + (neg_c ? 1 : 0));
     if (rc) return rc;
     if (!dloss || !q || !c || !scores || !lse || !dq || !dc || (neg_c && !dneg))
         return set_err(OTTER_EINVAL, "inbatch_loss_backward: NULL buffer");
+    if ((rc = check_workspace("inbatch_loss_backward", workspace, workspace_bytes, otter_inbatch_loss_backward_workspace(B, d)))) return rc;
+    const long long tiles = (long long)((B + 63) / 64) * ((d + 63) / 64);
+    if (tiles > 0x3FFFFFFF) return set_err(OTTER_EINVAL, "inbatch_loss_backward: B=%d x d=%d is too large for one launch", B, d);
     DeviceGuard g(device);
     if (!g.ok) return set_err(OTTER_EHIP, "inbatch_loss_backward: hipSetDevice(%d) failed", device);
     LossArgs a = {};
@@ -383,13 +737,17 @@ int otter_inbatch_loss_backward(int device, const float* dloss, const float* q, 
     a.d = d;
     a.ld = ld;
     hipStream_t st = (hipStream_t)stream;
-    const int bm = loss_tile(B);
-    const long long tiles = (long long)((B + bm - 1) / bm) * ((d + bm - 1) / bm);
-    if (tiles > 0x3FFFFFFF) return set_err(OTTER_EINVAL, "inbatch_loss_backward: B=%d x d=%d is too large for one launch", B, d);
-    if (bm == 128)
-        loss_grad_kernel<128><<<(unsigned)(2 * tiles), 256, 0, st>>>(a);
-    else
+    if (loss_planes(B, d)) {
+        SplitArgs s = split_args(q, c, B, d);
+        unsigned short* gp[2];
+        lay_backward(workspace, s, gp);
+        loss_top_kernel<<<dim3(NMAX, 2), 256, 0, st>>>(s);
+        loss_split_kernel<true><<<dim3((unsigned)(s.Bp / 4), 2), 256, 0, st>>>(s);
+        loss_gplanes_kernel<<<dim3((unsigned)(s.Bp + 1023) / 1024, (unsigned)s.Bp), 256, 0, st>>>(a, gp[0], gp[1], s.Bp);
+        loss_grad16_kernel<<<(unsigned)(2 * (s.Bp / 128) * ((d + 63) / 64)), 256, 0, st>>>(a, s, gp[0], gp[1]);
+    } else {
         loss_grad_kernel<64><<<(unsigned)(2 * tiles), 256, 0, st>>>(a);
+    }
     OTTER_HIP_TRY(hipGetLastError());
     return OTTER_OK;
 }

@@ -102,9 +102,14 @@ def inbatch_loss_backward(dloss, q, c, neg_c, product, lse):
     ld = product.stride(0) if B > 1 else ncol
     dq, dc = torch.empty_like(q), torch.empty_like(c)
     dneg = None if neg_c is None else torch.empty_like(neg_c)
+    nbytes = lib.otter_inbatch_loss_backward_workspace(B, d)
+    if nbytes < 0:
+        _lib.check(int(nbytes), "otter_inbatch_loss_backward_workspace")
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
     _lib.check(lib.otter_inbatch_loss_backward(
         dev.index, dloss.data_ptr(), q.data_ptr(), c.data_ptr(), None if neg_c is None else neg_c.data_ptr(), B, d,
         product.data_ptr(), ld, lse.data_ptr(), dq.data_ptr(), dc.data_ptr(), None if dneg is None else dneg.data_ptr(),
+        None if ws is None else ws.data_ptr(), nbytes,
         _stream(dev.index)), "otter_inbatch_loss_backward")
     return dq, dc, dneg
 

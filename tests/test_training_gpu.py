@@ -432,6 +432,31 @@ def test_inbatch_loss(B, d, neg):
         assert (P - product).abs().max().item() <= 2 * float(ref["product"][1].max())
 
 
+@pytest.mark.parametrize("B", [40, 640])
+@pytest.mark.parametrize("scale", [1e-30, 1e-4, 1e4])
+def test_inbatch_loss_of_small_and_large_embeddings(B, scale):
+    """q scaled down or up and c the other way round: the scores stay, the float16 planes have to follow the sizes."""
+    from otter_amd import inbatch as IB
+    q64, q = _rand(90, B, 128, scale=scale * 128 ** -0.25)
+    c64, c = _rand(91, B, 128, scale=128 ** -0.25 / scale)
+    ref = R.inbatch_loss(q64, c64, None, 1.0)
+    loss, product, lse = IB.inbatch_loss_forward(q, c)
+    dq, dc, _ = IB.inbatch_loss_backward(torch.ones((), device=_dev()), q, c, None, product, lse)
+    for name, t in (("loss", loss), ("product", product), ("lse", lse), ("dq", dq), ("dc", dc)):
+        _close(name, t, ref[name])
+    # rows of very different sizes
+    row = torch.logspace(-3, 3, B, dtype=torch.float64)[:, None]
+    q64, q = _rand(92, B, 128, scale=128 ** -0.25)
+    q64 = (q64 * row).float().double()
+    c64, c = _rand(93, B, 128, scale=1e-3)
+    ref = R.inbatch_loss(q64, c64, None, 1.0)
+    q = q64.float().to(_dev())
+    loss, product, lse = IB.inbatch_loss_forward(q, c)
+    dq, dc, _ = IB.inbatch_loss_backward(torch.ones((), device=_dev()), q, c, None, product, lse)
+    for name, t in (("loss", loss), ("product", product), ("lse", lse), ("dq", dq), ("dc", dc)):
+        _close(name, t, ref[name])
+
+
 def test_inbatch_loss_autograd_and_edges():
     from otter_amd import inbatch as IB
     dev = _dev()

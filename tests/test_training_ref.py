@@ -198,11 +198,15 @@ def test_inbatch_loss_entry_points_refuse_bad_calls():
     _fails(fwd(ws=need - 1), "workspace")
 
     def bwd(dl=P, neg=None, dneg=None, ld=8):
-        return lib.otter_inbatch_loss_backward(0, dl, P, P, neg, 4, 8, P, ld, P, P, P, dneg, None)
+        return lib.otter_inbatch_loss_backward(0, dl, P, P, neg, 4, 8, P, ld, P, P, P, dneg, None, 0, None)
 
     _fails(bwd(dl=None), "NULL")
     _fails(bwd(neg=P), "NULL")
     _fails(bwd(ld=2), "ld=2")
+    need = lib.otter_inbatch_loss_backward_workspace(600, 64)
+    assert need > 0 and lib.otter_inbatch_loss_backward_workspace(4, 8) == 0
+    _fails(lib.otter_inbatch_loss_backward(0, P, P, P, None, 600, 64, P, 600, P, P, P, None, P, need - 1, None), "workspace")
+    _fails(lib.otter_inbatch_loss_backward(0, P, P, P, None, 600, 64, P, 600, P, P, P, None, ctypes.c_void_p(4104), need, None), "aligned")
 
 
 def test_python_entry_points_refuse_cpu_tensors():
