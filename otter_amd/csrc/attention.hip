@@ -350,6 +350,12 @@ struct Key2 {
 
 // the larger one, a NaN if there is one (fmaxf would first quiet both operands, two instructions more)
 __device__ __forceinline__ float max_(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+// x, made before it is rounded: the compiler otherwise rounds in front of a select, each value for itself (two conversions and
+// a permutation for a pair instead of one)
+__device__ __forceinline__ float made(float x) {
+    asm("" : "+v"(x));
+    return x;
+}
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ------------------------------------------------------------------ forward
@@ -437,7 +443,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnTrainArgs a) {
                 for (int r = 0; r < 16; ++r) {
                     const float p = exp2_(fmaf(sc[sub][r], c2, -base));
                     sum[r & 1] += p;                                 // the softmax's sum is over all keys, dropped or not
-                    sc[sub][r] = !DROP || w.kept_q(r) ? p : 0.0f;
+                    sc[sub][r] = DROP ? made(w.kept_q(r) ? p : 0.0f) : p;
                 }
                 col_product<T>(o, sV[buf] + sub * 32 * X::PITCH + ln.col<T>(), sc[sub]);
             }
@@ -484,7 +490,6 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
             for (int e = 0; e < X::EPC; ++e) D += to_f<T>(x[e]) * to_f<T>(y[e]);
         }
         D += __shfl_xor(D, 32);
-        if (i < s.len && h == 0) a.delta[s.stat + i] = D;
         load_own<T>(qf, Q, a.q.st, ic, h);
         const float lse2 = a.lse[s.stat + ic] * 1.4426950408889634f;
         f32x16 o[2] = {zero16(), zero16()};
@@ -508,6 +513,26 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
                     kb.fetch(j0 + 2 * TR);
                 }
                 if (bits == 0) continue;
+                // D = sum dO O from the stored O carries O's rounding into every dS of the row.  Of short rows, whose O is not
+                // small, that is as much as dS's own rounding (8 keys: dQ off by 2.7e-3 instead of 2.4e-3); where one tile
+                // holds all keys D is had without it, as sum_j P_ij Z_ij dP_ij.
+                if (sizeof(T) == 2 && kend <= TR) {
+                    D = 0.0f;
+#pragma unroll 1
+                    for (int sub = 0; sub < 2; ++sub) {
+                        const f32x16 sc = row_product<T>(sK[buf] + sub * 32 * X::PITCH + ln.frag<T>(), qf);
+                        const f32x16 dp = row_product<T>(sV[buf] + sub * 32 * X::PITCH + ln.frag<T>(), df);
+                        Draws w;
+                        if constexpr (DROP) w.queries(a.drop, key.k0, key.k1, bh, i, j0 + 32 * sub, h);
+                        const u32 kb32 = (u32)(bits >> (32 * sub)) >> (4 * h);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const bool counts = ((kb32 >> acc_row(r, 0)) & 1u) && (!DROP || w.kept_q(r));
+                            D += counts ? exp2_(fmaf(sc[r], a.c2, -lse2)) * dp[r] * a.drop.scale : 0.0f;
+                        }
+                    }
+                    D += __shfl_xor(D, 32);
+                }
 #pragma unroll (DROP ? 2 : 1)
                 for (int sub = 0; sub < 2; ++sub) {
                     f32x16 sc = row_product<T>(sK[buf] + sub * 32 * X::PITCH + ln.frag<T>(), qf);
@@ -530,6 +555,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
             }
             __syncthreads();
         }
+        if (i < s.len && h == 0) a.delta[s.stat + i] = D;
         if (i < s.len) store_own<T>(dQ + (long long)i * a.dq.st, o, a.scale, h);
     }
 }
@@ -605,7 +631,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
                             const float p = exp2_(fmaf(sc[r], a.c2, -lv[e]));
                             const bool kept = !DROP || w.kept_k(r);
                             const float gr = !DROP ? dp[r] - dv[e] : fmaf(kept ? dp[r] : 0.0f, a.drop.scale, -dv[e]);
-                            sc[r] = kept ? p : 0.0f;
+                            sc[r] = DROP ? made(kept ? p : 0.0f) : p;
                             dp[r] = p * gr;
                         }
                     }
