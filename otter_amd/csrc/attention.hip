@@ -50,10 +50,14 @@ struct Seq {
     long long stat;            // index of its first row in lse / delta
 };
 
-__device__ __forceinline__ Seq find_seq(const AttnTrainArgs& a, int item) {
+// Workgroups b, b + 8, ... share an XCD and its L2.  The workgroups of one (sequence, head), which read the same rows, go to
+// one XCD; (sequence, head) pairs go round the XCDs one by one, so that every XCD gets its share of long and short sequences.
+__device__ __forceinline__ Seq find_seq(const AttnTrainArgs& a, int bid, int pair = -1) {
     Seq s;
-    s.blk = item % a.nblk;
-    const int bh = item / a.nblk;
+    const int whole = (a.B * a.heads & ~7) * a.nblk;      // the last pairs, fewer than 8, as they come
+    const int idx = bid < whole ? bid >> 3 : bid - whole;
+    const int bh = pair >= 0 ? pair : bid < whole ? idx / a.nblk * 8 + (bid & 7) : whole / a.nblk + idx / a.nblk;
+    s.blk = pair >= 0 ? 0 : idx % a.nblk;
     s.h = bh % a.heads;
     s.b = bh / a.heads;
     if (a.cu) {
@@ -177,27 +181,44 @@ __device__ __forceinline__ f32x16 row_product(const char* t, const float4 (&own)
     return acc;
 }
 
+// two of them side by side: neither waits for its own last step
+template <typename T>
+__device__ __forceinline__ void row_products(f32x16& x, f32x16& y, const char* tx, const float4 (&ox)[Tile<T>::NF], const char* ty,
+                                             const float4 (&oy)[Tile<T>::NF]) {
+    x = zero16();
+    y = zero16();
+#pragma unroll
+    for (int j = 0; j < Tile<T>::NF; ++j) {
+        mma<T>(x, *reinterpret_cast<const float4*>(tx + j * 32), ox[j]);
+        mma<T>(y, *reinterpret_cast<const float4*>(ty + j * 32), oy[j]);
+    }
+}
+
 // o[d half] += X^T w: X = tile rows (32 from t on), w = an accumulator tile with X's row on the registers; t: the tile +
 // Lane::col.  bf16: w is rounded here, the one rounding between the two products (2^-8 of each weight at most; the sums
 // stay in float32).
+__device__ __forceinline__ void col_product_b(f32x16 (&o)[2], const char* t, const bf16x8 (&wb)[2]) {
+    constexpr int P = Tile<bf16_t>::PITCH;
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            // X^T[d][row], rows 16 s2 + 8 (j >> 2) + 4 h + (j & 3): two transposed reads of 4 rows x 16 columns
+            const char* p0 = t + s2 * 16 * P + d * 64;
+            const s16x4 v[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)p0),
+                                __builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)(p0 + 8 * P))};
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), wb[s2], o[d], 0, 0, 0);
+        }
+}
+
 template <typename T>
 __device__ __forceinline__ void col_product(f32x16 (&o)[2], const char* t, const f32x16& w) {
     constexpr int P = Tile<T>::PITCH;
     if constexpr (sizeof(T) == 2) {
+        bf16x8 wb[2];
 #pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) {
-            bf16x8 wb;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) wb[j] = (__bf16)w[8 * s2 + j];
-#pragma unroll
-            for (int d = 0; d < 2; ++d) {
-                // X^T[d][row], rows 16 s2 + 8 (j >> 2) + 4 h + (j & 3): two transposed reads of 4 rows x 16 columns
-                const char* p0 = t + s2 * 16 * P + d * 64;
-                const s16x4 v[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)p0),
-                                    __builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)(p0 + 8 * P))};
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), wb, o[d], 0, 0, 0);
-            }
-        }
+        for (int r = 0; r < 16; ++r) wb[r >> 3][r & 7] = (__bf16)w[r];
+        col_product_b(o, t, wb);
     } else {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -372,7 +393,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnTrainArgs a) {
     const int h = ln.h, l31 = ln.l31, wave = ln.wave;
     const int items = a.nblk * a.heads * a.B;
     if ((int)blockIdx.x >= items) return zero_outside<T>(a, blockIdx.x - items, a.o, a.lse);
-    const Seq s = find_seq(a, xcd_remap(blockIdx.x, items));
+    const Seq s = find_seq(a, blockIdx.x);
     bool even;
     const int kend = key_end(a, s, even);
     const T *Q = head_ptr<T>(a, a.q, s), *K = head_ptr<T>(a, a.k, s), *V = head_ptr<T>(a, a.v, s);
@@ -463,13 +484,14 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnTrainArgs a) {
 template <typename T, bool DROP>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
     using X = Tile<T>;
+    constexpr int UNROLL = DROP ? 2 : 1;      // the draws of one half fill the waits of the other (packed, dropout: 440 -> 416 us)
     __shared__ __attribute__((aligned(16))) char sK[2][X::BYTES];
     __shared__ __attribute__((aligned(16))) char sV[2][X::BYTES];
     const Lane ln;
     const int h = ln.h, l31 = ln.l31, wave = ln.wave;
     const int items = a.nblk * a.heads * a.B;
     if ((int)blockIdx.x >= items) return zero_outside<T>(a, blockIdx.x - items, a.dq, nullptr);
-    const Seq s = find_seq(a, xcd_remap(blockIdx.x, items));
+    const Seq s = find_seq(a, blockIdx.x);
     bool even;
     const int kend = key_end(a, s, even);
     const T *Q = head_ptr<T>(a, a.q, s), *K = head_ptr<T>(a, a.k, s), *V = head_ptr<T>(a, a.v, s);
@@ -533,7 +555,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
                     }
                     D += __shfl_xor(D, 32);
                 }
-#pragma unroll (DROP ? 2 : 1)
+#pragma unroll UNROLL
                 for (int sub = 0; sub < 2; ++sub) {
                     f32x16 sc = row_product<T>(sK[buf] + sub * 32 * X::PITCH + ln.frag<T>(), qf);
                     const f32x16 dp = row_product<T>(sV[buf] + sub * 32 * X::PITCH + ln.frag<T>(), df);
@@ -565,6 +587,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
 template <typename T, bool DROP>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
     using X = Tile<T>;
+    constexpr int UNROLL = DROP ? 2 : 1;      // the draws of one half fill the waits of the other (packed, dropout: 440 -> 416 us)
     __shared__ __attribute__((aligned(16))) char sQ[2][X::BYTES];
     __shared__ __attribute__((aligned(16))) char sO[2][X::BYTES];
     __shared__ __attribute__((aligned(16))) float sL[2][TR], sD[2][TR];
@@ -575,7 +598,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
         zero_outside<T>(a, blockIdx.x - items, a.dk, nullptr);
         return zero_outside<T>(a, blockIdx.x - items, a.dv, nullptr);
     }
-    const Seq s = find_seq(a, xcd_remap(blockIdx.x, items));
+    const Seq s = find_seq(a, blockIdx.x);
     bool even;
     const int kend = key_end(a, s, even);
     const T *Q = head_ptr<T>(a, a.q, s), *K = head_ptr<T>(a, a.k, s), *V = head_ptr<T>(a, a.v, s);
@@ -586,7 +609,6 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
     for (int n0 = s.blk * OWN; n0 < s.len; n0 += a.nblk * OWN) {
         const int j = n0 + wave * 32 + l31, jc = min(j, s.len - 1);
         const bool counts = j < kend && (even || !a.mask || a.mask[(long long)s.b * a.L + jc] != 0);
-        const bool all = __all(counts);
         f32x16 ok[2] = {zero16(), zero16()}, ov[2] = {zero16(), zero16()};
         if (n0 < kend) {
             float4 kf[X::NF], vf[X::NF];
@@ -614,10 +636,10 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
                 }
                 __syncthreads();
                 if (i0 + TR < s.len) fetch(i0 + TR);
-#pragma unroll (DROP ? 2 : 1)
+#pragma unroll UNROLL
                 for (int sub = 0; sub < 2; ++sub) {
-                    f32x16 sc = row_product<T>(sQ[buf] + sub * 32 * X::PITCH + ln.frag<T>(), kf);
-                    f32x16 dp = row_product<T>(sO[buf] + sub * 32 * X::PITCH + ln.frag<T>(), vf);
+                    f32x16 sc, dp;
+                    row_products<T>(sc, dp, sQ[buf] + sub * 32 * X::PITCH + ln.frag<T>(), kf, sO[buf] + sub * 32 * X::PITCH + ln.frag<T>(), vf);
                     Draws w;
                     if constexpr (DROP) w.keys(a.drop, key.k0, key.k1, bh, j, i0 + 32 * sub, h);
 #pragma unroll
@@ -635,18 +657,217 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
                             dp[r] = p * gr;
                         }
                     }
-                    if (!all || even) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            sc[r] = counts ? sc[r] : 0.0f;
-                            dp[r] = counts && !even ? dp[r] : 0.0f;
-                        }
-                    }
                     col_product<T>(ov, sO[buf] + sub * 32 * X::PITCH + ln.col<T>(), sc);
                     col_product<T>(ok, sQ[buf] + sub * 32 * X::PITCH + ln.col<T>(), dp);
                 }
             }
             __syncthreads();
+        }
+        // a key's gradients are sums in its own lanes: what a key that does not count gathered is dropped here
+        if (!counts || even) {
+            ok[0] = ok[1] = zero16();
+            if (!counts) ov[0] = ov[1] = zero16();
+        }
+        if (j < s.len) {
+            store_own<T>(dK + (long long)j * a.dk.st, ok, a.scale, h);
+            store_own<T>(dV + (long long)j * a.dv.st, ov, a.drop.scale, h);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ backward in one pass
+// bfloat16.  A workgroup of 8 waves owns a (sequence, head); it takes its keys 256 at a time, a wave 32 (one on each lane of a
+// half), and streams the queries in tiles of 32.  Every score tile is made ONCE: probabilities and dS go from the registers
+// into dV and dK as in attn_dkv_kernel, dS also goes to LDS (64 bytes a key), from where all waves together make the tile's
+// dQ, a block of 16 queries x 16 elements each, with their 16 columns of K^T in registers.  dQ of more than 256 keys is
+// carried in a float32 buffer that the same thread writes and reads.  One barrier a tile; D comes out of the staging.
+constexpr int FK = 256, FQ = 32;      // keys at a time, rows of a streamed tile
+constexpr int SPITCH = FQ * 2 + 8;    // bytes a key of dS^T in LDS
+
+__device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
+
+template <int CTRL>
+__device__ __forceinline__ float dppf(float x) {
+    return __uint_as_float(quad<CTRL>(__float_as_uint(x)));
+}
+
+template <bool DROP>
+__global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
+    typedef bf16_t T;
+    using X = Tile<T>;
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    __shared__ __attribute__((aligned(16))) char sQ[2][FQ * X::PITCH];
+    __shared__ __attribute__((aligned(16))) char sO[2][FQ * X::PITCH];
+    __shared__ __attribute__((aligned(16))) char sS[2][FK * SPITCH];        // first K's 256 rows, then dS^T of a tile
+    __shared__ __attribute__((aligned(16))) float sL[2][FQ], sD[2][FQ];
+    __shared__ __attribute__((aligned(16))) char sK[FK * X::PITCH];
+    const Lane ln;
+    const int lane = ln.lane, wave = ln.wave, h = ln.h, l31 = ln.l31, tid = threadIdx.x;
+    const int items = a.heads * a.B;
+    if ((int)blockIdx.x >= items) {
+        zero_outside<T>(a, blockIdx.x - items, a.dq, nullptr);
+        zero_outside<T>(a, blockIdx.x - items, a.dk, nullptr);
+        return zero_outside<T>(a, blockIdx.x - items, a.dv, nullptr);
+    }
+    // nothing is shared between workgroups here: an XCD takes the heads of a sequence together (packed, 128 sequences: 323 us,
+    // 366 with the pairs going round)
+    const Seq s = find_seq(a, blockIdx.x, xcd_remap(blockIdx.x, items));
+    bool even;
+    const int kend = key_end(a, s, even);
+    const T *Q = head_ptr<T>(a, a.q, s), *K = head_ptr<T>(a, a.k, s), *V = head_ptr<T>(a, a.v, s);
+    const T *O = head_ptr<T>(a, a.o, s), *dO = head_ptr<T>(a, a.dout, s);
+    T *dQ = head_ptr<T>(a, a.dq, s), *dK = head_ptr<T>(a, a.dk, s), *dV = head_ptr<T>(a, a.dv, s);
+    const u32 bh = (u32)(s.b * a.heads + s.h);
+    const Key2 key(a.drop);
+    const long long* mask = a.mask && !even ? a.mask + (long long)s.b * a.L : nullptr;
+    // staging: threads 0-255 a chunk of Q, 256-511 the same chunk of dO and of O (their product is D)
+    const int sr = (tid & 255) >> 3, sc8 = tid & 7;
+    const bool isq = tid < 256;
+    const T* src = (isq ? Q : dO) + sc8 * X::EPC;
+    const long long sst = isq ? a.q.st : a.dout.st;
+    // dQ: this wave's block, this lane's query and four elements
+    const int dcol = 16 * (wave & 3), qhalf = 16 * (wave >> 2), g4 = lane >> 4, i16 = lane & 15;
+    const long long prow = (a.cu ? s.row0 : (long long)s.b * a.L);
+
+    for (int n0 = 0; n0 < s.len; n0 += FK) {
+        const int nk = min(FK, kend - n0);                 // keys that may count here
+        const int j = n0 + wave * 32 + l31, jc = min(j, s.len - 1);
+        const bool counts = j < kend && (!mask || mask[jc] != 0);
+        const bool all = __all(counts);
+        f32x16 ok[2] = {zero16(), zero16()}, ov[2] = {zero16(), zero16()};
+        if (nk > 0) {
+            const bool first = n0 == 0, last = n0 + FK >= kend, busy = wave * 32 < nk;
+            float4 kf[X::NF], vf[X::NF];
+            load_own<T>(kf, K, a.k.st, jc, h);
+            load_own<T>(vf, V, a.v.st, jc, h);
+            if (even) zero_frags<T>(kf);
+            // K^T: 16 elements x 256 keys, a lane one element and 8 keys of every 32
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = e * 64 + (tid >> 3), jj = n0 + r;
+                float4 v = *reinterpret_cast<const float4*>(K + (long long)min(jj, s.len - 1) * a.k.st + sc8 * X::EPC);
+                if (even || !(jj < kend && (!mask || mask[min(jj, s.len - 1)] != 0))) v = make_float4(0.f, 0.f, 0.f, 0.f);
+                *reinterpret_cast<float4*>(sK + r * X::PITCH + sc8 * 16) = v;
+            }
+            __syncthreads();
+            float4 rv, ro = make_float4(0.f, 0.f, 0.f, 0.f);
+            float rl = 0.0f;
+            auto fetch = [&](int i0) {
+                const long long row = min(i0 + sr, s.len - 1);
+                rv = *reinterpret_cast<const float4*>(src + row * sst);
+                if (!isq) ro = *reinterpret_cast<const float4*>(O + row * a.o.st + sc8 * X::EPC);
+                rl = a.lse[s.stat + min(i0 + (tid & (FQ - 1)), s.len - 1)];
+            };
+            auto store = [&](int i0, int buf) {
+                const bool in = i0 + sr < s.len;
+                if (!in || (even && isq)) rv = make_float4(0.f, 0.f, 0.f, 0.f);
+                *reinterpret_cast<float4*>((isq ? sQ[buf] : sO[buf]) + sr * X::PITCH + sc8 * 16) = rv;
+                if (!isq) {
+                    const T *x = reinterpret_cast<const T*>(&rv), *y = reinterpret_cast<const T*>(&ro);
+                    float d = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) d += to_f<T>(x[e]) * to_f<T>(y[e]);
+                    d += dppf<0xB1>(d);
+                    d += dppf<0x4E>(d);
+                    d += dppf<0x141>(d);
+                    if (sc8 == 0) sD[buf][sr] = in ? d : 0.0f;
+                }
+                // rows past the end: exp2(0 - inf) = 0
+                if (tid < FQ) sL[buf][tid] = i0 + tid < s.len ? rl * 1.4426950408889634f : INFINITY;
+            };
+            fetch(0);
+            store(0, 0);
+            if (FQ < s.len) fetch(FQ);
+            __syncthreads();                               // K^T is read, tile 0 is there
+            if (!busy)                                     // keys nobody has: their dS is zero once and for all
+                for (int e = lane; e < 32 * SPITCH / 4; e += 64) {
+                    reinterpret_cast<u32*>(sS[0] + wave * 32 * SPITCH)[e] = 0;
+                    reinterpret_cast<u32*>(sS[1] + wave * 32 * SPITCH)[e] = 0;
+                }
+            for (int i0 = 0, buf = 0; i0 < s.len; i0 += FQ, buf ^= 1) {
+                const int qi = i0 + qhalf + i16;
+                float* part = a.delta + ((prow + min(qi, s.len - 1)) * a.heads + s.h) * DH + dcol + 4 * g4;
+                f32x4 dq = {0.f, 0.f, 0.f, 0.f};
+                if (!first) dq = *reinterpret_cast<const f32x4*>(part);
+                if (busy) {
+                    f32x16 sc, dp;
+                    row_products<T>(sc, dp, sQ[buf] + ln.frag<T>(), kf, sO[buf] + ln.frag<T>(), vf);
+                    Draws w;
+                    if constexpr (DROP) w.keys(a.drop, key.k0, key.k1, bh, j, i0, h);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const float4 L4 = *reinterpret_cast<const float4*>(&sL[buf][8 * g + 4 * h]);
+                        const float4 D4 = *reinterpret_cast<const float4*>(&sD[buf][8 * g + 4 * h]);
+                        const float lv[4] = {L4.x, L4.y, L4.z, L4.w}, dv[4] = {D4.x, D4.y, D4.z, D4.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int r = 4 * g + e;
+                            const float p = exp2_(fmaf(sc[r], a.c2, -lv[e]));
+                            const bool kept = !DROP || w.kept_k(r);
+                            const float gr = !DROP ? dp[r] - dv[e] : fmaf(kept ? dp[r] : 0.0f, a.drop.scale, -dv[e]);
+                            sc[r] = DROP ? made(kept ? p : 0.0f) : p;
+                            dp[r] = p * gr;
+                        }
+                    }
+                    if (!all || even) {                    // what a key that does not count adds to dQ
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) dp[r] = counts && !even ? dp[r] : 0.0f;
+                    }
+                    bf16x8 ds[2];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) ds[r >> 3][r & 7] = (__bf16)dp[r];
+                    char* d = sS[buf] + (wave * 32 + l31) * SPITCH + 8 * h;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        typedef short s16x4a __attribute__((ext_vector_type(4)));
+                        const s16x4a v = reinterpret_cast<const s16x4a*>(&ds[g >> 1])[g & 1];
+                        *reinterpret_cast<s16x4a*>(d + 16 * g) = v;
+                    }
+                    col_product<T>(ov, sO[buf] + ln.col<T>(), sc);
+                    col_product_b(ok, sQ[buf] + ln.col<T>(), ds);
+                }
+                if (i0 + FQ < s.len) {
+                    store(i0 + FQ, buf ^ 1);
+                    if (i0 + 2 * FQ < s.len) fetch(i0 + 2 * FQ);
+                }
+                __syncthreads();
+                f32x4 dq2 = {0.f, 0.f, 0.f, 0.f};
+                const char* ps = sS[buf] + (8 * g4 + (i16 >> 2)) * SPITCH + (qhalf + 4 * (i16 & 3)) * 2;
+                const char* pk = sK + (8 * g4 + (i16 >> 2)) * X::PITCH + (dcol + 4 * (i16 & 3)) * 2;
+#pragma unroll
+                for (int k4 = 0; k4 < 8; k4 += 4) {
+                    s16x4 sb[4][2], kt[4][2];
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            sb[ks][e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)(ps + (32 * (k4 + ks) + 4 * e) * SPITCH));
+                            kt[ks][e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((OTTER_AS3 s16x4*)(pk + (32 * (k4 + ks) + 4 * e) * X::PITCH));
+                        }
+                    pin();
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        f32x4& acc = ks & 1 ? dq2 : dq;
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kt[ks]), __builtin_bit_cast(bf16x8, sb[ks]), acc, 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dq[e] += dq2[e];
+                if (qi < s.len) {
+                    if (last) {
+                        const u32 w0 = (u32)f2bf(dq[0] * a.scale) | ((u32)f2bf(dq[1] * a.scale) << 16);
+                        const u32 w1 = (u32)f2bf(dq[2] * a.scale) | ((u32)f2bf(dq[3] * a.scale) << 16);
+                        *reinterpret_cast<uint2*>(dQ + (long long)qi * a.dq.st + dcol + 4 * g4) = make_uint2(w0, w1);
+                    } else {
+                        *reinterpret_cast<f32x4*>(part) = dq;
+                    }
+                }
+            }
+        }
+        if (!counts || even) {
+            ok[0] = ok[1] = zero16();
+            if (!counts) ov[0] = ov[1] = zero16();
         }
         if (j < s.len) {
             store_own<T>(dK + (long long)j * a.dk.st, ok, a.scale, h);
@@ -704,6 +925,14 @@ void launch_fwd(const AttnTrainArgs& a, int grid, hipStream_t st) {
         attn_fwd_kernel<T, false><<<grid, 256, 0, st>>>(a);
 }
 
+// One pass over the scores (bfloat16) or two, one for dQ and one for dK and dV.  One pass makes each score tile once, but has only
+// one workgroup a (sequence, head), the chip to itself at 256 of them, and more to synchronise: 128 packed sequences of 64 to
+// 512, 12 heads, dropout 323 us (two passes 420), without dropout 289 (335); 16 x 512, 12 heads (192 workgroups) 86 us (92)
+// with, 72 (69) without.  Short sequences (up to OWN) are one workgroup a (sequence, head) either way.
+bool one_pass(const AttnTrainArgs& a, int dtype) {
+    return dtype == OTTER_BF16 && a.L > OWN && (long long)a.B * a.heads >= (a.drop.thr ? 192 : 256);
+}
+
 template <typename T>
 void launch_bwd(const AttnTrainArgs& a, int grid, hipStream_t st) {
     if (a.drop.thr) {
@@ -713,6 +942,12 @@ void launch_bwd(const AttnTrainArgs& a, int grid, hipStream_t st) {
         attn_dq_kernel<T, false><<<grid, 256, 0, st>>>(a);
         attn_dkv_kernel<T, false><<<grid, 256, 0, st>>>(a);
     }
+}
+
+// D of every row and head; in one pass the float32 dQ of sequences of more than FK keys (packed ones may be longer than `tokens`)
+int64_t backward_bytes(const AttnTrainArgs& a, int dtype, long long rows) {
+    const int64_t n = rows * a.heads * (int64_t)sizeof(float);
+    return one_pass(a, dtype) ? (a.cu || a.L > FK ? n * DH : 0) : n;
 }
 
 }  // namespace
@@ -747,7 +982,7 @@ int64_t otter_attention_backward_workspace(const otter_attention_args* x) {
     long long rows = 0;
     int rc = fill("attention_backward_workspace", x, &a, &rows);
     if (rc) return rc;
-    return rows * a.heads * (int64_t)sizeof(float);
+    return backward_bytes(a, x->dtype, rows);
 }
 
 int otter_attention_backward(int device, const otter_attention_args* x, void* stream) {
@@ -765,16 +1000,26 @@ int otter_attention_backward(int device, const otter_attention_args* x, void* st
                  {"dout", &x->dout, &a.dout}, {"dq", &x->dq, &a.dq}, {"dk", &x->dk, &a.dk}, {"dv", &x->dv, &a.dv}};
     for (const auto& v : views)
         if ((rc = set_view("attention_backward", v.name, *v.v, size, v.out))) return rc;
-    if (!a.lse || !x->workspace) return set_err(OTTER_EINVAL, "attention_backward: NULL lse or workspace");
-    const int64_t need = rows * a.heads * (int64_t)sizeof(float);
-    if (x->workspace_bytes < need)
-        return set_err(OTTER_EINVAL, "attention_backward: workspace of %lld bytes, needs %lld", (long long)x->workspace_bytes,
-                       (long long)need);
+    if (!a.lse) return set_err(OTTER_EINVAL, "attention_backward: NULL lse");
+    const int64_t need = backward_bytes(a, x->dtype, rows);
+    if (need > 0 && (!x->workspace || x->workspace_bytes < need || ((uintptr_t)x->workspace & 15)))
+        return set_err(OTTER_EINVAL, "attention_backward: workspace of %lld bytes, needs %lld, 16-byte aligned",
+                       (long long)x->workspace_bytes, (long long)need);
     a.delta = (float*)x->workspace;
     DeviceGuard g(device);
     if (!g.ok) return set_err(OTTER_EHIP, "attention_backward: hipSetDevice(%d) failed", device);
-    const int grid = a.nblk * a.heads * a.B + (a.cu ? a.heads : 0);
     hipStream_t st = (hipStream_t)stream;
+    if (one_pass(a, x->dtype)) {
+        a.nblk = 1;
+        const int n = a.heads * a.B + (a.cu ? a.heads : 0);
+        if (a.drop.thr)
+            attn_bwd_kernel<true><<<n, 512, 0, st>>>(a);
+        else
+            attn_bwd_kernel<false><<<n, 512, 0, st>>>(a);
+        OTTER_HIP_TRY(hipGetLastError());
+        return OTTER_OK;
+    }
+    const int grid = a.nblk * a.heads * a.B + (a.cu ? a.heads : 0);
     if (size == 2)
         launch_bwd<bf16_t>(a, grid, st);
     else

@@ -36,7 +36,7 @@ def new_seed(device=None, generator=None):
 
 def _on_gpu(what, name, t):
     """The tensor is on a GPU and of a supported dtype; returns (device, dtype code)."""
-    if not (torch.is_tensor(t) and t.is_cuda):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise ValueError("%s: %s must be a tensor on a GPU (the HIP path has no CPU fallback)" % (what, name))
     code = _DTYPES.get(t.dtype)
     if code is None:
@@ -46,7 +46,7 @@ def _on_gpu(what, name, t):
 
 def _like(what, name, t, first):
     """t has the first tensor's shape, dtype and device."""
-    if not torch.is_tensor(t) or t.dtype != first.dtype or t.device != first.device or t.shape != first.shape:
+    if not isinstance(t, torch.Tensor) or t.dtype is not first.dtype or t.shape != first.shape or t.device != first.device:
         raise ValueError("%s: %s must be like the first operand: expected %s %r on %s" % (
             what, name, first.dtype, tuple(first.shape), first.device))
 
@@ -130,10 +130,11 @@ def _norm_args(what, x, weight, residual, dropout_p, seed, call):
     if residual is not None:
         _like(what, "residual", residual, x)
     cols = x.shape[-1]
-    if not (torch.is_tensor(weight) and weight.device == dev and weight.dtype in _DTYPES and tuple(weight.shape) == (cols,)):
+    wdt = _DTYPES.get(weight.dtype) if isinstance(weight, torch.Tensor) else None
+    if wdt is None or weight.device != dev or weight.shape != (cols,):
         raise ValueError("%s: weight must be a float32 or bfloat16 tensor [%d] on %s" % (what, cols, dev))
     rows = x.numel() // cols if cols else 0
-    return dev, dt, _DTYPES[weight.dtype], rows, cols, _seed_ptr(what, seed, dropout_p, dev), _call_id(what, call)
+    return dev, dt, wdt, rows, cols, _seed_ptr(what, seed, dropout_p, dev), _call_id(what, call)
 
 
 def layer_norm_forward(x, weight, bias, eps=1e-5, residual=None, dropout_p=0.0, seed=None, call=0):
@@ -211,23 +212,27 @@ _TAIL = struct.Struct("=Qq")
 _NO_VIEWS = _VIEWS.pack(*(0,) * 16)
 
 
-def _aligned(t):
-    """t itself if the kernels can read it in place: heads of 64 contiguous elements, 16-byte aligned data and strides."""
-    mask = 15 // t.element_size()
-    *outer, inner = t.stride()
-    bad = t.data_ptr() & 15
-    for x in outer:
-        bad |= x & mask
-    return t.clone(memory_format=torch.contiguous_format) if bad or inner != 1 else t
+def _operand(t, mask):
+    """(t, its pointer and strides) if the kernels can read it in place -- heads of 64 contiguous elements, 16-byte aligned data
+    and strides (mask: elements of 16 bytes, less one) -- otherwise of a contiguous copy."""
+    s, p = t.stride(), t.data_ptr()
+    if len(s) == 4:
+        sb, st, sh, inner = s
+    else:
+        sb, (st, sh, inner) = 0, s
+    if inner != 1 or p & 15 or (sb | st | sh) & mask:
+        return _operand(t.clone(memory_format=torch.contiguous_format), mask)
+    return t, (p, sb, st, sh)
 
 
-def _view(t):
-    s = t.stride()
-    return (t.data_ptr(), s[0], s[1], s[2]) if len(s) == 4 else (t.data_ptr(), 0, s[0], s[1])
+def _dense(p, shape):
+    """Pointer and strides of a contiguous tensor."""
+    row = shape[-2] * shape[-1]
+    return (p, shape[1] * row if len(shape) == 4 else 0, row, shape[-1])
 
 
 def _attention_args(what, q, k, v, mask, cu_seqlens, max_seqlen, dropout_p, seed, call, scale):
-    """(packed head of the arguments, q, k, v as they are read, tensors to keep alive, device, lse shape)."""
+    """(packed head of the arguments, the views of q, k and v, tensors to keep alive, device, lse shape, alignment mask)."""
     dev, dt = _on_gpu(what, "q", q)
     packed = cu_seqlens is not None
     shape = q.shape
@@ -241,7 +246,11 @@ def _attention_args(what, q, k, v, mask, cu_seqlens, max_seqlen, dropout_p, seed
         raise ValueError("%s: no heads" % what)
     if packed and mask is not None:
         raise ValueError("%s: a key mask and packed sequences exclude each other" % what)
-    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    align = 16 // q.element_size() - 1
+    q, vq = _operand(q, align)
+    k, vk = _operand(k, align)
+    v, vv = _operand(v, align)
+    views = vq + vk + vv
     seed_ptr, call = _seed_ptr(what, seed, dropout_p, dev) or 0, _call_id(what, call)
     if scale is None:
         scale = 1.0 / math.sqrt(max(1, dim))
@@ -253,7 +262,7 @@ def _attention_args(what, q, k, v, mask, cu_seqlens, max_seqlen, dropout_p, seed
             max_seqlen = int(cu_seqlens.diff().max()) if cu_seqlens.numel() > 1 else 0
         head = _HEAD.pack(dt, cu_seqlens.numel() - 1, max(0, int(max_seqlen)), heads, dim, call, scale, dropout_p, shape[0], 0,
                           cu_seqlens.data_ptr(), seed_ptr)
-        return head, q, k, v, cu_seqlens, dev, (heads, shape[0])
+        return head, views, (q, k, v, cu_seqlens), dev, (heads, shape[0]), align
     mask_ptr = 0
     if mask is not None:
         if not torch.is_tensor(mask) or mask.shape != shape[:2] or mask.device != dev:
@@ -261,7 +270,7 @@ def _attention_args(what, q, k, v, mask, cu_seqlens, max_seqlen, dropout_p, seed
         mask = (mask if mask.dtype == torch.int64 else (mask != 0).to(torch.int64)).contiguous()
         mask_ptr = mask.data_ptr()
     head = _HEAD.pack(dt, shape[0], shape[1], heads, dim, call, scale, dropout_p, 0, mask_ptr, 0, seed_ptr)
-    return head, q, k, v, mask, dev, (shape[0], heads, shape[1])
+    return head, views, (q, k, v, mask), dev, (shape[0], heads, shape[1]), align
 
 
 def attention_forward(q, k, v, mask=None, cu_seqlens=None, max_seqlen=None, dropout_p=0.0, seed=None, call=0, scale=None):
@@ -274,11 +283,11 @@ def attention_forward(q, k, v, mask=None, cu_seqlens=None, max_seqlen=None, drop
     Views of a fused projection, qkv.unbind(-3), are read in place.  scale: 1 / 8 by default.
     lse (float32 [batch, heads, tokens] / [heads, total]) is what the backward pass needs."""
     lib = _lib.load()
-    head, q, k, v, keep, dev, lse_shape = _attention_args("attention", q, k, v, mask, cu_seqlens, max_seqlen, dropout_p, seed,
-                                                          call, scale)
+    head, views, keep, dev, lse_shape, _ = _attention_args("attention", q, k, v, mask, cu_seqlens, max_seqlen, dropout_p, seed,
+                                                           call, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty(lse_shape, dtype=torch.float32, device=dev)
-    args = b"".join((head, _VIEWS.pack(*_view(q), *_view(k), *_view(v), *_view(out)), lse.data_ptr().to_bytes(8, "little"),
+    args = b"".join((head, _VIEWS.pack(*views, *_dense(out.data_ptr(), out.shape)), lse.data_ptr().to_bytes(8, "little"),
                      _NO_VIEWS, _TAIL.pack(0, 0)))
     _lib.check(lib.otter_attention_forward(dev.index, args, _stream(dev.index)), "otter_attention_forward")
     return out, lse
@@ -290,29 +299,34 @@ def attention_backward(dout, q, k, v, out, lse, mask=None, cu_seqlens=None, max_
     write them to, for instance the views dqkv.unbind(-3) of one buffer."""
     lib = _lib.load()
     what = "attention_backward"
-    head, q, k, v, keep, dev, lse_shape = _attention_args(what, q, k, v, mask, cu_seqlens, max_seqlen, dropout_p, seed, call,
-                                                          scale)
+    head, views, keep, dev, lse_shape, align = _attention_args(what, q, k, v, mask, cu_seqlens, max_seqlen, dropout_p, seed,
+                                                               call, scale)
     _like(what, "dout", dout, q)
     _like(what, "out", out, q)
     if lse.shape != lse_shape or lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous():
         raise ValueError("%s: lse must be what attention_forward returned" % what)
-    dout, out = _aligned(dout), _aligned(out)
+    dout, v_dout = _operand(dout, align)
+    out, v_out = _operand(out, align)
     if grads is None:
-        grads = torch.empty((3,) + q.shape, dtype=q.dtype, device=dev).unbind(0)
+        buf = torch.empty((3,) + q.shape, dtype=q.dtype, device=dev)
+        p, step = buf.data_ptr(), q.numel() * q.element_size()
+        to = _dense(p, q.shape) + _dense(p + step, q.shape) + _dense(p + 2 * step, q.shape)
+        grads = buf.unbind(0)
     else:
+        to = ()
         for t in grads:
-            if t.shape != q.shape or t.dtype != q.dtype or t.device != dev or _aligned(t) is not t:
+            if t.shape != q.shape or t.dtype != q.dtype or t.device != dev or _operand(t, align)[0] is not t:
                 raise ValueError("%s: grads must be like q, their heads contiguous, data and strides multiples of 16 bytes" % what)
-    dq, dk, dv = grads
-    views = _VIEWS.pack(*_view(q), *_view(k), *_view(v), *_view(out))
+            to += _operand(t, align)[1]
+    views = _VIEWS.pack(*views, *v_out)
     lse_ptr = lse.data_ptr().to_bytes(8, "little")
     nbytes = lib.otter_attention_backward_workspace(b"".join((head, views, lse_ptr, _NO_VIEWS, _TAIL.pack(0, 0))))
     if nbytes < 0:
         _lib.check(int(nbytes), "otter_attention_backward_workspace")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    args = b"".join((head, views, lse_ptr, _VIEWS.pack(*_view(dout), *_view(dq), *_view(dk), *_view(dv)),
-                     _TAIL.pack(ws.data_ptr(), nbytes)))
+    args = b"".join((head, views, lse_ptr, _VIEWS.pack(*v_dout, *to), _TAIL.pack(ws.data_ptr(), nbytes)))
     _lib.check(lib.otter_attention_backward(dev.index, args, _stream(dev.index)), "otter_attention_backward")
+    dq, dk, dv = grads
     return dq, dk, dv
 
 

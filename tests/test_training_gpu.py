@@ -270,6 +270,55 @@ def test_attention_packed(lens, lead, tail, hint, dtype):
     _check_attention(*x, dict(cu_seqlens=cut, max_seqlen=hint, dropout_p=p, seed=_seed(), call=6), cu=cu, p=p)
 
 
+# Many heads and sequences of more than 128: the backward pass in one pass over the scores, keys 256 at a time
+@pytest.mark.parametrize("p", [0.0, 0.1])
+@pytest.mark.parametrize("L,kind", [(129, None), (256, "prefix"), (257, "holes"), (290, "tile"), (300, "first"), (300, "last"),
+                                    (300, "alternate"), (260, "none"), (520, "prefix"), (545, None)])
+def test_attention_one_pass_dense(L, kind, p):
+    B, H = 4, 64
+    m = None if kind is None else _mask(kind, B, L)
+    x = [_rand(100 + i, B, L, H, 64, dtype=BF16) for i in range(4)]
+    kw = dict(dropout_p=p, seed=_seed() if p else None, call=6)
+    if m is not None:
+        kw["mask"] = m.to(_dev())
+    _check_attention(*x, kw, mask=m, p=p)
+
+
+@pytest.mark.parametrize("lens,lead,tail,hint", [([300, 20, 1, 256], 0, 0, 300), ([0, 257, 130, 5], 3, 70, None), ([150, 520, 40, 33], 0, 2, 150)])
+def test_attention_one_pass_packed(lens, lead, tail, hint):
+    cu = [lead]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    total, H, p = cu[-1] + tail, 64, 0.1
+    x = [_rand(110 + i, total, H, 64, dtype=BF16) for i in range(4)]
+    for t64, t in x:
+        for rows in (slice(0, lead), slice(cu[-1], total)):
+            t64[rows] = 0
+            t[rows] = float("nan")
+    cut = torch.tensor(cu, dtype=torch.int32, device=_dev())
+    _check_attention(*x, dict(cu_seqlens=cut, max_seqlen=hint, dropout_p=p, seed=_seed(), call=6), cu=cu, p=p)
+
+
+def test_one_pass_masked_keys_reach_nothing_whatever_they_hold():
+    from otter_amd import training as T
+    B, L, H = 4, 270, 64
+    m = _mask("holes", B, L).to(_dev())
+    m[3] = 0
+    x = [torch.randn(B, L, H, 64, device=_dev()).to(BF16) for _ in range(4)]
+    q, k, v, do = x
+    kw = dict(mask=m, dropout_p=0.1, seed=_seed(), call=6)
+    out, lse = T.attention_forward(q, k, v, **kw)
+    grads = T.attention_backward(do, q, k, v, out, lse, **kw)
+    for bad in (float("nan"), float("inf"), torch.finfo(BF16).min):
+        k2, v2, q2 = k.clone(), v.clone(), q.clone()
+        live = m.any(1, keepdim=True).expand_as(m)
+        k2[m == 0] = bad                                        # of the sequence that leaves nothing: k and q, not v
+        v2[(m == 0) & live] = bad
+        q2[3] = bad
+        out2, lse2 = T.attention_forward(q2, k2, v2, **kw)
+        _same((out2, lse2, *T.attention_backward(do, q2, k2, v2, out2, lse2, **kw)), (out, lse, *grads))
+
+
 def test_packed_and_dense_agree_bit_for_bit():
     from otter_amd import training as T
     dev, H = _dev(), 3
@@ -321,6 +370,14 @@ def test_attention_large_scores_and_scale():
     _check_attention(q, k, v, do, dict(scale=0.3), scale=0.3)
     _check_attention(q, k, v, do, dict(scale=-0.01), scale=-0.01)
     _check_attention(q, k, v, do, dict(scale=0.0), scale=0.0)
+    m = _mask("holes", 1, 100)
+    for scale in (0.0, -0.3, 0.3):
+        _check_attention(q, k, v, do, dict(scale=scale, mask=m.to(_dev())), mask=m, scale=scale)
+    # scores far below zero throughout
+    low = (q[0].abs(), q[1].abs()), (-k[0].abs(), -k[1].abs())
+    _check_attention(*low, v, do, dict(mask=m.to(_dev())), mask=m)
+    low = [tuple(t[0].to(BF16).double() if i == 0 else t[1].to(BF16) for i in range(2)) for t in (*low, v, do)]
+    _check_attention(*low, dict(mask=m.to(_dev())), mask=m)
 
 
 def test_attention_autograd_and_broadcast_inputs():
