@@ -24,6 +24,7 @@ using namespace otter;
 
 constexpr int DH = 64;         // head dimension
 constexpr int TR = 64;         // rows of a streamed tile
+constexpr int CUS = 256;       // compute units of the chip
 constexpr int OWN = 128;       // rows a workgroup owns: 4 waves x 32
 
 struct View {                  // element strides of a [batch, token, head, 64] tensor (batch stride unused when packed)
@@ -681,6 +682,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
 // into dV and dK as in attn_dkv_kernel, dS also goes to LDS (64 bytes a key), from where all waves together make the tile's
 // dQ, a block of 16 queries x 16 elements each, with their 16 columns of K^T in registers.  dQ of more than 256 keys is
 // carried in a float32 buffer that the same thread writes and reads.  One barrier a tile; D comes out of the staging.
+// SHORT: batches of short sequences, see D below (in a batch of long ones it would cost 64 x 200 tokens 70 -> 96 us).
 constexpr int FK = 256, FQ = 32;      // keys at a time, rows of a streamed tile
 constexpr int SPITCH = FQ * 2 + 8;    // bytes a key of dS^T in LDS
 
@@ -691,7 +693,7 @@ __device__ __forceinline__ float dppf(float x) {
     return __uint_as_float(quad<CTRL>(__float_as_uint(x)));
 }
 
-template <bool DROP>
+template <bool DROP, bool SHORT>
 __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
     typedef bf16_t T;
     using X = Tile<T>;
@@ -701,6 +703,7 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
     __shared__ __attribute__((aligned(16))) char sS[2][FK * SPITCH];        // first K's 256 rows, then dS^T of a tile
     __shared__ __attribute__((aligned(16))) float sL[2][FQ], sD[2][FQ];
     __shared__ __attribute__((aligned(16))) char sK[FK * X::PITCH];
+    __shared__ float sE[SHORT ? 2 : 1][FQ];
     const Lane ln;
     const int lane = ln.lane, wave = ln.wave, h = ln.h, l31 = ln.l31, tid = threadIdx.x;
     const int items = a.heads * a.B;
@@ -790,6 +793,28 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
                 float* part = a.delta + ((prow + min(qi, s.len - 1)) * a.heads + s.h) * DH + dcol + 4 * g4;
                 f32x4 dq = {0.f, 0.f, 0.f, 0.f};
                 if (!first) dq = *reinterpret_cast<const f32x4*>(part);
+                if (SHORT && kend <= 2 * 32 && !even) {    // D of short rows without O's rounding, as in attn_dq_kernel
+                    if (busy) {
+                        f32x16 sc, dp;
+                        row_products<T>(sc, dp, sQ[buf] + ln.frag<T>(), kf, sO[buf] + ln.frag<T>(), vf);
+                        Draws w;
+                        if constexpr (DROP) w.keys(a.drop, key.k0, key.k1, bh, j, i0, h);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const bool in = counts && (!DROP || w.kept_k(r));
+                            float e = in ? exp2_(fmaf(sc[r], a.c2, -sL[buf][acc_row(r, h)])) * dp[r] * a.drop.scale : 0.0f;
+                            e += dppf<0xB1>(e);
+                            e += dppf<0x4E>(e);
+                            e += dppf<0x141>(e);
+                            e += dppf<0x140>(e);
+                            e += __shfl_xor(e, 16);
+                            if (l31 == 0) sE[wave & (SHORT ? 1 : 0)][acc_row(r, h)] = e;
+                        }
+                    }
+                    __syncthreads();
+                    if (tid < FQ) sD[buf][tid] = sE[0][tid] + (kend > 32 ? sE[SHORT ? 1 : 0][tid] : 0.0f);
+                    __syncthreads();
+                }
                 if (busy) {
                     f32x16 sc, dp;
                     row_products<T>(sc, dp, sQ[buf] + ln.frag<T>(), kf, sO[buf] + ln.frag<T>(), vf);
@@ -925,12 +950,28 @@ void launch_fwd(const AttnTrainArgs& a, int grid, hipStream_t st) {
         attn_fwd_kernel<T, false><<<grid, 256, 0, st>>>(a);
 }
 
-// One pass over the scores (bfloat16) or two, one for dQ and one for dK and dV.  One pass makes each score tile once, but has only
-// one workgroup a (sequence, head), the chip to itself at 256 of them, and more to synchronise: 128 packed sequences of 64 to
-// 512, 12 heads, dropout 323 us (two passes 420), without dropout 289 (335); 16 x 512, 12 heads (192 workgroups) 86 us (92)
-// with, 72 (69) without.  Short sequences (up to OWN) are one workgroup a (sequence, head) either way.
+// One pass over the scores (bfloat16) or two, one for dQ and one for dK and dV.  One pass makes each score tile once and is one
+// launch, but it is one workgroup a (sequence, head) of which a CU holds one, and it needs FK keys to fill its waves.  Measured
+// (us, one pass and two, 12 heads, dropout):
+//   up to OWN tokens        16 x 70: 19 and 21, 16 x 128: 17.5 and 20.6; 64 x 70: 53 and 39        -> while the CUs hold all pairs
+//   up to FK                16 x 200: 26.5 and 38, 64 x 200: 70 and 92, 4 x 150, 4 heads: 18 and 22 -> always
+//   longer                  128 packed up to 512: 323 and 420, 16 x 512: 87 and 92, 40 packed: 139 and 143; but 32 x 512 (one and a
+//                           half rounds of workgroups): 163 and 145, 2 x 4001: 626 and 502 -> where the last round is not mostly empty
+// Several workgroups a pair, whose parts of dQ another launch adds up, did not help (16 x 512: 97).
 bool one_pass(const AttnTrainArgs& a, int dtype) {
-    return dtype == OTTER_BF16 && a.L > OWN && (long long)a.B * a.heads >= (a.drop.thr ? 192 : 256);
+    const long long pairs = (long long)a.B * a.heads;
+    if (dtype != OTTER_BF16) return false;
+    if (a.L <= FK) return a.L > OWN || pairs <= CUS;
+    const long long slots = (pairs + CUS - 1) / CUS * CUS;
+    return slots == CUS ? 4 * pairs >= 3 * slots : 5 * pairs >= 4 * slots;
+}
+
+template <bool DROP>
+void launch_one_pass(const AttnTrainArgs& a, int grid, hipStream_t st) {
+    if (a.L <= OWN)
+        attn_bwd_kernel<DROP, true><<<grid, 512, 0, st>>>(a);
+    else
+        attn_bwd_kernel<DROP, false><<<grid, 512, 0, st>>>(a);
 }
 
 template <typename T>
@@ -1013,9 +1054,9 @@ int otter_attention_backward(int device, const otter_attention_args* x, void* st
         a.nblk = 1;
         const int n = a.heads * a.B + (a.cu ? a.heads : 0);
         if (a.drop.thr)
-            attn_bwd_kernel<true><<<n, 512, 0, st>>>(a);
+            launch_one_pass<true>(a, n, st);
         else
-            attn_bwd_kernel<false><<<n, 512, 0, st>>>(a);
+            launch_one_pass<false>(a, n, st);
         OTTER_HIP_TRY(hipGetLastError());
         return OTTER_OK;
     }
