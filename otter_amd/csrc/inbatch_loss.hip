@@ -24,6 +24,7 @@ struct LossArgs {
     float* scores;                 // [B][ld]
     float* part;                   // [splits][B][B] when splits > 1
     float *lse, *rowloss, *loss;   // [B], [B], [1]
+    unsigned* done;                // rows whose loss is there: cleared by the scores' launch, counted by the rows'
     const float* dloss;            // [1]
     float *dq, *dc, *dneg;
     int B, d, ld, splits, kchunk;
@@ -186,6 +187,7 @@ __global__ __launch_bounds__(256) void loss_scores_kernel(LossArgs a) {
     const int nt = (a.B + BM - 1) / BM;
     const int t = xcd_remap(blockIdx.x, gridDim.x);
     const int m0 = (t / nt) * BM, n0 = (t % nt) * BM;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.done = 0;
     const int ka = blockIdx.y * a.kchunk, kb = min(a.d, ka + a.kchunk);
     f32x16 acc[BM / 64][BM / 64];
     clear<BM>(acc);
@@ -204,10 +206,14 @@ __device__ __forceinline__ void online(float& m, float& l, float m2, float l2) {
     m = n;
 }
 
-// one workgroup a row: the pieces of S summed in order (PIECES), the hard negative's score, lse and the row's loss
+// one workgroup a row: the pieces of S summed in order (PIECES), the hard negative's score, lse and the row's loss; of a
+// small batch the last workgroup takes the mean as well (B = 64: 19.6 -> 16.5 us without the launch for it; the fence in front of
+// the count is dear where much was just written, B = 4096: 160 -> 240)
 template <bool PIECES>
 __global__ __launch_bounds__(256) void loss_rows_kernel(LossArgs a) {
     __shared__ float sm[4], sl[4], sd[4];
+    __shared__ double sum[4];
+    __shared__ bool last;
     const int i = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float* row = a.scores + (long long)i * a.ld;
     float m = -INFINITY, l = 0.0f;
@@ -258,7 +264,23 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossArgs a) {
         const float lse = m + __logf(l);
         a.lse[i] = lse;
         a.rowloss[i] = lse - row[i];
+        if (PIECES) {
+            __threadfence();                               // the row's loss before the count of it
+            last = atomicAdd(a.done, 1u) == (unsigned)a.B - 1u;
+        }
     }
+    if (!PIECES) return;
+    __syncthreads();
+    if (!last) return;
+    // the workgroup that finished last takes the mean, in one fixed order whichever it is
+    __threadfence();
+    double s = 0.0;
+    for (int k = threadIdx.x; k < a.B; k += 256) s += (double)__builtin_nontemporal_load(a.rowloss + k);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if (lane == 0) sum[wave] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) *a.loss = (float)((sum[0] + sum[1] + sum[2] + sum[3]) / a.B);
 }
 
 __global__ __launch_bounds__(1024) void loss_mean_kernel(LossArgs a) {
@@ -622,6 +644,7 @@ SplitArgs split_args(const float* q, const float* c, int B, int d) {
 int64_t lay_forward(void* ws, LossArgs& a, SplitArgs& s) {
     Take t{(char*)ws};
     a.rowloss = t.template operator()<float>(a.B);
+    a.done = t.template operator()<unsigned>(1);
     if (loss_planes(a.B, a.d)) {
         s.qs = t.template operator()<float>(s.Bp);
         s.cs = t.template operator()<float>(s.Bp);
@@ -694,11 +717,12 @@ int otter_inbatch_loss_forward(int device, const float* q, const float* c, const
         const unsigned nt = (unsigned)(B + 63) / 64;
         loss_scores_kernel<64><<<dim3(nt * nt, (unsigned)a.splits), 256, 0, st>>>(a);
     }
-    if (a.splits > 1)
+    if (a.splits > 1) {
         loss_rows_kernel<true><<<B, 256, 0, st>>>(a);
-    else
+    } else {
         loss_rows_kernel<false><<<B, 256, 0, st>>>(a);
-    loss_mean_kernel<<<1, 1024, 0, st>>>(a);
+        loss_mean_kernel<<<1, 1024, 0, st>>>(a);
+    }
     OTTER_HIP_TRY(hipGetLastError());
     return OTTER_OK;
 }

@@ -234,13 +234,18 @@ __device__ __forceinline__ void make_z(const NormArgs& a, const RowLoad<T, VEC, 
         unpack<T>(x.r[i], z[i]);
         if (a.drop.thr) {
             keep[i] = keep8((u32)(c >> 3), (u32)row, a.drop, k0, k1);
-            apply_keep(z[i], keep[i], a.drop.scale);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[i][e] = (keep[i] >> e) & 1u ? z[i][e] : 0.0f;
         }
+        // written out as one fma, as are the sums below: a row's bits do not depend on how it is aligned
         if (a.residual) {
             float r[8];
             unpack<T>(res.r[i], r);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z[i][e] += r[e];
+            for (int e = 0; e < 8; ++e) z[i][e] = fmaf(z[i][e], a.drop.scale, r[e]);
+        } else if (a.drop.thr) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[i][e] *= a.drop.scale;
         }
         if (c + 8 > a.cols) {
 #pragma unroll
@@ -306,11 +311,11 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(NormArgs a) {
             for (int e = 0; e < 8; ++e) {
                 const float d = z[i][e] - mean;
                 z[i][e] = d;
-                if (VEC ? c < a.cols : c + e < a.cols) v += d * d;
+                v = fmaf(d, (VEC ? c < a.cols : c + e < a.cols) ? d : 0.0f, v);
             }
         }
         row_sum2<LPR>(v, dummy, lds);
-        const float rstd = 1.0f / sqrtf(v * inv + a.eps);
+        const float rstd = 1.0f / sqrtf(fmaf(v, inv, a.eps));
         if (!in) continue;
         if (l == 0) {
             a.mean[row] = mean;
@@ -396,7 +401,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(NormArgs a) {
             if (n <= 0) continue;
             float o[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = rs * (dy[i][e] - m1 - z[i][e] * m2);
+            for (int e = 0; e < 8; ++e) o[e] = rs * fmaf(-z[i][e], m2, dy[i][e] - m1);
             if (a.dresidual) store8<T, VEC>((T*)a.dresidual + row * a.cols + c, n, o);
             if (a.drop.thr) apply_keep(o, keep[i], a.drop.scale);
             store8<T, VEC>((T*)a.dx + row * a.cols + c, n, o);

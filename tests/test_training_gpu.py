@@ -139,6 +139,18 @@ def test_layer_norm_shapes_strides_and_empty():
     assert y.shape == (6, 4, 40) and mean.shape == (6, 4) and torch.equal(y, z.transpose(0, 1))
     u = torch.randn(4 * 40 + 1, device=dev)[1:].view(4, 40)     # 4-byte aligned
     assert torch.equal(T.layer_norm_forward(u, w, b)[0], T.layer_norm_forward(u.clone(), w, b)[0])
+    # the bits of a row do not depend on its alignment, with everything switched on either
+    for dt in (F32, BF16):
+        g = torch.Generator(device=dev).manual_seed(7)
+        big = [torch.randn(300 * 768 + 1, generator=g, device=dev).to(dt) for _ in range(3)]
+        w2, b2 = torch.randn(768, generator=g, device=dev), torch.randn(768, generator=g, device=dev)
+        res = []
+        for o in (0, 1):
+            x2, r2, d2 = (t[1:].view(300, 768) if o else t[1:].clone().view(300, 768) for t in big)
+            kw = dict(residual=r2, dropout_p=0.2, seed=_seed(), call=4)
+            f = T.layer_norm_forward(x2, w2, b2, **kw)
+            res.append((*f, *T.layer_norm_backward(d2, x2, w2, f[1], f[2], **kw)))
+        _same(res[0], res[1])
     y, mean, rstd = T.layer_norm_forward(x[:0], w, b)
     dx, dres, dw, db = T.layer_norm_backward(x[:0], x[:0], w, mean, rstd)
     assert y.shape == dx.shape == (0, 6, 40) and dres is None and (dw == 0).all() and (db == 0).all()
