@@ -402,7 +402,8 @@ typedef struct otter_attention_args {
     otter_view q, k, v, out;
     float* lse;
     otter_view dout, dq, dk, dv;      /* backward only */
-    void* workspace;                  /* backward only: otter_attention_backward_workspace() bytes */
+    void* workspace;                  /* backward only: otter_attention_backward_workspace() bytes, 16-byte
+                                       * aligned (may be 0) */
     int64_t workspace_bytes;
 } otter_attention_args;
 

@@ -409,7 +409,7 @@ __global__ __launch_bounds__(256) void loss_split_kernel(SplitArgs a) {
 
 // G 2^14 as two planes [Bp][Bp], zeros outside [B][B]
 __global__ __launch_bounds__(256) void loss_gplanes_kernel(LossArgs a, unsigned short* hi, unsigned short* lo, int Bp) {
-    const int i = blockIdx.y, j = (blockIdx.x * 256 + threadIdx.x) * 4;
+    const int nb = (Bp + 1023) / 1024, i = blockIdx.x / nb, j = (blockIdx.x % nb * 256 + threadIdx.x) * 4;
     if (j >= Bp) return;
     const Grad G{a.scores, a.lse, a.ld, a.B, 16384.0f};
     const f4u v = G(i, j);
@@ -767,7 +767,7 @@ int otter_inbatch_loss_backward(int device, const float* dloss, const float* q, 
         lay_backward(workspace, s, gp);
         loss_top_kernel<<<dim3(NMAX, 2), 256, 0, st>>>(s);
         loss_split_kernel<true><<<dim3((unsigned)(s.Bp / 4), 2), 256, 0, st>>>(s);
-        loss_gplanes_kernel<<<dim3((unsigned)(s.Bp + 1023) / 1024, (unsigned)s.Bp), 256, 0, st>>>(a, gp[0], gp[1], s.Bp);
+        loss_gplanes_kernel<<<(unsigned)s.Bp * ((unsigned)(s.Bp + 1023) / 1024), 256, 0, st>>>(a, gp[0], gp[1], s.Bp);
         loss_grad16_kernel<<<(unsigned)(2 * (s.Bp / 128) * ((d + 63) / 64)), 256, 0, st>>>(a, s, gp[0], gp[1]);
     } else {
         loss_grad_kernel<64><<<(unsigned)(2 * tiles), 256, 0, st>>>(a);

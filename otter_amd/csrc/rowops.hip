@@ -117,7 +117,7 @@ struct DropoutArgs {
 
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
-    const u64 seed = (u64)*a.drop.seed;
+    const u64 seed = a.drop.thr ? (u64)*a.drop.seed : 0;
     const u32 k0 = (u32)seed, k1 = (u32)(seed >> 32);
     const long long step = (long long)gridDim.x * 256;
     long long g = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -542,7 +542,6 @@ int otter_dropout(int device, int dtype, const void* x, void* y, int64_t rows, i
     if (rc) return rc;
     if (rows == 0 || cols == 0) return OTTER_OK;
     if (!x || !y) return set_err(OTTER_EINVAL, "dropout: NULL buffer");
-    if (!seed) return set_err(OTTER_EINVAL, "dropout: needs a seed");
     DeviceGuard g(device);
     if (!g.ok) return set_err(OTTER_EHIP, "dropout: hipSetDevice(%d) failed", device);
     a.x = x;

@@ -496,6 +496,8 @@ def test_inbatch_loss(B, d, neg):
     again = IB.inbatch_loss_forward(q, c, n)
     _same(again, (loss, product, lse))
     _same(IB.inbatch_loss_backward(dloss, q, c, n, product, lse), (dq, dc, dneg))
+    # a contiguous copy of the scores does as well (rows that are not whole 16-byte pieces)
+    _same(IB.inbatch_loss_backward(dloss, q, c, n, product.contiguous(), lse), (dq, dc, dneg))
     if B <= 513:                                                # the matrix of the dev-set evaluation, in the same order
         P, _ = IB.inbatch_scores(q, c, n)
         assert (P - product).abs().max().item() <= 2 * float(ref["product"][1].max())
@@ -524,6 +526,34 @@ def test_inbatch_loss_of_small_and_large_embeddings(B, scale):
     dq, dc, _ = IB.inbatch_loss_backward(torch.ones((), device=_dev()), q, c, None, product, lse)
     for name, t in (("loss", loss), ("product", product), ("lse", lse), ("dq", dq), ("dc", dc)):
         _close(name, t, ref[name])
+
+
+def test_inbatch_loss_at_its_limit():
+    """B = 65536: offsets past 32 bits; rows and columns here and there against 64 bits."""
+    from otter_amd import inbatch as IB
+    B, d, dev = 65536, 64, _dev()
+    g = torch.Generator(device=dev).manual_seed(5)
+    q, c = (torch.randn(B, d, generator=g, device=dev) * d ** -0.25 for _ in range(2))
+    loss, product, lse = IB.inbatch_loss_forward(q, c)
+    dq, dc, _ = IB.inbatch_loss_backward(torch.ones((), device=dev), q, c, None, product, lse)
+    pick = torch.tensor([0, 1, 32767, 32768, 50001, 65535], device=dev)
+    qd, cd = q.double(), c.double()
+    S = qd[pick] @ cd.t()
+    tol = (d + 8) * R.E32 * float(qd.abs().sum(1).max() * cd.abs().max())     # of a score, and of what follows from it
+    assert (product[pick].double() - S).abs().max() <= tol
+    assert (lse[pick].double() - torch.logsumexp(S, 1)).abs().max() <= tol + (B / 256 + 64) * R.E32
+    rows = torch.logsumexp(qd[:4096] @ cd.t(), 1) - (qd[:4096] * cd[:4096]).sum(1)
+    every = lse.double() - (qd * cd).sum(1)
+    assert (every[:4096] - rows).abs().max() <= 2 * tol + (B / 256 + 64) * R.E32
+    assert abs(loss.double() - every.mean()) <= tol
+    G = torch.exp(S - lse[pick].double()[:, None])
+    G[torch.arange(len(pick), device=dev), pick] -= 1
+    Gc = torch.exp(qd @ cd[pick].t() - lse.double()[:, None])
+    Gc[pick, torch.arange(len(pick), device=dev)] -= 1
+    # a gradient's error: its G's relative one (a score's, twice) over all terms, and the sum's own over B of them
+    rel = 4 * tol + (B / 64 + 64) * R.E32
+    for got, ref, mag in ((dq[pick], G @ cd, G.abs() @ cd.abs()), (dc[pick], Gc.t() @ qd, Gc.abs().t() @ qd.abs())):
+        assert ((got.double() * B - ref).abs() <= rel * mag).all()
 
 
 def test_inbatch_loss_autograd_and_edges():
