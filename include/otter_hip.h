@@ -218,16 +218,17 @@ int otter_inbatch_scores(int device, const float* q, const float* c, const float
  *   G = (exp(S - lse) - 1[j = i]) * *dloss / B,  dq = G c + G_neg neg_c,  dc = G^T q,  dneg = G_neg q
  * All pointers are device pointers: q, c, neg_c (may be NULL) float32 [B, d]; scores float32 [B, ld] with
  * ld >= B + (neg_c != NULL) -- the forward pass fills the first B (+ 1) columns, the backward pass reads them;
- * lse float32 [B]; loss, dloss float32 [1].  1 <= B <= 65536.  Each call needs a workspace of
+ * stats float32 [2, B]: lse, and 1 - the target's probability (what G's diagonal is made of: exp(S_ii - lse_i) - 1 itself
+ * would be all rounding where a row's loss is small); loss, dloss float32 [1].  1 <= B <= 65536.  Each call needs a workspace of
  * otter_inbatch_loss_workspace(B, d) / otter_inbatch_loss_backward_workspace(B, d) bytes (may be 0), 16-byte aligned,
  * for its time (stream order).  Both calls only enqueue; the same inputs give the same bits (no atomics). */
 int64_t otter_inbatch_loss_workspace(int B, int d);
 int64_t otter_inbatch_loss_backward_workspace(int B, int d);
 int otter_inbatch_loss_forward(int device, const float* q, const float* c, const float* neg_c, int B, int d,
-                               float* scores, int ld, float* lse, float* loss, void* workspace,
+                               float* scores, int ld, float* stats, float* loss, void* workspace,
                                int64_t workspace_bytes, void* stream);
 int otter_inbatch_loss_backward(int device, const float* dloss, const float* q, const float* c, const float* neg_c,
-                                int B, int d, const float* scores, int ld, const float* lse, float* dq, float* dc,
+                                int B, int d, const float* scores, int ld, const float* stats, float* dq, float* dc,
                                 float* dneg, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- encoder */

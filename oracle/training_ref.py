@@ -195,7 +195,9 @@ def inbatch_loss(q, c, neg, dloss=1.0):
         aS = torch.cat((aS, (q * neg).abs().sum(1, keepdim=True)), 1)
     n = S.shape[1]
     lse = torch.logsumexp(S, 1)
-    rows = lse - torch.diagonal(S)
+    diag_out = S.clone()
+    diag_out[:, :B].fill_diagonal_(-math.inf)
+    rows = torch.nn.functional.softplus(torch.logsumexp(diag_out, 1) - torch.diagonal(S)) if n > 1 else torch.zeros(B, dtype=torch.float64)
     P = torch.exp(S - lse[:, None])
     eS = (d + 8) * E32 * aS
     spread = (P * eS).sum(1)
@@ -205,9 +207,23 @@ def inbatch_loss(q, c, neg, dloss=1.0):
     g = dloss / B
     one = torch.zeros_like(P)
     one[:, :B] = torch.eye(B, dtype=torch.float64)
-    G = (P - one) * g
-    eG = abs(g) * (P * (eS + elseb[:, None] + (6 * top[:, None] + 8) * E32) + 4 * E32 * (P + one))
-    out = {"loss": (rows.mean(), erow.mean() + 2 * E32 * rows.mean().abs()), "product": (S, eS), "lse": (lse, elseb)}
+    # the diagonal is minus the sum of the other probabilities: no number near 1 is subtracted from 1, nor lse from the target's
+    # score; each term's relative error is that of a difference of two scores (and of lse where the target is not the largest)
+    off = torch.ones_like(P)
+    off[:, :B] -= torch.eye(B, dtype=torch.float64)
+    rest = (P * off).sum(1)
+    rel = eS + elseb[:, None] + (6 * top[:, None] + 8) * E32
+    diag = torch.diagonal(eS)
+    erest = (P * off * rel).sum(1) + rest * (diag + (n + 24 + 6 * top) * E32)
+    largest = torch.diagonal(S) >= S.masked_fill(off == 0, -math.inf).amax(1)
+    erest = torch.where(largest, erest, erest + 4 * E32)
+    erow = torch.where(largest, erest / (1 - rest).clamp(min=0.5) + 4 * E32 * rows, erow)
+    G = P * off * g
+    G[:, :B] -= torch.diag(rest) * g
+    eG = abs(g) * P * off * (rel + 4 * E32)
+    eG[:, :B] += torch.diag(erest + 4 * E32 * rest) * abs(g)
+    out = {"loss": (rows.mean(), erow.mean() + 2 * E32 * rows.mean().abs()), "product": (S, eS), "lse": (lse, elseb),
+           "rest": (rest, erest)}
     A, eA = G[:, :B], eG[:, :B]
     dq, edq = A @ c, eA @ c.abs() + (B + 4) * E32 * (A.abs() @ c.abs())
     out["dc"] = (A.t() @ q, eA.t() @ q.abs() + (B + 4) * E32 * (A.abs().t() @ q.abs()))

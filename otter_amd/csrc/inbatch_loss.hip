@@ -4,6 +4,9 @@
 //   S = [q c^T | q . neg]  (B x B | B x 1),  lse_i = log sum_j exp S_ij,  loss = mean_i (lse_i - S_ii)
 //   G = (exp(S - lse) - 1[j = i]) dloss / B,  dq = G c + G_neg neg,  dc = G^T q,  dneg = G_neg q
 //
+// Where the target has nearly all of a row's weight, lse - S_ii and exp(S_ii - lse) - 1 are differences of nearly equal numbers
+// and a float32 gradient would be mostly rounding.  So the rows' pass keeps the OTHER columns' sum apart: with
+// u = sum_(j != i) exp(S_ij - S_ii), the row's loss is log1p(u) and G_ii = -u / (1 + u) dloss / B, good to float32's last bits.
 // Small batches: the three products run on v_mfma_f32_32x32x2_f32 (an fma chain: no operand is rounded), G is made from S and
 // lse where a product's tile is loaded.  Large ones: every operand is split into two float16 planes, x = (hi + lo) 2^-e with
 // hi + lo good to 22 bits, and hi hi' + hi lo' + lo hi' run on v_mfma_f32_32x32x16_f16, sixteen times float32's rate for
@@ -23,7 +26,8 @@ struct LossArgs {
     const float *q, *c, *neg;      // [B][d]; neg may be null
     float* scores;                 // [B][ld]
     float* part;                   // [splits][B][B] when splits > 1
-    float *lse, *rowloss, *loss;   // [B], [B], [1]
+    float *lse, *rest;             // [B]: of the row; 1 - the target's probability
+    float *rowloss, *loss;         // [B], [1]
     unsigned* done;                // rows whose loss is there: cleared by the scores' launch, counted by the rows'
     const float* dloss;            // [1]
     float *dq, *dc, *dneg;
@@ -51,7 +55,7 @@ struct Plain {                     // a stored matrix
 };
 
 struct Grad {                      // G[i][j .. j + 3] from the scores
-    const float *scores, *lse;
+    const float *scores, *lse, *rest;
     long long ld;
     int B;
     float g;                       // dloss / B
@@ -59,8 +63,7 @@ struct Grad {                      // G[i][j .. j + 3] from the scores
         f4u v = load4(scores, ld, B, B, i, j);
         const float l = i < B ? lse[i] : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            v[e] = i < B && j + e < B ? (__expf(v[e] - l) - (j + e == i ? 1.0f : 0.0f)) * g : 0.0f;
+        for (int e = 0; e < 4; ++e) v[e] = i < B && j + e < B ? (j + e == i ? -rest[i] : __expf(v[e] - l)) * g : 0.0f;
         return v;
     }
 };
@@ -223,7 +226,7 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossArgs a) {
 #pragma unroll 12
             for (int p = 0; p < a.splits; ++p) s += a.part[((size_t)p * a.B + i) * a.B + j];
             row[j] = s;
-            online(m, l, s, 1.0f);
+            if (j != i) online(m, l, s, 1.0f);
         }
     } else {
         // four scores a load: one exponential each and one for the four's maximum
@@ -233,6 +236,9 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossArgs a) {
 #pragma unroll
             for (int e = 1; e < 4; ++e)
                 if (j + e >= a.B) v[e] = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (j + e == i) v[e] = -INFINITY;
             const float top = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), n = fmaxf(m, top), base = n == -INFINITY ? 0.0f : n;
             l = l * __expf(m - base) + ((__expf(v[0] - base) + __expf(v[1] - base)) + (__expf(v[2] - base) + __expf(v[3] - base)));
             m = n;
@@ -261,9 +267,22 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossArgs a) {
             row[a.B] = dot;
             online(m, l, dot, 1.0f);
         }
-        const float lse = m + __logf(l);
+        // m, l: the other columns (l = 0 if there are none)
+        const float t = row[i];
+        float lse, rest, loss;
+        if (m <= t) {
+            const float u = l * __expf(m - t);
+            loss = log1pf(u);
+            lse = t + loss;
+            rest = u / (1.0f + u);
+        } else {
+            lse = m + logf(l + __expf(t - m));
+            loss = lse - t;
+            rest = 1.0f - __expf(t - lse);
+        }
         a.lse[i] = lse;
-        a.rowloss[i] = lse - row[i];
+        a.rest[i] = rest;
+        a.rowloss[i] = loss;
         if (PIECES) {
             __threadfence();                               // the row's loss before the count of it
             last = atomicAdd(a.done, 1u) == (unsigned)a.B - 1u;
@@ -307,7 +326,7 @@ __global__ __launch_bounds__(256) void loss_grad_kernel(LossArgs a) {
     const int t = second ? id - half : id;
     const int m0 = (t / nt) * BM, n0 = (t % nt) * BM;
     const float g = *a.dloss / (float)a.B;
-    const Grad G{a.scores, a.lse, a.ld, a.B, g};
+    const Grad G{a.scores, a.lse, a.rest, a.ld, a.B, g};
     f32x16 acc[BM / 64][BM / 64];
     clear<BM>(acc);
     if (second) {
@@ -341,7 +360,8 @@ struct SplitArgs {
     const float *q, *c;            // [B][d]
     unsigned short* plane[4];      // q hi, q lo, c hi, c lo: [Bp][dp], zeros outside [B][d]
     float *qs, *cs;                // [Bp]: what a row of the planes is to be multiplied by (forward)
-    float* top;                    // [2][NMAX] largest elements (backward: one scale a matrix)
+    float* top;                    // [3][NMAX] largest elements of q, c and G (backward: one scale a matrix)
+    const float* rest;             // [B]: a row of G has no larger element
     int B, d, Bp, dp;
 };
 
@@ -361,8 +381,8 @@ __device__ __forceinline__ void split1(float x, unsigned short& hi, unsigned sho
 
 __global__ __launch_bounds__(256) void loss_top_kernel(SplitArgs a) {
     __shared__ float red[4];
-    const float* x = blockIdx.y ? a.c : a.q;
-    const long long n = (long long)a.B * a.d;
+    const float* x = blockIdx.y == 2 ? a.rest : blockIdx.y ? a.c : a.q;
+    const long long n = blockIdx.y == 2 ? a.B : (long long)a.B * a.d;
     float t = 0.0f;
     // four elements a load, four loads in flight; the last n % 4 by the first threads
     const long long n4 = n / 4, step = (long long)gridDim.x * 256;
@@ -380,6 +400,15 @@ __global__ __launch_bounds__(256) void loss_top_kernel(SplitArgs a) {
     if (threadIdx.x == 0) a.top[blockIdx.y * NMAX + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
+// the largest element of matrix m, in every lane
+__device__ __forceinline__ float matrix_top(const float* top, int m) {
+    float t = 0.0f;
+    for (int i = threadIdx.x & 63; i < NMAX; i += 64) t = fmaxf(t, top[m * NMAX + i]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o));
+    return t;
+}
+
 // one wave a row of one matrix; WHOLE: the scale of the whole matrix, otherwise the row's own
 template <bool WHOLE>
 __global__ __launch_bounds__(256) void loss_split_kernel(SplitArgs a) {
@@ -388,12 +417,12 @@ __global__ __launch_bounds__(256) void loss_split_kernel(SplitArgs a) {
     const float* x = (m ? a.c : a.q) + (long long)row * a.d;
     float t = 0.0f;
     if (WHOLE) {
-        for (int i = lane; i < NMAX; i += 64) t = fmaxf(t, a.top[m * NMAX + i]);
+        t = matrix_top(a.top, m);
     } else if (row < a.B) {
         for (int i = lane; i < a.d; i += 64) t = fmaxf(t, fabsf(x[i]));
-    }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o));
+        for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o));
+    }
     const float f = plane_scale(t);
     unsigned short *hi = a.plane[2 * m] + (long long)row * a.dp, *lo = a.plane[2 * m + 1] + (long long)row * a.dp;
     for (int i = lane; i < a.dp / 4; i += 64) {
@@ -407,11 +436,12 @@ __global__ __launch_bounds__(256) void loss_split_kernel(SplitArgs a) {
     if (lane == 0 && !WHOLE) (m ? a.cs : a.qs)[row] = 1.0f / f;
 }
 
-// G 2^14 as two planes [Bp][Bp], zeros outside [B][B]
-__global__ __launch_bounds__(256) void loss_gplanes_kernel(LossArgs a, unsigned short* hi, unsigned short* lo, int Bp) {
+// G without dloss / B as two planes [Bp][Bp], zeros outside [B][B]
+__global__ __launch_bounds__(256) void loss_gplanes_kernel(LossArgs a, const float* top, unsigned short* hi, unsigned short* lo, int Bp) {
     const int nb = (Bp + 1023) / 1024, i = blockIdx.x / nb, j = (blockIdx.x % nb * 256 + threadIdx.x) * 4;
+    const float f = plane_scale(matrix_top(top, 2));
     if (j >= Bp) return;
-    const Grad G{a.scores, a.lse, a.ld, a.B, 16384.0f};
+    const Grad G{a.scores, a.lse, a.rest, a.ld, a.B, f};
     const f4u v = G(i, j);
     unsigned short h[4], l[4];
 #pragma unroll
@@ -565,11 +595,8 @@ __global__ __launch_bounds__(256, 2) void loss_grad16_kernel(LossArgs a, SplitAr
     const int nt = (a.d + 63) / 64, half = gridDim.x / 2, id = xcd_remap(blockIdx.x, gridDim.x);
     const bool second = id >= half;
     const int t = second ? id - half : id, m0 = (t / nt) * 128, n0 = (t % nt) * 64;
-    float top = 0.0f;
-    for (int i = threadIdx.x & 63; i < NMAX; i += 64) top = fmaxf(top, s.top[(second ? 0 : NMAX) + i]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const float g = *a.dloss / (float)a.B, back = 1.0f / plane_scale(top), gback = g / 16384.0f;
+    const float g = *a.dloss / (float)a.B;
+    const float back = 1.0f / plane_scale(matrix_top(s.top, second ? 0 : 1)), gback = g / plane_scale(matrix_top(s.top, 2));
     f32x16 acc[2][1];
     clear16<1>(acc);
     if (second) {
@@ -658,7 +685,7 @@ int64_t lay_forward(void* ws, LossArgs& a, SplitArgs& s) {
 int64_t lay_backward(void* ws, SplitArgs& s, unsigned short** g) {
     Take t{(char*)ws};
     if (!loss_planes(s.B, s.d)) return 0;
-    s.top = t.template operator()<float>(2 * NMAX);
+    s.top = t.template operator()<float>(3 * NMAX);
     take_planes(t, s);
     g[0] = t.template operator()<unsigned short>((int64_t)s.Bp * s.Bp);
     g[1] = t.template operator()<unsigned short>((int64_t)s.Bp * s.Bp);
@@ -687,10 +714,10 @@ int64_t otter_inbatch_loss_workspace(int B, int d) {
 }
 
 int otter_inbatch_loss_forward(int device, const float* q, const float* c, const float* neg_c, int B, int d, float* scores,
-                               int ld, float* lse, float* loss, void* workspace, int64_t workspace_bytes, void* stream) {
+                               int ld, float* stats, float* loss, void* workspace, int64_t workspace_bytes, void* stream) {
     int rc = check_loss("inbatch_loss_forward", B, d, ld, B + (neg_c ? 1 : 0));
     if (rc) return rc;
-    if (!q || !c || !scores || !lse || !loss) return set_err(OTTER_EINVAL, "inbatch_loss_forward: NULL buffer");
+    if (!q || !c || !scores || !stats || !loss) return set_err(OTTER_EINVAL, "inbatch_loss_forward: NULL buffer");
     if ((rc = check_workspace("inbatch_loss_forward", workspace, workspace_bytes, otter_inbatch_loss_workspace(B, d)))) return rc;
     DeviceGuard g(device);
     if (!g.ok) return set_err(OTTER_EHIP, "inbatch_loss_forward: hipSetDevice(%d) failed", device);
@@ -699,7 +726,8 @@ int otter_inbatch_loss_forward(int device, const float* q, const float* c, const
     a.c = c;
     a.neg = neg_c;
     a.scores = scores;
-    a.lse = lse;
+    a.lse = stats;
+    a.rest = stats + B;
     a.loss = loss;
     a.B = B;
     a.d = d;
@@ -736,11 +764,11 @@ int64_t otter_inbatch_loss_backward_workspace(int B, int d) {
 }
 
 int otter_inbatch_loss_backward(int device, const float* dloss, const float* q, const float* c, const float* neg_c, int B, int d,
-                                const float* scores, int ld, const float* lse, float* dq, float* dc, float* dneg, void* workspace,
+                                const float* scores, int ld, const float* stats, float* dq, float* dc, float* dneg, void* workspace,
                                 int64_t workspace_bytes, void* stream) {
     int rc = check_loss("inbatch_loss_backward", B, d, ld, B + (neg_c ? 1 : 0));
     if (rc) return rc;
-    if (!dloss || !q || !c || !scores || !lse || !dq || !dc || (neg_c && !dneg))
+    if (!dloss || !q || !c || !scores || !stats || !dq || !dc || (neg_c && !dneg))
         return set_err(OTTER_EINVAL, "inbatch_loss_backward: NULL buffer");
     if ((rc = check_workspace("inbatch_loss_backward", workspace, workspace_bytes, otter_inbatch_loss_backward_workspace(B, d)))) return rc;
     const long long tiles = (long long)((B + 63) / 64) * ((d + 63) / 64);
@@ -753,7 +781,8 @@ int otter_inbatch_loss_backward(int device, const float* dloss, const float* q, 
     a.c = c;
     a.neg = neg_c;
     a.scores = const_cast<float*>(scores);
-    a.lse = const_cast<float*>(lse);
+    a.lse = const_cast<float*>(stats);
+    a.rest = a.lse + B;
     a.dq = dq;
     a.dc = dc;
     a.dneg = dneg;
@@ -765,9 +794,10 @@ int otter_inbatch_loss_backward(int device, const float* dloss, const float* q, 
         SplitArgs s = split_args(q, c, B, d);
         unsigned short* gp[2];
         lay_backward(workspace, s, gp);
-        loss_top_kernel<<<dim3(NMAX, 2), 256, 0, st>>>(s);
+        s.rest = a.rest;
+        loss_top_kernel<<<dim3(NMAX, 3), 256, 0, st>>>(s);
         loss_split_kernel<true><<<dim3((unsigned)(s.Bp / 4), 2), 256, 0, st>>>(s);
-        loss_gplanes_kernel<<<(unsigned)s.Bp * ((unsigned)(s.Bp + 1023) / 1024), 256, 0, st>>>(a, gp[0], gp[1], s.Bp);
+        loss_gplanes_kernel<<<(unsigned)s.Bp * ((unsigned)(s.Bp + 1023) / 1024), 256, 0, st>>>(a, s.top, gp[0], gp[1], s.Bp);
         loss_grad16_kernel<<<(unsigned)(2 * (s.Bp / 128) * ((d + 63) / 64)), 256, 0, st>>>(a, s, gp[0], gp[1]);
     } else {
         loss_grad_kernel<64><<<(unsigned)(2 * tiles), 256, 0, st>>>(a);

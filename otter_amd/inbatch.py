@@ -63,8 +63,8 @@ def _loss_operands(what, q, c, neg_c):
 
 def inbatch_loss_forward(q, c, neg_c=None):
     """loss_single (retrieval/criterions.py:10-27): cross entropy of the in-batch scores against their diagonal, mean over the
-    batch.  Returns (loss, product, lse): float32 scalar, the scores [B, B + (neg_c is not None)] and their row-wise
-    logsumexp [B]; the backward pass needs the last two.  B <= 65536."""
+    batch.  Returns (loss, product, stats): float32 scalar, the scores [B, B + (neg_c is not None)] and, [2, B], their
+    row-wise logsumexp and one minus the target's probability; the backward pass needs the last two.  B <= 65536."""
     lib = _lib.load()
     q, c, neg_c = _loss_operands("inbatch_loss", q, c, neg_c)
     dev = q.device
@@ -75,17 +75,17 @@ def inbatch_loss_forward(q, c, neg_c=None):
     if nbytes < 0:
         _lib.check(int(nbytes), "otter_inbatch_loss_workspace")
     buf = torch.empty((B, ld), dtype=torch.float32, device=dev)
-    lse = torch.empty((B,), dtype=torch.float32, device=dev)
+    stats = torch.empty((2, B), dtype=torch.float32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
     _lib.check(lib.otter_inbatch_loss_forward(
         dev.index, q.data_ptr(), c.data_ptr(), None if neg_c is None else neg_c.data_ptr(), B, d, buf.data_ptr(), ld,
-        lse.data_ptr(), loss.data_ptr(), ws.data_ptr(), nbytes, _stream(dev.index)),
+        stats.data_ptr(), loss.data_ptr(), ws.data_ptr(), nbytes, _stream(dev.index)),
         "otter_inbatch_loss_forward")
-    return loss, buf[:, :ncol], lse
+    return loss, buf[:, :ncol], stats
 
 
-def inbatch_loss_backward(dloss, q, c, neg_c, product, lse):
+def inbatch_loss_backward(dloss, q, c, neg_c, product, stats):
     """Gradients (dq, dc, dneg_c or None), float32 [B, d], of inbatch_loss_forward for dloss, the gradient of the loss
     (float32, one element on the GPU)."""
     lib = _lib.load()
@@ -94,9 +94,9 @@ def inbatch_loss_backward(dloss, q, c, neg_c, product, lse):
     B, d = q.shape
     ncol = B + (neg_c is not None)
     if (tuple(product.shape) != (B, ncol) or product.dtype != torch.float32 or product.device != dev
-            or (ncol > 1 and product.stride(1) != 1) or tuple(lse.shape) != (B,) or lse.dtype != torch.float32
-            or lse.device != dev or not lse.is_contiguous()):
-        raise ValueError("inbatch_loss_backward: product and lse must be what inbatch_loss_forward returned")
+            or (ncol > 1 and product.stride(1) != 1) or stats.shape != (2, B)
+            or stats.dtype != torch.float32 or stats.device != dev or not stats.is_contiguous()):
+        raise ValueError("inbatch_loss_backward: product and stats must be what inbatch_loss_forward returned")
     if dloss.numel() != 1 or dloss.dtype != torch.float32 or dloss.device != dev:
         raise ValueError("inbatch_loss_backward: dloss must be one float32 element on %s" % dev)
     ld = product.stride(0) if B > 1 else ncol
@@ -108,7 +108,7 @@ def inbatch_loss_backward(dloss, q, c, neg_c, product, lse):
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
     _lib.check(lib.otter_inbatch_loss_backward(
         dev.index, dloss.data_ptr(), q.data_ptr(), c.data_ptr(), None if neg_c is None else neg_c.data_ptr(), B, d,
-        product.data_ptr(), ld, lse.data_ptr(), dq.data_ptr(), dc.data_ptr(), None if dneg is None else dneg.data_ptr(),
+        product.data_ptr(), ld, stats.data_ptr(), dq.data_ptr(), dc.data_ptr(), None if dneg is None else dneg.data_ptr(),
         None if ws is None else ws.data_ptr(), nbytes,
         _stream(dev.index)), "otter_inbatch_loss_backward")
     return dq, dc, dneg
@@ -117,15 +117,15 @@ def inbatch_loss_backward(dloss, q, c, neg_c, product, lse):
 class _InbatchLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, c, neg_c):
-        loss, product, lse = inbatch_loss_forward(q, c, neg_c)
-        ctx.save_for_backward(q, c, neg_c, product, lse)
+        loss, product, stats = inbatch_loss_forward(q, c, neg_c)
+        ctx.save_for_backward(q, c, neg_c, product, stats)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        q, c, neg_c, product, lse = ctx.saved_tensors
-        dq, dc, dneg = inbatch_loss_backward(dloss.contiguous(), q, c, neg_c, product, lse)
+        q, c, neg_c, product, stats = ctx.saved_tensors
+        dq, dc, dneg = inbatch_loss_backward(dloss.contiguous(), q, c, neg_c, product, stats)
         return dq.to(q.dtype), dc.to(c.dtype), None if dneg is None else dneg.to(neg_c.dtype)
 
 

@@ -486,21 +486,37 @@ def test_inbatch_loss(B, d, neg):
     n64, n = _rand(72, B, d, scale=d ** -0.25) if neg else (None, None)
     dloss = torch.tensor(1.7, device=_dev())
     ref = R.inbatch_loss(q64, c64, n64, float(dloss.double()))
-    loss, product, lse = IB.inbatch_loss_forward(q, c, n)
-    dq, dc, dneg = IB.inbatch_loss_backward(dloss, q, c, n, product, lse)
-    got = {"loss": loss, "product": product, "lse": lse, "dq": dq, "dc": dc}
+    loss, product, stats = IB.inbatch_loss_forward(q, c, n)
+    dq, dc, dneg = IB.inbatch_loss_backward(dloss, q, c, n, product, stats)
+    got = {"loss": loss, "product": product, "lse": stats[0], "rest": stats[1], "dq": dq, "dc": dc}
     if neg:
         got["dneg"] = dneg
     for name, t in got.items():
         _close(name, t, ref[name])
     again = IB.inbatch_loss_forward(q, c, n)
-    _same(again, (loss, product, lse))
-    _same(IB.inbatch_loss_backward(dloss, q, c, n, product, lse), (dq, dc, dneg))
+    _same(again, (loss, product, stats))
+    _same(IB.inbatch_loss_backward(dloss, q, c, n, product, stats), (dq, dc, dneg))
     # a contiguous copy of the scores does as well (rows that are not whole 16-byte pieces)
-    _same(IB.inbatch_loss_backward(dloss, q, c, n, product.contiguous(), lse), (dq, dc, dneg))
+    _same(IB.inbatch_loss_backward(dloss, q, c, n, product.contiguous(), stats), (dq, dc, dneg))
     if B <= 513:                                                # the matrix of the dev-set evaluation, in the same order
         P, _ = IB.inbatch_scores(q, c, n)
         assert (P - product).abs().max().item() <= 2 * float(ref["product"][1].max())
+
+
+@pytest.mark.parametrize("B", [2, 40, 640])
+@pytest.mark.parametrize("margin", [5.0, 16.0, 40.0])
+def test_inbatch_loss_of_confident_rows(B, margin):
+    """Targets far above the other columns: a loss of e^-margin and gradients as small keep their relative precision."""
+    from otter_amd import inbatch as IB
+    c64 = torch.nn.functional.normalize(_rand(94, B, 128)[0], dim=1).float().double()
+    q64 = (margin * c64).float().double()
+    ref = R.inbatch_loss(q64, c64, None, 1.0)
+    q, c = q64.float().to(_dev()), c64.float().to(_dev())
+    loss, product, stats = IB.inbatch_loss_forward(q, c)
+    dq, dc, _ = IB.inbatch_loss_backward(torch.ones((), device=_dev()), q, c, None, product, stats)
+    for name, t in (("loss", loss), ("rest", stats[1]), ("dq", dq), ("dc", dc)):
+        _close(name, t, ref[name])
+    assert float(loss) > 0
 
 
 @pytest.mark.parametrize("B", [40, 640])
@@ -511,9 +527,9 @@ def test_inbatch_loss_of_small_and_large_embeddings(B, scale):
     q64, q = _rand(90, B, 128, scale=scale * 128 ** -0.25)
     c64, c = _rand(91, B, 128, scale=128 ** -0.25 / scale)
     ref = R.inbatch_loss(q64, c64, None, 1.0)
-    loss, product, lse = IB.inbatch_loss_forward(q, c)
-    dq, dc, _ = IB.inbatch_loss_backward(torch.ones((), device=_dev()), q, c, None, product, lse)
-    for name, t in (("loss", loss), ("product", product), ("lse", lse), ("dq", dq), ("dc", dc)):
+    loss, product, stats = IB.inbatch_loss_forward(q, c)
+    dq, dc, _ = IB.inbatch_loss_backward(torch.ones((), device=_dev()), q, c, None, product, stats)
+    for name, t in (("loss", loss), ("product", product), ("lse", stats[0]), ("dq", dq), ("dc", dc)):
         _close(name, t, ref[name])
     # rows of very different sizes
     row = torch.logspace(-3, 3, B, dtype=torch.float64)[:, None]
@@ -522,9 +538,9 @@ def test_inbatch_loss_of_small_and_large_embeddings(B, scale):
     c64, c = _rand(93, B, 128, scale=1e-3)
     ref = R.inbatch_loss(q64, c64, None, 1.0)
     q = q64.float().to(_dev())
-    loss, product, lse = IB.inbatch_loss_forward(q, c)
-    dq, dc, _ = IB.inbatch_loss_backward(torch.ones((), device=_dev()), q, c, None, product, lse)
-    for name, t in (("loss", loss), ("product", product), ("lse", lse), ("dq", dq), ("dc", dc)):
+    loss, product, stats = IB.inbatch_loss_forward(q, c)
+    dq, dc, _ = IB.inbatch_loss_backward(torch.ones((), device=_dev()), q, c, None, product, stats)
+    for name, t in (("loss", loss), ("product", product), ("lse", stats[0]), ("dq", dq), ("dc", dc)):
         _close(name, t, ref[name])
 
 
@@ -534,8 +550,9 @@ def test_inbatch_loss_at_its_limit():
     B, d, dev = 65536, 64, _dev()
     g = torch.Generator(device=dev).manual_seed(5)
     q, c = (torch.randn(B, d, generator=g, device=dev) * d ** -0.25 for _ in range(2))
-    loss, product, lse = IB.inbatch_loss_forward(q, c)
-    dq, dc, _ = IB.inbatch_loss_backward(torch.ones((), device=dev), q, c, None, product, lse)
+    loss, product, stats = IB.inbatch_loss_forward(q, c)
+    dq, dc, _ = IB.inbatch_loss_backward(torch.ones((), device=dev), q, c, None, product, stats)
+    lse = stats[0]
     pick = torch.tensor([0, 1, 32767, 32768, 50001, 65535], device=dev)
     qd, cd = q.double(), c.double()
     S = qd[pick] @ cd.t()
@@ -576,14 +593,14 @@ def test_inbatch_loss_autograd_and_edges():
         _close(name, t, (ref[name][0], ref[name][1] + R.half_step(BF16) * ref[name][0].abs()))
     # scores of thousands: the softmax is one-hot, the gradient exactly so
     big = torch.eye(8, device=dev) * 100.0
-    loss, product, lse = IB.inbatch_loss_forward(big, big)
-    assert loss.item() == 0.0 and all((g == 0).all() for g in IB.inbatch_loss_backward(torch.ones((), device=dev), big, big, None, product, lse)[:2])
+    loss, product, stats = IB.inbatch_loss_forward(big, big)
+    assert loss.item() == 0.0 and all((g == 0).all() for g in IB.inbatch_loss_backward(torch.ones((), device=dev), big, big, None, product, stats)[:2])
     with pytest.raises(ValueError, match="mean over no rows"):
         IB.inbatch_loss(torch.zeros((0, 8), device=dev), torch.zeros((0, 8), device=dev))
     with pytest.raises(ValueError, match="B, d"):
         IB.inbatch_loss(torch.zeros((3, 8), device=dev), torch.zeros((4, 8), device=dev))
     with pytest.raises(ValueError, match="returned"):
-        IB.inbatch_loss_backward(torch.ones((), device=dev), big, big, big, product, lse)
+        IB.inbatch_loss_backward(torch.ones((), device=dev), big, big, big, product, stats)
 
 
 # ------------------------------------------------------------------------------------ streams, graphs and a whole layer
@@ -599,8 +616,8 @@ def _step(T, IB, W, x, mask, dy, seed):
     y, mean, rstd = T.layer_norm_forward(a, W["g"], W["b"], 1e-5, e, p, seed, 2)
     emb = y[:, 0].float()
     n = B // 2
-    loss, product, llse = IB.inbatch_loss_forward(emb[:n], emb[n:])
-    dq, dc, _ = IB.inbatch_loss_backward(torch.ones_like(loss), emb[:n], emb[n:], None, product, llse)
+    loss, product, stats = IB.inbatch_loss_forward(emb[:n], emb[n:])
+    dq, dc, _ = IB.inbatch_loss_backward(torch.ones_like(loss), emb[:n], emb[n:], None, product, stats)
     dyy = dy.clone()
     dyy[:, 0] += torch.cat((dq, dc)).to(dy.dtype)
     da, de, dg, db = T.layer_norm_backward(dyy, a, W["g"], mean, rstd, e, p, seed, 2)
