@@ -100,6 +100,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_calls = None
 
 
 class OtterError(RuntimeError):
@@ -128,6 +129,24 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def calls():
+    """otter_amd._calls (csrc/calls.cpp), the host side of the training operators, bound to the library.  Raises if it has not
+    been built."""
+    global _calls
+    if _calls is not None:
+        return _calls
+    load()
+    import torch
+    try:
+        from . import _calls as m
+    except ImportError as e:
+        raise OtterError("otter_amd/_calls.so cannot be loaded (%s): build it with `python -m otter_amd.build`" % e)
+    # the handle of a device's current stream: torch.cuda.current_stream() builds an object around it, 2 us
+    m.load(LIB_PATH, check, torch._C._cuda_getCurrentRawStream)
+    _calls = m
+    return m
 
 
 def check(rc, what=""):

@@ -3,7 +3,8 @@
     python -m otter_amd.build [--force]
 
 The library is a plain C-ABI shared object (include/otter_hip.h); it links no torch
-symbols and is loaded with ctypes (otter_amd/_lib.py).
+symbols and is loaded with ctypes (otter_amd/_lib.py).  Beside it a Python module, _calls.so,
+compiled by the host compiler against torch: the host side of the training operators' calls.
 """
 import os
 import re
@@ -13,10 +14,12 @@ import sys
 _PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_PKG, "csrc")
 LIB = os.path.join(_PKG, "libotter_hip.so")
+CALLS = os.path.join(_PKG, "_calls.so")
 OBJDIR = os.path.join(_PKG, "csrc", "_obj")
 SOURCES = ["common.hip", "index.hip", "encoder.hip", "gemm_bf16.hip", "rowops.hip", "attention.hip", "inbatch_loss.hip"]
 HEADERS = ["otter_common.h", "otter_device.h", "otter_gemm.h", "otter_philox.h", os.path.join("..", "..", "include", "otter_hip.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+CXX = os.environ.get("CXX", "g++")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-pthread", "-Wall", "-Wno-unused-function",
          "-Rpass-analysis=kernel-resource-usage",
          # no packed float32 instructions: some of their forms have given wrong results on this hardware
@@ -49,6 +52,26 @@ def check_no_spill(remarks, names=NO_SPILL):
                 bad.append("%s (%s bytes/lane)" % (name, m.group(1)))
             name = None
     return bad
+
+
+def build_calls(force=False, verbose=True):
+    """otter_amd/_calls.so from csrc/calls.cpp."""
+    src = os.path.join(CSRC, "calls.cpp")
+    if not force and _mtime(CALLS) >= max(_mtime(src), _mtime(os.path.join(CSRC, "..", "..", "include", "otter_hip.h"))):
+        return CALLS
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    libs = cpp_extension.library_paths()
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-pthread", "-Wall", "-fvisibility=hidden",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
+    cmd += ["-isystem" + d for d in cpp_extension.include_paths() + [sysconfig.get_paths()["include"]]]
+    cmd += [src, "-o", CALLS] + ["-L" + d for d in libs] + ["-Wl,-rpath," + d for d in libs]
+    cmd += ["-ltorch_python", "-ltorch_cpu", "-lc10", "-ldl"]
+    if verbose:
+        print("[otter_amd.build]", " ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return CALLS
 
 
 def build_lib(force=False, verbose=True):
@@ -103,4 +126,5 @@ def build_lib(force=False, verbose=True):
 
 if __name__ == "__main__":
     build_lib(force="--force" in sys.argv)
+    build_calls(force="--force" in sys.argv)
     print(LIB)

@@ -21,8 +21,6 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 
-_stream = torch._C._cuda_getCurrentRawStream     # a device's current stream, without an object around it
-
 
 def inbatch_scores(q, c, neg_c=None):
     """q, c, neg_c: float32 [B, d] tensors on one GPU.  Returns (product float32 [B, B + (neg_c is not None)],
@@ -49,69 +47,17 @@ def inbatch_scores(q, c, neg_c=None):
     return product, rank
 
 
-def _loss_operands(what, q, c, neg_c):
-    if not (torch.is_tensor(q) and q.is_cuda):
-        raise ValueError("%s: q must be a tensor on a GPU (the HIP path has no CPU fallback)" % what)
-    if q.dim() != 2 or c.shape != q.shape or (neg_c is not None and neg_c.shape != q.shape):
-        raise ValueError("%s: q, c and neg_c must all be [B, d]; got %s %s %s" % (
-            what, tuple(q.shape), tuple(c.shape), None if neg_c is None else tuple(neg_c.shape)))
-    if c.device != q.device or (neg_c is not None and neg_c.device != q.device):
-        raise ValueError("%s: q, c and neg_c must be on one GPU" % what)
-    f32 = torch.float32
-    return [t if t is None or (t.dtype == f32 and t.is_contiguous()) else t.to(f32).contiguous() for t in (q, c, neg_c)]
-
-
 def inbatch_loss_forward(q, c, neg_c=None):
     """loss_single (retrieval/criterions.py:10-27): cross entropy of the in-batch scores against their diagonal, mean over the
     batch.  Returns (loss, product, stats): float32 scalar, the scores [B, B + (neg_c is not None)] and, [2, B], their
     row-wise logsumexp and one minus the target's probability; the backward pass needs the last two.  B <= 65536."""
-    lib = _lib.load()
-    q, c, neg_c = _loss_operands("inbatch_loss", q, c, neg_c)
-    dev = q.device
-    B, d = q.shape
-    ncol = B + (neg_c is not None)
-    ld = (ncol + 3) // 4 * 4                  # rows of whole 16-byte pieces
-    nbytes = lib.otter_inbatch_loss_workspace(B, d)
-    if nbytes < 0:
-        _lib.check(int(nbytes), "otter_inbatch_loss_workspace")
-    buf = torch.empty((B, ld), dtype=torch.float32, device=dev)
-    stats = torch.empty((2, B), dtype=torch.float32, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-    _lib.check(lib.otter_inbatch_loss_forward(
-        dev.index, q.data_ptr(), c.data_ptr(), None if neg_c is None else neg_c.data_ptr(), B, d, buf.data_ptr(), ld,
-        stats.data_ptr(), loss.data_ptr(), ws.data_ptr(), nbytes, _stream(dev.index)),
-        "otter_inbatch_loss_forward")
-    return loss, buf[:, :ncol], stats
+    return _lib.calls().inbatch_loss_forward(q, c, neg_c)
 
 
 def inbatch_loss_backward(dloss, q, c, neg_c, product, stats):
     """Gradients (dq, dc, dneg_c or None), float32 [B, d], of inbatch_loss_forward for dloss, the gradient of the loss
     (float32, one element on the GPU)."""
-    lib = _lib.load()
-    q, c, neg_c = _loss_operands("inbatch_loss_backward", q, c, neg_c)
-    dev = q.device
-    B, d = q.shape
-    ncol = B + (neg_c is not None)
-    if (tuple(product.shape) != (B, ncol) or product.dtype != torch.float32 or product.device != dev
-            or (ncol > 1 and product.stride(1) != 1) or stats.shape != (2, B)
-            or stats.dtype != torch.float32 or stats.device != dev or not stats.is_contiguous()):
-        raise ValueError("inbatch_loss_backward: product and stats must be what inbatch_loss_forward returned")
-    if dloss.numel() != 1 or dloss.dtype != torch.float32 or dloss.device != dev:
-        raise ValueError("inbatch_loss_backward: dloss must be one float32 element on %s" % dev)
-    ld = product.stride(0) if B > 1 else ncol
-    dq, dc = torch.empty_like(q), torch.empty_like(c)
-    dneg = None if neg_c is None else torch.empty_like(neg_c)
-    nbytes = lib.otter_inbatch_loss_backward_workspace(B, d)
-    if nbytes < 0:
-        _lib.check(int(nbytes), "otter_inbatch_loss_backward_workspace")
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
-    _lib.check(lib.otter_inbatch_loss_backward(
-        dev.index, dloss.data_ptr(), q.data_ptr(), c.data_ptr(), None if neg_c is None else neg_c.data_ptr(), B, d,
-        product.data_ptr(), ld, stats.data_ptr(), dq.data_ptr(), dc.data_ptr(), None if dneg is None else dneg.data_ptr(),
-        None if ws is None else ws.data_ptr(), nbytes,
-        _stream(dev.index)), "otter_inbatch_loss_backward")
-    return dq, dc, dneg
+    return _lib.calls().inbatch_loss_backward(dloss, q, c, neg_c, product, stats)
 
 
 class _InbatchLoss(torch.autograd.Function):

@@ -722,3 +722,67 @@ def test_another_stream_and_two_at_once():
     torch.cuda.synchronize()
     _same(res[0], exp)
     _same(res[1], _step(T, IB, W, x, mask, dy, seeds[1]))
+
+
+def test_two_threads_at_once():
+    """The calls let other threads run while they allocate and launch."""
+    import threading
+    from otter_amd import inbatch as IB, training as T
+    W, x, mask, dy = _layer(BF16)
+    seeds = [_seed(5), _seed(6)]
+    exp = [_step(T, IB, W, x, mask, dy, s) for s in seeds]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = _step(T, IB, W, x, mask, dy, seeds[i])
+                    torch.cuda.current_stream().synchronize()
+                    _same(got, exp[i])
+        except BaseException as e:                              # noqa: B902 -- reported below
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
+
+
+def test_calls_refuse_what_is_no_tensor():
+    from otter_amd import inbatch as IB, training as T
+    dev = _dev()
+    q = torch.zeros(2, 8, 2, 64, device=dev)
+    x, w = torch.zeros(4, 8, device=dev), torch.ones(8, device=dev)
+    cu = torch.tensor([0, 8, 16], dtype=torch.int32, device=dev)
+    for bad in (None, 3.0, "q", [1, 2]):
+        for call in (lambda: T.attention_forward(bad, q, q), lambda: T.attention_forward(q, q, bad),
+                     lambda: T.layer_norm_forward(bad, w, w), lambda: T.layer_norm_forward(x, bad, w),
+                     lambda: T.layer_norm_forward(x, w, bad), lambda: T.dropout_forward(bad, 0.1, _seed()),
+                     lambda: T.dropout_forward(x, 0.1, bad), lambda: IB.inbatch_loss_forward(bad, x),
+                     lambda: IB.inbatch_loss_forward(x, bad), lambda: T.attention_backward(bad, q, q, q, q, q)):
+            with pytest.raises(ValueError):
+                call()
+    with pytest.raises(TypeError):
+        T.dropout_forward(x, "0.1", _seed())
+    with pytest.raises(ValueError, match="probability"):
+        T.dropout_forward(x, float("nan"), _seed())
+    with pytest.raises(TypeError):
+        T.dropout_forward(x, 0.1, _seed(), call="a")
+    for call in (2 ** 32, 2 ** 70, -1):
+        with pytest.raises(ValueError, match="call"):
+            T.dropout_forward(x, 0.1, _seed(), call=call)
+    with pytest.raises(ValueError, match="max_seqlen"):
+        T.attention_forward(q[0].repeat(2, 1, 1), *(q[0].repeat(2, 1, 1),) * 2, cu_seqlens=cu, max_seqlen=2 ** 40)
+    out, lse = T.attention_forward(q, q, q)
+    for grads in ((q, q), (q, q, None), q[..., 1:], 5):
+        with pytest.raises((ValueError, TypeError), match="grads"):
+            T.attention_backward(out, q, q, q, out, lse, grads=grads)
+    with pytest.raises(ValueError, match="out must be"):
+        T.dropout_forward(x, 0.1, _seed(), out=x.t())
+    y, mean, rstd = T.layer_norm_forward(x, w, w)
+    with pytest.raises(ValueError, match="mean"):
+        T.layer_norm_backward(x, x, w, mean[:2], rstd)

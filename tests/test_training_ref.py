@@ -219,3 +219,15 @@ def test_python_entry_points_refuse_cpu_tensors():
                  lambda: inbatch.inbatch_loss(x, x)):
         with pytest.raises(ValueError, match="no CPU fallback"):
             call()
+
+
+def test_call_module_is_bound_to_the_library():
+    """otter_amd._calls: wrong argument counts and errors of the library's own checks come out as Python exceptions."""
+    m = _lib.calls()
+    assert m is _lib.calls()
+    with pytest.raises(TypeError, match="arguments"):
+        m.dropout_forward(1)
+    with pytest.raises(RuntimeError, match="no_such_library"):
+        m.load("/no_such_library.so", _lib.check, None)
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        m.dropout_forward(torch.zeros(2, 8), 0.1, None, 0, None)
