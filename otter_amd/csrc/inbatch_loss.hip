@@ -7,8 +7,8 @@
 // Where the target has nearly all of a row's weight, lse - S_ii and exp(S_ii - lse) - 1 are differences of nearly equal numbers
 // and a float32 gradient would be mostly rounding.  So the rows' pass keeps the OTHER columns' sum apart: with
 // u = sum_(j != i) exp(S_ij - S_ii), the row's loss is log1p(u) and G_ii = -u / (1 + u) dloss / B, good to float32's last bits.
-// Small batches: the three products run on v_mfma_f32_32x32x2_f32 (an fma chain: no operand is rounded), G is made from S and
-// lse where a product's tile is loaded.  Large ones: every operand is split into two float16 planes, x = (hi + lo) 2^-e with
+// Little work: the three products run on v_mfma_f32_32x32x2_f32 (an fma chain: no operand is rounded), G is made from S and
+// lse where a product's tile is loaded.  Much work: every operand is split into two float16 planes, x = (hi + lo) 2^-e with
 // hi + lo good to 22 bits, and hi hi' + hi lo' + lo hi' run on v_mfma_f32_32x32x16_f16, sixteen times float32's rate for
 // three times its products.  What that leaves out is at most 3 2^-22 of each |term|, less than the float32 sums' own rounding
 // over a row of 64 and more.  S is kept (4 B^2 bytes) instead of multiplied out again in the backward pass (2 B^2 d flops).
@@ -19,6 +19,7 @@ namespace {
 using namespace otter;
 
 constexpr int LOSS_MAX_B = 65536;
+constexpr int MEAN_B = 64;         // up to here the rows' launch takes the mean as well
 constexpr int KB = 32;             // contraction depth of a staged tile
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // 16-byte load at any 4-byte address
 
@@ -32,6 +33,8 @@ struct LossArgs {
     const float* dloss;            // [1]
     float *dq, *dc, *dneg;
     int B, d, ld, splits, kchunk;
+    float* gpart;                  // [gsplits][2][B][d] of dq and dc when gsplits > 1
+    int gsplits, gchunk;           // gchunk: the contraction depth of a piece
 };
 
 // n values of a row of a matrix with `rows` rows, zeros outside: v[e] = m[row][col + e]
@@ -210,9 +213,9 @@ __device__ __forceinline__ void online(float& m, float& l, float m2, float l2) {
 }
 
 // one workgroup a row: the pieces of S summed in order (PIECES), the hard negative's score, lse and the row's loss; of a
-// small batch the last workgroup takes the mean as well (B = 64: 19.6 -> 16.5 us without the launch for it; the fence in front of
-// the count is dear where much was just written, B = 4096: 160 -> 240)
-template <bool PIECES>
+// small batch the last workgroup takes the mean as well (MEAN; B = 64: 19.6 -> 16.5 us without the launch for it; the fence in
+// front of the count is dear where there are many rows, B = 200: 13.7 -> 14.5, B = 4096: 160 -> 240)
+template <bool PIECES, bool MEAN>
 __global__ __launch_bounds__(256) void loss_rows_kernel(LossArgs a) {
     __shared__ float sm[4], sl[4], sd[4];
     __shared__ double sum[4];
@@ -283,12 +286,12 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossArgs a) {
         a.lse[i] = lse;
         a.rest[i] = rest;
         a.rowloss[i] = loss;
-        if (PIECES) {
+        if (MEAN) {
             __threadfence();                               // the row's loss before the count of it
             last = atomicAdd(a.done, 1u) == (unsigned)a.B - 1u;
         }
     }
-    if (!PIECES) return;
+    if (!MEAN) return;
     __syncthreads();
     if (!last) return;
     // the workgroup that finished last takes the mean, in one fixed order whichever it is
@@ -316,7 +319,59 @@ __global__ __launch_bounds__(1024) void loss_mean_kernel(LossArgs a) {
     }
 }
 
-// dq and dc, half the grid each
+// Element (row, n) of dq (SECOND: of dc): a piece of its sum to its place, or, where there is one piece, the gradient
+// itself with the hard negative's share.
+__device__ __forceinline__ void put_grad(const LossArgs& a, bool second, int piece, float g, int row, int n, float v) {
+    if (row >= a.B || n >= a.d) return;
+    const long long at = (long long)row * a.d + n;
+    if (a.gsplits > 1) {
+        a.gpart[((long long)piece * 2 + second) * a.B * a.d + at] = v;
+        return;
+    }
+    if (second) {
+        a.dc[at] = v;
+        return;
+    }
+    if (a.neg) {
+        const float gn = __expf(a.scores[(long long)row * a.ld + a.B] - a.lse[row]) * g;
+        v = fmaf(gn, a.neg[at], v);
+        a.dneg[at] = gn * a.q[at];
+    }
+    a.dq[at] = v;
+}
+
+// dq (blockIdx.y = 0) and dc from their pieces, summed in order
+__global__ __launch_bounds__(256) void loss_join_kernel(LossArgs a) {
+    const bool second = blockIdx.y;
+    const long long n = (long long)a.B * a.d, at = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at >= n) return;
+    const float* p = a.gpart + (second ? n : 0) + at;
+    const int m = (int)min(4ll, n - at);
+    f4u v = {0.f, 0.f, 0.f, 0.f};
+    if (m == 4) {
+#pragma unroll 4
+        for (int k = 0; k < a.gsplits; ++k) v += *reinterpret_cast<const f4u*>(p + 2 * n * k);
+    } else {
+        for (int k = 0; k < a.gsplits; ++k)
+            for (int e = 0; e < m; ++e) v[e] += p[2 * n * k + e];
+    }
+    const float g = *a.dloss / (float)a.B;
+    float* out = second ? a.dc : a.dq;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (e >= m) break;
+        float x = v[e];
+        if (!second && a.neg) {
+            const long long row = (at + e) / a.d;
+            const float gn = __expf(a.scores[row * a.ld + a.B] - a.lse[row]) * g;
+            x = fmaf(gn, a.neg[at + e], x);
+            a.dneg[at + e] = gn * a.q[at + e];
+        }
+        out[at + e] = x;
+    }
+}
+
+// dq and dc, half the grid each; blockIdx.y: a piece of the contraction
 template <int BM>
 __global__ __launch_bounds__(256) void loss_grad_kernel(LossArgs a) {
     __shared__ __attribute__((aligned(16))) float lds[2 * BM * KB];
@@ -325,28 +380,16 @@ __global__ __launch_bounds__(256) void loss_grad_kernel(LossArgs a) {
     const bool second = id >= half;
     const int t = second ? id - half : id;
     const int m0 = (t / nt) * BM, n0 = (t % nt) * BM;
+    const int ka = blockIdx.y * a.gchunk, kb = min(a.B, ka + a.gchunk);
     const float g = *a.dloss / (float)a.B;
     const Grad G{a.scores, a.lse, a.rest, a.ld, a.B, g};
     f32x16 acc[BM / 64][BM / 64];
     clear<BM>(acc);
-    if (second) {
-        product<BM, false, false>(acc, G, Plain{a.q, a.B, a.d, a.d}, m0, n0, 0, a.B, lds);
-        each<BM>(acc, m0, n0, [&](int j, int n, float v) {
-            if (j < a.B && n < a.d) a.dc[(long long)j * a.d + n] = v;
-        });
-    } else {
-        product<BM, true, false>(acc, G, Plain{a.c, a.B, a.d, a.d}, m0, n0, 0, a.B, lds);
-        each<BM>(acc, m0, n0, [&](int i, int n, float v) {
-            if (i >= a.B || n >= a.d) return;
-            const long long at = (long long)i * a.d + n;
-            if (a.neg) {
-                const float gn = __expf(a.scores[(long long)i * a.ld + a.B] - a.lse[i]) * g;
-                v = fmaf(gn, a.neg[at], v);
-                a.dneg[at] = gn * a.q[at];
-            }
-            a.dq[at] = v;
-        });
-    }
+    if (second)
+        product<BM, false, false>(acc, G, Plain{a.q, a.B, a.d, a.d}, m0, n0, ka, kb, lds);
+    else
+        product<BM, true, false>(acc, G, Plain{a.c, a.B, a.d, a.d}, m0, n0, ka, kb, lds);
+    each<BM>(acc, m0, n0, [&](int i, int n, float v) { put_grad(a, second, blockIdx.y, g, i, n, v); });
 }
 
 // ------------------------------------------------------------------ two float16 planes
@@ -497,12 +540,12 @@ struct Planes {
     }
 };
 
-// acc += A B^T over k in [0, K): 4 waves as 2 x 2, a wave 64 x (BN / 2); lds: both operands' planes, one stage (two stages
+// acc += A B^T over k in [ka, kb), multiples of SB: 4 waves as 2 x 2, a wave 64 x (BN / 2); lds: both operands' planes, one stage (two stages
 // would halve the workgroups of a CU, which are what hides the loads)
 template <int BN, bool AKC, bool BKC>
 __device__ __forceinline__ void product16(f32x16 (&acc)[2][BN / 64], const unsigned short* Ahi, const unsigned short* Alo,
                                           long long lda, const unsigned short* Bhi, const unsigned short* Blo, long long ldb, int m0,
-                                          int n0, int K, char* lds) {
+                                          int n0, int ka, int kb, char* lds) {
     constexpr int NB = BN / 64;
     constexpr bool BOTH = AKC && BKC;
     typedef Planes<128, AKC> PA;
@@ -513,14 +556,14 @@ __device__ __forceinline__ void product16(f32x16 (&acc)[2][BN / 64], const unsig
     char* sB = lds + 2 * PA::BYTES;
     PA ra;
     PB rb;
-    ra.load(Ahi, Alo, lda, m0, 0);
-    rb.load(Bhi, Blo, ldb, n0, 0);
-    for (int k0 = 0; k0 < K; k0 += SB) {
+    ra.load(Ahi, Alo, lda, m0, ka);
+    rb.load(Bhi, Blo, ldb, n0, ka);
+    for (int k0 = ka; k0 < kb; k0 += SB) {
         __syncthreads();
         ra.store(sA);
         rb.store(sB);
         __syncthreads();
-        if (k0 + SB < K) {
+        if (k0 + SB < kb) {
             ra.load(Ahi, Alo, lda, m0, k0 + SB);
             rb.load(Bhi, Blo, ldb, n0, k0 + SB);
         }
@@ -580,15 +623,18 @@ __global__ __launch_bounds__(256, 2) void loss_scores16_kernel(LossArgs a, Split
     __shared__ __attribute__((aligned(16))) char lds[4 * Planes<128, true>::BYTES];
     const int nt = s.Bp / 128, t = xcd_remap(blockIdx.x, gridDim.x);
     const int m0 = (t / nt) * 128, n0 = (t % nt) * 128;
+    const int ka = blockIdx.y * a.kchunk;
+    float* out = a.splits > 1 ? a.part + (size_t)blockIdx.y * a.B * a.B : a.scores;
+    const long long ld = a.splits > 1 ? a.B : a.ld;
     f32x16 acc[2][2];
     clear16<2>(acc);
-    product16<128, true, true>(acc, s.plane[0], s.plane[1], s.dp, s.plane[2], s.plane[3], s.dp, m0, n0, s.dp, lds);
+    product16<128, true, true>(acc, s.plane[0], s.plane[1], s.dp, s.plane[2], s.plane[3], s.dp, m0, n0, ka, min(s.dp, ka + a.kchunk), lds);
     each16<128>(acc, m0, n0, [&](int i, int j, float v) {
-        if (i < a.B && j < a.B) a.scores[(long long)i * a.ld + j] = v * s.qs[i] * s.cs[j];
+        if (i < a.B && j < a.B) out[(long long)i * ld + j] = v * s.qs[i] * s.cs[j];
     });
 }
 
-// dq and dc, half the grid each
+// dq and dc, half the grid each; blockIdx.y: a piece of the contraction
 __global__ __launch_bounds__(256, 2) void loss_grad16_kernel(LossArgs a, SplitArgs s, const unsigned short* ghi, const unsigned short* glo) {
     constexpr int LDS1 = 2 * Planes<128, true>::BYTES, LDS2 = 2 * Planes<128, false>::BYTES;
     __shared__ __attribute__((aligned(16))) char lds[(LDS1 > LDS2 ? LDS1 : LDS2) + 2 * Planes<64, false>::BYTES];
@@ -597,28 +643,14 @@ __global__ __launch_bounds__(256, 2) void loss_grad16_kernel(LossArgs a, SplitAr
     const int t = second ? id - half : id, m0 = (t / nt) * 128, n0 = (t % nt) * 64;
     const float g = *a.dloss / (float)a.B;
     const float back = 1.0f / plane_scale(matrix_top(s.top, second ? 0 : 1)), gback = g / plane_scale(matrix_top(s.top, 2));
+    const int ka = blockIdx.y * a.gchunk, kb = min(s.Bp, ka + a.gchunk);
     f32x16 acc[2][1];
     clear16<1>(acc);
-    if (second) {
-        product16<64, false, false>(acc, ghi, glo, s.Bp, s.plane[0], s.plane[1], s.dp, m0, n0, s.Bp, lds);
-        each16<64>(acc, m0, n0, [&](int j, int n, float v) {
-            if (j < a.B && n < a.d) a.dc[(long long)j * a.d + n] = v * back * gback;
-        });
-    } else {
-        product16<64, true, false>(acc, ghi, glo, s.Bp, s.plane[2], s.plane[3], s.dp, m0, n0, s.Bp, lds);
-        each16<64>(acc, m0, n0, [&](int i, int n, float v) {
-            if (i >= a.B || n >= a.d) return;
-            const long long at = (long long)i * a.d + n;
-            v *= back;
-            v *= gback;
-            if (a.neg) {
-                const float gn = __expf(a.scores[(long long)i * a.ld + a.B] - a.lse[i]) * g;
-                v = fmaf(gn, a.neg[at], v);
-                a.dneg[at] = gn * a.q[at];
-            }
-            a.dq[at] = v;
-        });
-    }
+    if (second)
+        product16<64, false, false>(acc, ghi, glo, s.Bp, s.plane[0], s.plane[1], s.dp, m0, n0, ka, kb, lds);
+    else
+        product16<64, true, false>(acc, ghi, glo, s.Bp, s.plane[2], s.plane[3], s.dp, m0, n0, ka, kb, lds);
+    each16<64>(acc, m0, n0, [&](int i, int n, float v) { put_grad(a, second, blockIdx.y, g, i, n, v * back * gback); });
 }
 
 // ------------------------------------------------------------------ host side
@@ -629,15 +661,40 @@ int check_loss(const char* what, int B, int d, int ld, int ncol) {
     return OTTER_OK;
 }
 
-// pieces of d so that a small batch still has work for the chip: at least 64 of d each
-int loss_splits(int B, int d) {
-    const long long tiles = (long long)((B + 63) / 64) * ((B + 63) / 64);
-    const int s = (int)(tiles < 256 ? 256 / tiles : 1), most = (d + 63) / 64;
-    return s < most ? s : most;
+// Pieces of a contraction of depth k so that `tiles` workgroups become about `want`, each at least `least` deep
+int pieces(long long tiles, int k, int want, int least) {
+    const int s = (int)(tiles < want ? want / tiles : 1), most = k / least;
+    return max(1, min(s, most));
 }
 
-// Two float16 planes or float32: the planes cost two passes over the operands, and over G in the backward pass.
-bool loss_planes(int B, int d) { return B > 512 && d >= 64; }
+// Two float16 planes or float32, by B^2 d with d in whole tiles.  The planes cost passes over the operands, and over G in the
+// backward pass.  float32 -> planes, us: forward B = 600 d = 768 30 -> 40, 400 x 2304 44 -> 47, 500 x 2304 50 -> 47, 800 x 768
+// 51 -> 43, 1500 x 256 33 -> 35, 2000 x 256 42 -> 40; backward 800 x 256 27 -> 33, 1000 x 256 33 -> 34, 600 x 768 36 -> 36,
+// 1500 x 256 75 -> 43, 500 x 2304 64 -> 49.  Of short sums what the planes leave out would show beside float32's own rounding:
+// scores of less than 64 elements stay float32 (and take the same time: 38 and 36 us of B = 4096).
+double loss_work(int B, int d) { return (double)B * B * round_up(d, 64); }
+bool score_planes(int B, int d) { return B > 256 && d >= 64 && loss_work(B, d) > 4e8; }
+bool grad_planes(int B, int d) { return B > 256 && loss_work(B, d) > 2.7e8; }
+
+// Pieces of the scores' contraction (d) and of the gradients' (B) where there are few tiles, each piece `chunk` deep.  Fewer or
+// shallower pieces and more or deeper ones measured 0 to 20 % slower; without pieces: scores of B = 600 d = 768 54 -> 40 us
+// forward, gradients of 512 x 40 36 -> 11, 2000 x 63 182 -> 38, 4096 x 64 138 -> 78, 2000 x 768 106 -> 93.  Gradients of up to
+// 128 rows are one piece: a launch to join pieces costs what they save.
+int score_splits(int B, int d, int* chunk) {
+    const bool planes = score_planes(B, d);
+    const long long n = planes ? (B + 127) / 128 : (B + 63) / 64;
+    const int k = round_up(d, 64), s = pieces(n * n, k, 256, planes ? 128 : 64);
+    *chunk = round_up((k + s - 1) / s, KB);
+    return (k + *chunk - 1) / *chunk;
+}
+int grad_splits(int B, int d, int* chunk) {
+    const bool planes = grad_planes(B, d);
+    const long long tiles = 2ll * (planes ? (B + 127) / 128 : (B + 63) / 64) * ((d + 63) / 64);
+    const int k = planes ? round_up(B, 128) : B;
+    const int s = planes ? pieces(tiles, k, 1024, 128) : B > 128 ? pieces(tiles, k, 512, 32) : 1;
+    *chunk = round_up((k + s - 1) / s, KB);
+    return (k + *chunk - 1) / *chunk;
+}
 
 int64_t align16(int64_t x) { return (x + 15) / 16 * 16; }
 
@@ -672,19 +729,19 @@ int64_t lay_forward(void* ws, LossArgs& a, SplitArgs& s) {
     Take t{(char*)ws};
     a.rowloss = t.template operator()<float>(a.B);
     a.done = t.template operator()<unsigned>(1);
-    if (loss_planes(a.B, a.d)) {
+    if (score_planes(a.B, a.d)) {
         s.qs = t.template operator()<float>(s.Bp);
         s.cs = t.template operator()<float>(s.Bp);
         take_planes(t, s);
-    } else if (a.splits > 1) {
-        a.part = t.template operator()<float>((int64_t)a.splits * a.B * a.B);
     }
+    if (a.splits > 1) a.part = t.template operator()<float>((int64_t)a.splits * a.B * a.B);
     return t.used;
 }
 
-int64_t lay_backward(void* ws, SplitArgs& s, unsigned short** g) {
+int64_t lay_backward(void* ws, LossArgs& a, SplitArgs& s, unsigned short** g) {
     Take t{(char*)ws};
-    if (!loss_planes(s.B, s.d)) return 0;
+    if (a.gsplits > 1) a.gpart = t.template operator()<float>((int64_t)a.gsplits * 2 * s.B * s.d);
+    if (!grad_planes(s.B, s.d)) return t.used;
     s.top = t.template operator()<float>(3 * NMAX);
     take_planes(t, s);
     g[0] = t.template operator()<unsigned short>((int64_t)s.Bp * s.Bp);
@@ -708,7 +765,7 @@ int64_t otter_inbatch_loss_workspace(int B, int d) {
     LossArgs a = {};
     a.B = B;
     a.d = d;
-    a.splits = loss_splits(B, d);
+    a.splits = score_splits(B, d, &a.kchunk);
     SplitArgs s = split_args(nullptr, nullptr, B, d);
     return lay_forward(nullptr, a, s);
 }
@@ -732,23 +789,27 @@ int otter_inbatch_loss_forward(int device, const float* q, const float* c, const
     a.B = B;
     a.d = d;
     a.ld = ld;
-    a.splits = loss_splits(B, d);
-    a.kchunk = round_up((d + a.splits - 1) / a.splits, KB);
+    a.splits = score_splits(B, d, &a.kchunk);
     SplitArgs s = split_args(q, c, B, d);
     lay_forward(workspace, a, s);
     hipStream_t st = (hipStream_t)stream;
-    if (loss_planes(B, d)) {
-        a.splits = 1;
+    if (score_planes(B, d)) {
         loss_split_kernel<false><<<dim3((unsigned)(s.Bp / 4), 2), 256, 0, st>>>(s);
-        loss_scores16_kernel<<<(unsigned)((s.Bp / 128) * (s.Bp / 128)), 256, 0, st>>>(a, s);
+        loss_scores16_kernel<<<dim3((unsigned)((s.Bp / 128) * (s.Bp / 128)), (unsigned)a.splits), 256, 0, st>>>(a, s);
     } else {
         const unsigned nt = (unsigned)(B + 63) / 64;
         loss_scores_kernel<64><<<dim3(nt * nt, (unsigned)a.splits), 256, 0, st>>>(a);
     }
-    if (a.splits > 1) {
-        loss_rows_kernel<true><<<B, 256, 0, st>>>(a);
+    if (B <= MEAN_B) {
+        if (a.splits > 1)
+            loss_rows_kernel<true, true><<<B, 256, 0, st>>>(a);
+        else
+            loss_rows_kernel<false, true><<<B, 256, 0, st>>>(a);
     } else {
-        loss_rows_kernel<false><<<B, 256, 0, st>>>(a);
+        if (a.splits > 1)
+            loss_rows_kernel<true, false><<<B, 256, 0, st>>>(a);
+        else
+            loss_rows_kernel<false, false><<<B, 256, 0, st>>>(a);
         loss_mean_kernel<<<1, 1024, 0, st>>>(a);
     }
     OTTER_HIP_TRY(hipGetLastError());
@@ -758,9 +819,11 @@ int otter_inbatch_loss_forward(int device, const float* q, const float* c, const
 int64_t otter_inbatch_loss_backward_workspace(int B, int d) {
     const int rc = check_loss("inbatch_loss_backward_workspace", B, d, 0, 0);
     if (rc) return rc;
+    LossArgs a = {};
+    a.gsplits = grad_splits(B, d, &a.gchunk);
     SplitArgs s = split_args(nullptr, nullptr, B, d);
     unsigned short* g[2];
-    return lay_backward(nullptr, s, g);
+    return lay_backward(nullptr, a, s, g);
 }
 
 int otter_inbatch_loss_backward(int device, const float* dloss, const float* q, const float* c, const float* neg_c, int B, int d,
@@ -789,19 +852,21 @@ int otter_inbatch_loss_backward(int device, const float* dloss, const float* q, 
     a.B = B;
     a.d = d;
     a.ld = ld;
+    a.gsplits = grad_splits(B, d, &a.gchunk);
+    SplitArgs s = split_args(q, c, B, d);
+    unsigned short* gp[2];
+    lay_backward(workspace, a, s, gp);
     hipStream_t st = (hipStream_t)stream;
-    if (loss_planes(B, d)) {
-        SplitArgs s = split_args(q, c, B, d);
-        unsigned short* gp[2];
-        lay_backward(workspace, s, gp);
+    if (grad_planes(B, d)) {
         s.rest = a.rest;
         loss_top_kernel<<<dim3(NMAX, 3), 256, 0, st>>>(s);
         loss_split_kernel<true><<<dim3((unsigned)(s.Bp / 4), 2), 256, 0, st>>>(s);
         loss_gplanes_kernel<<<(unsigned)s.Bp * ((unsigned)(s.Bp + 1023) / 1024), 256, 0, st>>>(a, s.top, gp[0], gp[1], s.Bp);
-        loss_grad16_kernel<<<(unsigned)(2 * (s.Bp / 128) * ((d + 63) / 64)), 256, 0, st>>>(a, s, gp[0], gp[1]);
+        loss_grad16_kernel<<<dim3((unsigned)(2 * (s.Bp / 128) * ((d + 63) / 64)), (unsigned)a.gsplits), 256, 0, st>>>(a, s, gp[0], gp[1]);
     } else {
-        loss_grad_kernel<64><<<(unsigned)(2 * tiles), 256, 0, st>>>(a);
+        loss_grad_kernel<64><<<dim3((unsigned)(2 * tiles), (unsigned)a.gsplits), 256, 0, st>>>(a);
     }
+    if (a.gsplits > 1) loss_join_kernel<<<dim3((unsigned)(((int64_t)B * d + 1023) / 1024), 2), 256, 0, st>>>(a);
     OTTER_HIP_TRY(hipGetLastError());
     return OTTER_OK;
 }

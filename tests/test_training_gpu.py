@@ -786,3 +786,35 @@ def test_calls_refuse_what_is_no_tensor():
     y, mean, rstd = T.layer_norm_forward(x, w, w)
     with pytest.raises(ValueError, match="mean"):
         T.layer_norm_backward(x, x, w, mean[:2], rstd)
+
+
+@pytest.mark.parametrize("B,d,neg", [(513, 2304, True), (260, 6400, False), (900, 768, True), (1500, 200, True), (1100, 330, False),
+                                     (2100, 60, True), (2050, 65, False), (300, 40, True), (200, 768, True), (129, 1, True)])
+def test_inbatch_loss_in_pieces_and_planes(B, d, neg):
+    """Both sides of the choices by work and by tiles: float16 planes or float32, sums in one piece or several."""
+    test_inbatch_loss(B, d, neg)
+
+
+@pytest.mark.parametrize("margin", [3.0, 20.0])
+def test_inbatch_loss_of_confident_rows_in_planes(margin):
+    test_inbatch_loss_of_confident_rows(2000, margin)
+
+
+@pytest.mark.parametrize("scale", [1e-6, 1e6])
+def test_inbatch_loss_of_small_and_large_embeddings_in_planes(scale):
+    test_inbatch_loss_of_small_and_large_embeddings(2000, scale)
+
+
+@pytest.mark.parametrize("B,d", [(300, 64), (700, 100), (1600, 256)])
+def test_inbatch_loss_repeats_its_bits(B, d):
+    from otter_amd import inbatch as IB
+    q, c, n = (_rand(95 + i, B, d, scale=d ** -0.25)[1] for i in range(3))
+    one = torch.ones((), device=_dev())
+
+    def run():
+        loss, product, stats = IB.inbatch_loss_forward(q, c, n)
+        return (loss, product, stats, *IB.inbatch_loss_backward(one, q, c, n, product, stats))
+
+    first = run()
+    for _ in range(3):
+        _same(run(), first)
