@@ -25,7 +25,7 @@ using namespace otter;
 constexpr int DH = 64;         // head dimension
 constexpr int TR = 64;         // rows of a streamed tile
 constexpr int CUS = 256;       // compute units of the chip
-constexpr int OWN = 128;       // rows a workgroup owns: 4 waves x 32
+constexpr int OWN = 128;       // rows a workgroup owns: 4 waves x 32; 64 where two waves share 32 rows (HALF)
 
 struct View {                  // element strides of a [batch, token, head, 64] tensor (batch stride unused when packed)
     void* p;
@@ -103,6 +103,24 @@ struct Tile {
     static constexpr int NF = CH / 2;                     // fragment chunks a lane: 2 j + lane half
     static constexpr int EPC = 16 / (int)sizeof(T);
     static constexpr int BYTES = TR * PITCH;
+};
+
+// HALF: waves w and w + 2 own the same 32 rows; each takes its half of every streamed tile, and what they gathered is added up
+// through LDS at the end.  x: n registers of waves 2 and 3 to those of waves 0 and 1, one slot of 64 lanes x N floats a wave.
+template <int N>
+struct Handover {
+    float* p;
+    __device__ __forceinline__ Handover(char* lds) : p(reinterpret_cast<float*>(lds) + (threadIdx.x >> 6 & 1) * N * 64 + (threadIdx.x & 63)) {}
+    __device__ __forceinline__ void put(int i, float x) const { p[i * 64] = x; }
+    __device__ __forceinline__ void put(int i, const f32x16 (&o)[2]) const {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) put(i + e, o[e >> 4][e & 15]);
+    }
+    __device__ __forceinline__ float get(int i) const { return p[i * 64]; }
+    __device__ __forceinline__ void add(int i, f32x16 (&o)[2]) const {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e >> 4][e & 15] += get(i + e);
+    }
 };
 
 struct Lane {
@@ -385,13 +403,14 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 // The running maximum is let stand while no score passes it by more than 2^8 (in base 2 exponents: the sums and the
 // probabilities then stay below 2^8 times their final size, harmless in float32 and for bfloat16's relative rounding), so
 // that the accumulators are rescaled once or twice a row and not at every tile.
-template <typename T, bool DROP>
+template <typename T, bool DROP, bool HALF>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnTrainArgs a) {
     using X = Tile<T>;
+    constexpr int ROWS = HALF ? OWN / 2 : OWN, NS = HALF ? 1 : 2;   // rows of the workgroup; halves of a tile a wave takes
     __shared__ __attribute__((aligned(16))) char sK[2][X::BYTES];
     __shared__ __attribute__((aligned(16))) char sV[2][X::BYTES];
     const Lane ln;
-    const int h = ln.h, l31 = ln.l31, wave = ln.wave;
+    const int h = ln.h, l31 = ln.l31, wave = HALF ? ln.wave & 1 : ln.wave, sub0 = HALF ? ln.wave >> 1 : 0;
     const int items = a.nblk * a.heads * a.B;
     if ((int)blockIdx.x >= items) return zero_outside<T>(a, blockIdx.x - items, a.o, a.lse);
     const Seq s = find_seq(a, blockIdx.x);
@@ -402,7 +421,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnTrainArgs a) {
     const u32 bh = (u32)(s.b * a.heads + s.h);
     const Key2 key(a.drop);
     const float c2 = fmaxf(fabsf(a.c2), 1e-30f);   // not 0: a left-out key's -inf has to stay one
-    for (int q0 = s.blk * OWN; q0 < s.len; q0 += a.nblk * OWN) {
+    for (int q0 = s.blk * ROWS; q0 < s.len; q0 += a.nblk * ROWS) {
         const int i = q0 + wave * 32 + l31;
         float4 qf[X::NF];
         load_own<T>(qf, Q, a.q.st, min(i, s.len - 1), h);
@@ -429,20 +448,20 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnTrainArgs a) {
                 kb.fetch(j0 + 2 * TR);
             }
             if (bits == 0) continue;
-            f32x16 sc[2];
+            f32x16 sc[NS];
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub) sc[sub] = row_product<T>(sK[buf] + sub * 32 * X::PITCH + ln.frag<T>(), qf);
+            for (int sub = 0; sub < NS; ++sub) sc[sub] = row_product<T>(sK[buf] + (sub0 + sub) * 32 * X::PITCH + ln.frag<T>(), qf);
             if (~bits != 0) {
 #pragma unroll
-                for (int sub = 0; sub < 2; ++sub) {
-                    const u32 kb32 = (u32)(bits >> (32 * sub)) >> (4 * h);
+                for (int sub = 0; sub < NS; ++sub) {
+                    const u32 kb32 = (u32)(bits >> (32 * (sub0 + sub))) >> (4 * h);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) sc[sub][r] = (kb32 >> acc_row(r, 0)) & 1u ? sc[sub][r] : -INFINITY;
                 }
             }
-            float mx = max_(sc[0][0], sc[1][0]);
+            float mx = max_(sc[0][0], sc[NS - 1][0]);
 #pragma unroll
-            for (int r = 1; r < 16; ++r) mx = max_(max_(sc[0][r], sc[1][r]), mx);
+            for (int r = 1; r < 16; ++r) mx = max_(max_(sc[0][r], sc[NS - 1][r]), mx);
             mx = max_(mx, __shfl_xor(mx, 32)) * c2;
             // mx > m + 8 or a NaN: move the maximum
             if (__any(!(mx <= m + 8.0f))) {
@@ -458,21 +477,40 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnTrainArgs a) {
             }
             float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
+            for (int sub = 0; sub < NS; ++sub) {
                 Draws w;
-                if constexpr (DROP) w.queries(a.drop, key.k0, key.k1, bh, i, j0 + 32 * sub, h);
+                if constexpr (DROP) w.queries(a.drop, key.k0, key.k1, bh, i, j0 + 32 * (sub0 + sub), h);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const float p = exp2_(fmaf(sc[sub][r], c2, -base));
                     sum[r & 1] += p;                                 // the softmax's sum is over all keys, dropped or not
                     sc[sub][r] = DROP ? made(w.kept_q(r) ? p : 0.0f) : p;
                 }
-                col_product<T>(o, sV[buf] + sub * 32 * X::PITCH + ln.col<T>(), sc[sub]);
+                col_product<T>(o, sV[buf] + (sub0 + sub) * 32 * X::PITCH + ln.col<T>(), sc[sub]);
             }
             l += sum[0] + sum[1];
         }
+        if constexpr (HALF) {
+            static_assert(2 * 34 * 64 * sizeof(float) <= sizeof(sK));
+            const Handover<34> to(sK[0]);
+            __syncthreads();               // the last tile is read
+            if (sub0) {
+                to.put(0, o);
+                to.put(32, m);
+                to.put(33, l);
+            }
+            __syncthreads();
+            if (!sub0) {
+                const float m2 = to.get(32), mnew = max_(m, m2);
+                base = mnew == -INFINITY ? 0.0f : mnew;
+                const float alpha = exp2_(m - base), beta = exp2_(m2 - base);
+                l = l * alpha + to.get(33) * beta;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e >> 4][e & 15] = o[e >> 4][e & 15] * alpha + to.get(e) * beta;
+            }
+        }
         l += __shfl_xor(l, 32);
-        if (i < s.len) {
+        if (i < s.len && (!HALF || !sub0)) {
             store_own<T>(O + (long long)i * a.o.st, o, a.drop.scale / l, h);
             if (h == 0) a.lse[s.stat + i] = (base + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
         }
@@ -482,14 +520,15 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnTrainArgs a) {
 
 // ------------------------------------------------------------------ backward: dQ (and D)
 // The forward kernel's walk again: queries on the lanes, dS^T is the right operand of dQ^T = K^T dS^T.
-template <typename T, bool DROP>
+template <typename T, bool DROP, bool HALF>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
     using X = Tile<T>;
+    constexpr int ROWS = HALF ? OWN / 2 : OWN, NS = HALF ? 1 : 2;
     constexpr int UNROLL = DROP ? 2 : 1;      // the draws of one half fill the waits of the other (packed, dropout: 440 -> 416 us)
     __shared__ __attribute__((aligned(16))) char sK[2][X::BYTES];
     __shared__ __attribute__((aligned(16))) char sV[2][X::BYTES];
     const Lane ln;
-    const int h = ln.h, l31 = ln.l31, wave = ln.wave;
+    const int h = ln.h, l31 = ln.l31, wave = HALF ? ln.wave & 1 : ln.wave, sub0 = HALF ? ln.wave >> 1 : 0;
     const int items = a.nblk * a.heads * a.B;
     if ((int)blockIdx.x >= items) return zero_outside<T>(a, blockIdx.x - items, a.dq, nullptr);
     const Seq s = find_seq(a, blockIdx.x);
@@ -500,7 +539,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
     T* dQ = head_ptr<T>(a, a.dq, s);
     const u32 bh = (u32)(s.b * a.heads + s.h);
     const Key2 key(a.drop);
-    for (int q0 = s.blk * OWN; q0 < s.len; q0 += a.nblk * OWN) {
+    for (int q0 = s.blk * ROWS; q0 < s.len; q0 += a.nblk * ROWS) {
         const int i = q0 + wave * 32 + l31, ic = min(i, s.len - 1);
         float4 qf[X::NF], df[X::NF];
         load_own<T>(qf, O, a.o.st, ic, h);
@@ -557,7 +596,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
                     D += __shfl_xor(D, 32);
                 }
 #pragma unroll UNROLL
-                for (int sub = 0; sub < 2; ++sub) {
+                for (int sub = sub0; sub < sub0 + NS; ++sub) {
                     f32x16 sc = row_product<T>(sK[buf] + sub * 32 * X::PITCH + ln.frag<T>(), qf);
                     const f32x16 dp = row_product<T>(sV[buf] + sub * 32 * X::PITCH + ln.frag<T>(), df);
                     Draws w;
@@ -578,6 +617,15 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
             }
             __syncthreads();
         }
+        if constexpr (HALF) {
+            static_assert(2 * 32 * 64 * sizeof(float) <= sizeof(sK));
+            const Handover<32> to(sK[0]);  // free: the walk ended with a barrier
+            if (sub0) to.put(0, o);
+            __syncthreads();
+            if (!sub0) to.add(0, o);
+            __syncthreads();
+            if (sub0) continue;
+        }
         if (i < s.len && h == 0) a.delta[s.stat + i] = D;
         if (i < s.len) store_own<T>(dQ + (long long)i * a.dq.st, o, a.scale, h);
     }
@@ -585,15 +633,16 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
 
 // ------------------------------------------------------------------ backward: dK, dV
 // A workgroup owns 128 keys, a wave 32 (one on each lane of a half), and streams the queries in tiles of 64.
-template <typename T, bool DROP>
+template <typename T, bool DROP, bool HALF>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
     using X = Tile<T>;
+    constexpr int ROWS = HALF ? OWN / 2 : OWN, NS = HALF ? 1 : 2;
     constexpr int UNROLL = DROP ? 2 : 1;      // the draws of one half fill the waits of the other (packed, dropout: 440 -> 416 us)
     __shared__ __attribute__((aligned(16))) char sQ[2][X::BYTES];
     __shared__ __attribute__((aligned(16))) char sO[2][X::BYTES];
     __shared__ __attribute__((aligned(16))) float sL[2][TR], sD[2][TR];
     const Lane ln;
-    const int h = ln.h, l31 = ln.l31, wave = ln.wave;
+    const int h = ln.h, l31 = ln.l31, wave = HALF ? ln.wave & 1 : ln.wave, sub0 = HALF ? ln.wave >> 1 : 0;
     const int items = a.nblk * a.heads * a.B;
     if ((int)blockIdx.x >= items) {
         zero_outside<T>(a, blockIdx.x - items, a.dk, nullptr);
@@ -607,7 +656,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
     T *dK = head_ptr<T>(a, a.dk, s), *dV = head_ptr<T>(a, a.dv, s);
     const u32 bh = (u32)(s.b * a.heads + s.h);
     const Key2 key(a.drop);
-    for (int n0 = s.blk * OWN; n0 < s.len; n0 += a.nblk * OWN) {
+    for (int n0 = s.blk * ROWS; n0 < s.len; n0 += a.nblk * ROWS) {
         const int j = n0 + wave * 32 + l31, jc = min(j, s.len - 1);
         const bool counts = j < kend && (even || !a.mask || a.mask[(long long)s.b * a.L + jc] != 0);
         f32x16 ok[2] = {zero16(), zero16()}, ov[2] = {zero16(), zero16()};
@@ -638,7 +687,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
                 __syncthreads();
                 if (i0 + TR < s.len) fetch(i0 + TR);
 #pragma unroll UNROLL
-                for (int sub = 0; sub < 2; ++sub) {
+                for (int sub = sub0; sub < sub0 + NS; ++sub) {
                     f32x16 sc, dp;
                     row_products<T>(sc, dp, sQ[buf] + sub * 32 * X::PITCH + ln.frag<T>(), kf, sO[buf] + sub * 32 * X::PITCH + ln.frag<T>(), vf);
                     Draws w;
@@ -663,6 +712,21 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
                 }
             }
             __syncthreads();
+        }
+        if constexpr (HALF) {
+            static_assert(2 * 32 * 64 * sizeof(float) <= sizeof(sQ));
+            const Handover<32> tk(sQ[0]), tv(sO[0]);   // free: the walk ended with a barrier
+            if (sub0) {
+                tk.put(0, ok);
+                tv.put(0, ov);
+            }
+            __syncthreads();
+            if (!sub0) {
+                tk.add(0, ok);
+                tv.add(0, ov);
+            }
+            __syncthreads();
+            if (sub0) continue;
         }
         // a key's gradients are sums in its own lanes: what a key that does not count gathered is dropped here
         if (!counts || even) {
@@ -935,53 +999,70 @@ int fill(const char* what, const otter_attention_args* x, AttnTrainArgs* a, long
     a->scale = x->scale;
     a->c2 = x->scale * 1.4426950408889634f;
     a->lse = x->lse;
-    a->nblk = x->tokens > OWN ? (x->tokens + OWN - 1) / OWN : 1;
+    a->nblk = x->tokens > OWN ? (x->tokens + OWN - 1) / OWN : 1;     // own_half() may double it
     *rows = x->cu_seqlens ? x->total : (long long)x->batch * x->tokens;
     if ((long long)a->nblk * a->heads * a->B + a->heads > 0x7FFFFFFFll || (long long)a->B * a->heads > 0x7FFFFFFFll)
         return set_err(OTTER_EINVAL, "%s: batch x heads x tokens is too large for one launch", what);
     return OTTER_OK;
 }
 
-template <typename T>
-void launch_fwd(const AttnTrainArgs& a, int grid, hipStream_t st) {
-    if (a.drop.thr)
-        attn_fwd_kernel<T, true><<<grid, 256, 0, st>>>(a);
+// Two waves share their rows (HALF): twice the workgroups, each half as long, for twice the staging of tiles.  Sequences of up
+// to 64 rows leave no wave idle that way and stage no more (64 x 64 tokens, 12 heads, float32: 22.8 -> 17.7 us forward, 75 -> 59
+// backward).  Longer ones take it where there are few workgroups, us forward / backward, 12 heads, dropout:
+//   bfloat16  1 x 1024 26 / 62 -> 20 / 44, 8 x 300 16 / 39 -> 12 / 30, 1 x 4096 136 / 321 -> 115 / 300
+//   float32   1 x 1024 87 / 265 -> 51 / 149, 8 x 512 87 / 257 -> 77 / 218
+// and no longer with 432 (12 x 300: 16 / 40 -> 15 / 44) and 480 workgroups (20 x 256 forward: 15 -> 17).  Between 65 and 128 rows
+// it gains nothing (16 x 128 float32 15.8 / 50 -> 16.7 / 52).
+bool own_half(AttnTrainArgs& a) {
+    if (a.L > OWN / 2 && (a.L <= OWN || (long long)a.nblk * a.heads * a.B > CUS * 3 / 2)) return false;
+    a.nblk = a.L > OWN / 2 ? (a.L + OWN / 2 - 1) / (OWN / 2) : 1;
+    return true;
+}
+
+// a workgroup an item, and one a head for the rows of no sequence
+int grid_of(const AttnTrainArgs& a) { return a.nblk * a.heads * a.B + (a.cu ? a.heads : 0); }
+
+template <typename T, bool DROP>
+void launch_fwd(AttnTrainArgs& a, hipStream_t st) {
+    if (own_half(a))
+        attn_fwd_kernel<T, DROP, true><<<grid_of(a), 256, 0, st>>>(a);
     else
-        attn_fwd_kernel<T, false><<<grid, 256, 0, st>>>(a);
+        attn_fwd_kernel<T, DROP, false><<<grid_of(a), 256, 0, st>>>(a);
 }
 
 // One pass over the scores (bfloat16) or two, one for dQ and one for dK and dV.  One pass makes each score tile once and is one
 // launch, but it is one workgroup a (sequence, head) of which a CU holds one, and it needs FK keys to fill its waves.  Measured
 // (us, one pass and two, 12 heads, dropout):
 //   up to OWN tokens        16 x 70: 19 and 21, 16 x 128: 17.5 and 20.6; 64 x 70: 53 and 39        -> while the CUs hold all pairs
-//   up to FK                16 x 200: 26.5 and 38, 64 x 200: 70 and 92, 4 x 150, 4 heads: 18 and 22 -> always
+//   up to FK                16 x 200: 24.4 and 40, 40 x 200: 48 and 65, 8 x 200: 23.5 and 26.7; 4 x 256: 26 and 19.7, 1 x 256: 25
+//                           and 18 (two passes, two waves to a row) -> beyond a quarter of the CUs
 //   longer                  128 packed up to 512: 323 and 420, 16 x 512: 87 and 92, 40 packed: 139 and 143; but 32 x 512 (one and a
 //                           half rounds of workgroups): 163 and 145, 2 x 4001: 626 and 502 -> where the last round is not mostly empty
 // Several workgroups a pair, whose parts of dQ another launch adds up, did not help (16 x 512: 97).
 bool one_pass(const AttnTrainArgs& a, int dtype) {
     const long long pairs = (long long)a.B * a.heads;
     if (dtype != OTTER_BF16) return false;
-    if (a.L <= FK) return a.L > OWN || pairs <= CUS;
+    if (a.L <= FK) return a.L > OWN ? pairs > CUS / 4 : pairs <= CUS;
     const long long slots = (pairs + CUS - 1) / CUS * CUS;
     return slots == CUS ? 4 * pairs >= 3 * slots : 5 * pairs >= 4 * slots;
 }
 
 template <bool DROP>
-void launch_one_pass(const AttnTrainArgs& a, int grid, hipStream_t st) {
+void launch_one_pass(const AttnTrainArgs& a, hipStream_t st) {
     if (a.L <= OWN)
-        attn_bwd_kernel<DROP, true><<<grid, 512, 0, st>>>(a);
+        attn_bwd_kernel<DROP, true><<<grid_of(a), 512, 0, st>>>(a);
     else
-        attn_bwd_kernel<DROP, false><<<grid, 512, 0, st>>>(a);
+        attn_bwd_kernel<DROP, false><<<grid_of(a), 512, 0, st>>>(a);
 }
 
-template <typename T>
-void launch_bwd(const AttnTrainArgs& a, int grid, hipStream_t st) {
-    if (a.drop.thr) {
-        attn_dq_kernel<T, true><<<grid, 256, 0, st>>>(a);
-        attn_dkv_kernel<T, true><<<grid, 256, 0, st>>>(a);
+template <typename T, bool DROP>
+void launch_bwd(AttnTrainArgs& a, hipStream_t st) {
+    if (own_half(a)) {
+        attn_dq_kernel<T, DROP, true><<<grid_of(a), 256, 0, st>>>(a);
+        attn_dkv_kernel<T, DROP, true><<<grid_of(a), 256, 0, st>>>(a);
     } else {
-        attn_dq_kernel<T, false><<<grid, 256, 0, st>>>(a);
-        attn_dkv_kernel<T, false><<<grid, 256, 0, st>>>(a);
+        attn_dq_kernel<T, DROP, false><<<grid_of(a), 256, 0, st>>>(a);
+        attn_dkv_kernel<T, DROP, false><<<grid_of(a), 256, 0, st>>>(a);
     }
 }
 
@@ -1008,12 +1089,11 @@ int otter_attention_forward(int device, const otter_attention_args* x, void* str
     if (!a.lse) return set_err(OTTER_EINVAL, "attention_forward: NULL lse");
     DeviceGuard g(device);
     if (!g.ok) return set_err(OTTER_EHIP, "attention_forward: hipSetDevice(%d) failed", device);
-    const int grid = a.nblk * a.heads * a.B + (a.cu ? a.heads : 0);
     hipStream_t st = (hipStream_t)stream;
     if (size == 2)
-        launch_fwd<bf16_t>(a, grid, st);
+        a.drop.thr ? launch_fwd<bf16_t, true>(a, st) : launch_fwd<bf16_t, false>(a, st);
     else
-        launch_fwd<float>(a, grid, st);
+        a.drop.thr ? launch_fwd<float, true>(a, st) : launch_fwd<float, false>(a, st);
     OTTER_HIP_TRY(hipGetLastError());
     return OTTER_OK;
 }
@@ -1052,19 +1132,14 @@ int otter_attention_backward(int device, const otter_attention_args* x, void* st
     hipStream_t st = (hipStream_t)stream;
     if (one_pass(a, x->dtype)) {
         a.nblk = 1;
-        const int n = a.heads * a.B + (a.cu ? a.heads : 0);
-        if (a.drop.thr)
-            launch_one_pass<true>(a, n, st);
-        else
-            launch_one_pass<false>(a, n, st);
+        a.drop.thr ? launch_one_pass<true>(a, st) : launch_one_pass<false>(a, st);
         OTTER_HIP_TRY(hipGetLastError());
         return OTTER_OK;
     }
-    const int grid = a.nblk * a.heads * a.B + (a.cu ? a.heads : 0);
     if (size == 2)
-        launch_bwd<bf16_t>(a, grid, st);
+        a.drop.thr ? launch_bwd<bf16_t, true>(a, st) : launch_bwd<bf16_t, false>(a, st);
     else
-        launch_bwd<float>(a, grid, st);
+        a.drop.thr ? launch_bwd<float, true>(a, st) : launch_bwd<float, false>(a, st);
     OTTER_HIP_TRY(hipGetLastError());
     return OTTER_OK;
 }

@@ -818,3 +818,39 @@ def test_inbatch_loss_repeats_its_bits(B, d):
     first = run()
     for _ in range(3):
         _same(run(), first)
+
+
+# Many workgroups: a wave to 32 rows (where there are few, two waves share them), the backward pass in two passes
+@pytest.mark.parametrize("dtype,L,kind,p", [(F32, 129, None, 0.1), (F32, 200, "tile", 0.0), (F32, 260, "alternate", 0.1), (F32, 150, "holes", 0.1),
+                                            (BF16, 257, "holes", 0.1), (BF16, 300, "alternate", 0.0), (BF16, 320, "none", 0.1)])
+def test_attention_many_workgroups_dense(dtype, L, kind, p):
+    B, H = 5, 64
+    m = None if kind is None else _mask(kind, B, L)
+    x = [_rand(130 + i, B, L, H, 64, dtype=dtype) for i in range(4)]
+    kw = dict(dropout_p=p, seed=_seed() if p else None, call=6)
+    if m is not None:
+        kw["mask"] = m.to(_dev())
+    _check_attention(*x, kw, mask=m, p=p)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_many_workgroups_packed(dtype):
+    lens, H, p = [300, 20, 1, 256, 65], 64, 0.1
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    x = [_rand(140 + i, cu[-1] + 9, H, 64, dtype=dtype) for i in range(4)]
+    for t64, t in x:
+        t64[cu[-1]:] = 0
+        t[cu[-1]:] = float("nan")
+    cut = torch.tensor(cu, dtype=torch.int32, device=_dev())
+    _check_attention(*x, dict(cu_seqlens=cut, max_seqlen=300, dropout_p=p, seed=_seed(), call=6), cu=cu, p=p)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scale", [0.0, -0.125, 3.0])
+def test_attention_scales(dtype, scale):
+    """Also scores of hundreds, where a wave's half of the keys holds none of a row's weight."""
+    m = _mask("holes", 2, 150)
+    x = [_rand(150 + i, 2, 150, 2, 64, dtype=dtype) for i in range(4)]
+    _check_attention(*x, dict(mask=m.to(_dev()), dropout_p=0.1, seed=_seed(), call=6, scale=scale), mask=m, p=0.1, scale=scale)
