@@ -5,7 +5,7 @@
 //   D_i = sum_d dO_id O_id,  dS = P (Z (dO V^T) - D),  dQ = scale dS K,  dK = scale dS^T Q,  dV = (P Z)^T dO
 //
 // A sequence whose mask leaves nothing attends to all its L keys evenly (P = 1 / L, the encoder's rule); no gradient
-// reaches its queries and keys.  What masked keys hold reaches nothing: they enter the products as zeros.
+// reaches its queries and keys, as where one key counts (P = 1).  What masked keys hold reaches nothing: they enter the products as zeros.
 //
 // Both operands of a product come from 16-byte fragments of 64-element rows; a score tile leaves the matrix unit with one
 // of its two indices on the lane and sixteen of the other in the registers, which is the layout the next product's right
@@ -555,7 +555,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
         load_own<T>(qf, Q, a.q.st, ic, h);
         const float lse2 = a.lse[s.stat + ic] * 1.4426950408889634f;
         f32x16 o[2] = {zero16(), zero16()};
-        if (!even) {                                // even: dS = 0
+        if (!even && kend > 1) {                    // even, and with one key: dS = 0
             KeyBits kb(a, s, even);
             Stage<T> rk(K, a.k.st, s.len), rv(V, a.v.st, s.len);
             kb.fetch(0);
@@ -652,6 +652,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
     bool even;
     const int kend = key_end(a, s, even);
     const T *Q = head_ptr<T>(a, a.q, s), *K = head_ptr<T>(a, a.k, s), *V = head_ptr<T>(a, a.v, s);
+    const bool flat = even || kend == 1;       // one key: dS = 0, not what is left of P dO V^T - D
     const T* dO = head_ptr<T>(a, a.dout, s);
     T *dK = head_ptr<T>(a, a.dk, s), *dV = head_ptr<T>(a, a.dv, s);
     const u32 bh = (u32)(s.b * a.heads + s.h);
@@ -729,7 +730,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
             if (sub0) continue;
         }
         // a key's gradients are sums in its own lanes: what a key that does not count gathered is dropped here
-        if (!counts || even) {
+        if (!counts || flat) {
             ok[0] = ok[1] = zero16();
             if (!counts) ov[0] = ov[1] = zero16();
         }
@@ -781,6 +782,7 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
     const Seq s = find_seq(a, blockIdx.x, xcd_remap(blockIdx.x, items));
     bool even;
     const int kend = key_end(a, s, even);
+    const bool flat = even || kend == 1;
     const T *Q = head_ptr<T>(a, a.q, s), *K = head_ptr<T>(a, a.k, s), *V = head_ptr<T>(a, a.v, s);
     const T *O = head_ptr<T>(a, a.o, s), *dO = head_ptr<T>(a, a.dout, s);
     T *dQ = head_ptr<T>(a, a.dq, s), *dK = head_ptr<T>(a, a.dk, s), *dV = head_ptr<T>(a, a.dv, s);
@@ -899,9 +901,9 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
                             dp[r] = p * gr;
                         }
                     }
-                    if (!all || even) {                    // what a key that does not count adds to dQ
+                    if (!all || flat) {                    // what a key that does not count adds to dQ
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) dp[r] = counts && !even ? dp[r] : 0.0f;
+                        for (int r = 0; r < 16; ++r) dp[r] = counts && !flat ? dp[r] : 0.0f;
                     }
                     bf16x8 ds[2];
 #pragma unroll
@@ -954,7 +956,7 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
                 }
             }
         }
-        if (!counts || even) {
+        if (!counts || flat) {
             ok[0] = ok[1] = zero16();
             if (!counts) ov[0] = ov[1] = zero16();
         }

@@ -854,3 +854,23 @@ def test_attention_scales(dtype, scale):
     m = _mask("holes", 2, 150)
     x = [_rand(150 + i, 2, 150, 2, 64, dtype=dtype) for i in range(4)]
     _check_attention(*x, dict(mask=m.to(_dev()), dropout_p=0.1, seed=_seed(), call=6, scale=scale), mask=m, p=0.1, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,L,H,how", [(3, 1, 2, "dense"), (300, 1, 4, "dense"), (4, 40, 2, "mask"), (3, 300, 2, "mask"), (5, 200, 64, "mask"),
+                                       (70, 1, 4, "packed"), (3, 1, 1, "packed")])
+def test_one_key_leaves_no_gradient(B, L, H, how, dtype):
+    """With one key the probabilities are 1 whatever q and k are: their gradients are zero and not a rounding's rest."""
+    from otter_amd import training as T
+    dev = _dev()
+    q, k, v, do = (_rand(160 + i, B, L, H, 64, dtype=dtype)[1] * 3 for i in range(4))
+    kw = dict(dropout_p=0.1, seed=_seed(), call=6)
+    if how == "mask":
+        kw["mask"] = torch.zeros(B, L, dtype=torch.int64, device=dev)
+        kw["mask"][:, 0] = 1
+    elif how == "packed":
+        q, k, v, do = (t[:, 0] for t in (q, k, v, do))
+        kw.update(cu_seqlens=torch.arange(B + 1, dtype=torch.int32, device=dev), max_seqlen=1)
+    out, lse = T.attention_forward(q, k, v, **kw)
+    dq, dk, dv = T.attention_backward(do, q, k, v, out, lse, **kw)
+    assert (dq == 0).all() and (dk == 0).all() and (dv != 0).any()
