@@ -5,7 +5,8 @@
 //   D_i = sum_d dO_id O_id,  dS = P (Z (dO V^T) - D),  dQ = scale dS K,  dK = scale dS^T Q,  dV = (P Z)^T dO
 //
 // A sequence whose mask leaves nothing attends to all its L keys evenly (P = 1 / L, the encoder's rule); no gradient
-// reaches its queries and keys, as where one key counts (P = 1).  What masked keys hold reaches nothing: they enter the products as zeros.
+// reaches its queries and keys, as where one key counts (P = 1).  What masked keys hold reaches nothing: they enter the
+// products as zeros.
 //
 // Both operands of a product come from 16-byte fragments of 64-element rows; a score tile leaves the matrix unit with one
 // of its two indices on the lane and sixteen of the other in the registers, which is the layout the next product's right
@@ -403,6 +404,10 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 // The running maximum is let stand while no score passes it by more than 2^8 (in base 2 exponents: the sums and the
 // probabilities then stay below 2^8 times their final size, harmless in float32 and for bfloat16's relative rounding), so
 // that the accumulators are rescaled once or twice a row and not at every tile.
+// Bound by the matrix unit and the vector unit together: of their times only about a third overlaps, with exp2, the draws and
+// the conversion to bfloat16 about as long as the products.  bfloat16: 2 x 4001 tokens, 12 heads, no dropout 131 us
+// = 0.75 PFLOP/s (a large matrix product: 1.15); 128 packed of up to 512 with dropout 131 us, without 96; 16 x 512 ragged 28 us.
+// float32, 8 x 512 ragged: 64 us, 57 TFLOP/s on the 32x32x2 products (a large product: 154).
 template <typename T, bool DROP, bool HALF>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnTrainArgs a) {
     using X = Tile<T>;
@@ -519,7 +524,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnTrainArgs a) {
 }
 
 // ------------------------------------------------------------------ backward: dQ (and D)
-// The forward kernel's walk again: queries on the lanes, dS^T is the right operand of dQ^T = K^T dS^T.
+// The forward kernel's walk again: queries on the lanes, dS^T is the right operand of dQ^T = K^T dS^T.  Three products a score
+// against the four of attn_dkv_kernel; float32, 8 x 512 ragged, 12 heads: 83 us and 118 us.
 template <typename T, bool DROP, bool HALF>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
     using X = Tile<T>;
@@ -632,7 +638,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
 }
 
 // ------------------------------------------------------------------ backward: dK, dV
-// A workgroup owns 128 keys, a wave 32 (one on each lane of a half), and streams the queries in tiles of 64.
+// A workgroup owns 128 keys, a wave 32 (one on each lane of a half), and streams the queries in tiles of 64.  P and dS are right
+// operands as they stand; lse and D of a tile's queries lie in LDS, four of them a read.
 template <typename T, bool DROP, bool HALF>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
     using X = Tile<T>;
@@ -747,6 +754,10 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
 // into dV and dK as in attn_dkv_kernel, dS also goes to LDS (64 bytes a key), from where all waves together make the tile's
 // dQ, a block of 16 queries x 16 elements each, with their 16 columns of K^T in registers.  dQ of more than 256 keys is
 // carried in a float32 buffer that the same thread writes and reads.  One barrier a tile; D comes out of the staging.
+// Bound by the workgroup that a CU holds: eight waves that meet at a barrier for every tile, where matrix and vector unit take
+// turns: 2.6 to 3.4 us a tile of 32 x 256, whose five products take 1.2 us at a large matrix product's rate.  128 packed sequences
+// of up to 512, 12 heads, dropout: 323 us (0.26 PFLOP/s), without dropout 289.  Tiles of 64 queries, half the barriers, measured
+// no better (337 us), nor did orders of the instructions pinned by hand.
 // SHORT: batches of short sequences, see D below (in a batch of long ones it would cost 64 x 200 tokens 70 -> 96 us).
 constexpr int FK = 256, FQ = 32;      // keys at a time, rows of a streamed tile
 constexpr int SPITCH = FQ * 2 + 8;    // bytes a key of dS^T in LDS

@@ -186,7 +186,8 @@ __device__ __forceinline__ void each(const f32x16 (&acc)[BM / 64][BM / 64], int 
                 out(m0 + wm + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * h, n0 + wn + 32 * n + l31, acc[i][n][r]);
 }
 
-// S = q c^T; grid (tiles, splits of d)
+// S = q c^T; grid (tiles, splits of d).  float32 products, tiles of 64: the chip is filled by pieces of d (B = 64 d = 2304:
+// 36 workgroups, 5.6 us; 4096 x 63, 4096 workgroups: 37 us, 57 TFLOP/s).
 template <int BM>
 __global__ __launch_bounds__(256) void loss_scores_kernel(LossArgs a) {
     __shared__ __attribute__((aligned(16))) float lds[2 * BM * KB];
@@ -305,6 +306,7 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossArgs a) {
     if (threadIdx.x == 0) *a.loss = (float)((sum[0] + sum[1] + sum[2] + sum[3]) / a.B);
 }
 
+// 4 us, a launch and the latency of a few loads
 __global__ __launch_bounds__(1024) void loss_mean_kernel(LossArgs a) {
     __shared__ double red[16];
     double s = 0.0;
@@ -340,7 +342,7 @@ __device__ __forceinline__ void put_grad(const LossArgs& a, bool second, int pie
     a.dq[at] = v;
 }
 
-// dq (blockIdx.y = 0) and dc from their pieces, summed in order
+// dq (blockIdx.y = 0) and dc from their pieces, summed in order; bound by reading them
 __global__ __launch_bounds__(256) void loss_join_kernel(LossArgs a) {
     const bool second = blockIdx.y;
     const long long n = (long long)a.B * a.d, at = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
@@ -371,7 +373,8 @@ __global__ __launch_bounds__(256) void loss_join_kernel(LossArgs a) {
     }
 }
 
-// dq and dc, half the grid each; blockIdx.y: a piece of the contraction
+// dq and dc, half the grid each; blockIdx.y: a piece of the contraction.  G is made from S where a tile of it is loaded (once for
+// every 64 columns of d).  B = 64 d = 2304: 9 us; 400 x 256 in 12 pieces: 33 -> 11 us with the join.
 template <int BM>
 __global__ __launch_bounds__(256) void loss_grad_kernel(LossArgs a) {
     __shared__ __attribute__((aligned(16))) float lds[2 * BM * KB];
@@ -422,6 +425,7 @@ __device__ __forceinline__ void split1(float x, unsigned short& hi, unsigned sho
     lo = __builtin_bit_cast(unsigned short, l);
 }
 
+// the largest elements' parts, one a workgroup: q and c of 4096 x 768 in 5.6 us (4.5 TB/s)
 __global__ __launch_bounds__(256) void loss_top_kernel(SplitArgs a) {
     __shared__ float red[4];
     const float* x = blockIdx.y == 2 ? a.rest : blockIdx.y ? a.c : a.q;
@@ -452,7 +456,8 @@ __device__ __forceinline__ float matrix_top(const float* top, int m) {
     return t;
 }
 
-// one wave a row of one matrix; WHOLE: the scale of the whole matrix, otherwise the row's own
+// one wave a row of one matrix; WHOLE: the scale of the whole matrix, otherwise the row's own.  The scores' planes have a scale a
+// row (S_ij only needs its two rows'), the gradients' one a matrix, because their sums run over rows.  4096 x 768: 12 and 9 us.
 template <bool WHOLE>
 __global__ __launch_bounds__(256) void loss_split_kernel(SplitArgs a) {
     const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, m = blockIdx.y;
@@ -479,7 +484,8 @@ __global__ __launch_bounds__(256) void loss_split_kernel(SplitArgs a) {
     if (lane == 0 && !WHOLE) (m ? a.cs : a.qs)[row] = 1.0f / f;
 }
 
-// G without dloss / B as two planes [Bp][Bp], zeros outside [B][B]
+// G without dloss / B as two planes [Bp][Bp], zeros outside [B][B]: one read and one write of B^2 float32, B = 4096 27 us
+// (5 TB/s).  Made where the products load it, it would be made again for every 64 of d.
 __global__ __launch_bounds__(256) void loss_gplanes_kernel(LossArgs a, const float* top, unsigned short* hi, unsigned short* lo, int Bp) {
     const int nb = (Bp + 1023) / 1024, i = blockIdx.x / nb, j = (blockIdx.x % nb * 256 + threadIdx.x) * 4;
     const float f = plane_scale(matrix_top(top, 2));
@@ -619,6 +625,7 @@ __device__ __forceinline__ void clear16(f32x16 (&acc)[2][NB]) {
             for (int r = 0; r < 16; ++r) acc[i][n][r] = 0.0f;
 }
 
+// 128 x 128 tiles; B = 4096 d = 768: 130 us, 0.6 PFLOP/s of float16 products (a large product: 1.1), short loops of 24 steps
 __global__ __launch_bounds__(256, 2) void loss_scores16_kernel(LossArgs a, SplitArgs s) {
     __shared__ __attribute__((aligned(16))) char lds[4 * Planes<128, true>::BYTES];
     const int nt = s.Bp / 128, t = xcd_remap(blockIdx.x, gridDim.x);
@@ -634,7 +641,8 @@ __global__ __launch_bounds__(256, 2) void loss_scores16_kernel(LossArgs a, Split
     });
 }
 
-// dq and dc, half the grid each; blockIdx.y: a piece of the contraction
+// dq and dc, half the grid each; blockIdx.y: a piece of the contraction.  128 x 64 tiles, so that the 768 of B = 4096 d = 768 are
+// resident at once: 222 us, 0.7 PFLOP/s.
 __global__ __launch_bounds__(256, 2) void loss_grad16_kernel(LossArgs a, SplitArgs s, const unsigned short* ghi, const unsigned short* glo) {
     constexpr int LDS1 = 2 * Planes<128, true>::BYTES, LDS2 = 2 * Planes<128, false>::BYTES;
     __shared__ __attribute__((aligned(16))) char lds[(LDS1 > LDS2 ? LDS1 : LDS2) + 2 * Planes<64, false>::BYTES];
