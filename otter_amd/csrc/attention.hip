@@ -769,6 +769,30 @@ __device__ __forceinline__ float dppf(float x) {
     return __uint_as_float(quad<CTRL>(__float_as_uint(x)));
 }
 
+// The sums of sixteen values over the 32 lanes of a half, one a lane: lane l gets that of value lane_value(l).  A step halves the
+// values and the lanes that hold each (15 moves and one shuffle; a butterfly for every value took 64 and 16).
+__device__ __forceinline__ int lane_value(int l31) { return (l31 & 1) * 8 + (l31 >> 1 & 1) * 4 + (l31 >> 2 & 1) * 2 + (l31 >> 3 & 1); }
+__device__ __forceinline__ float lane_sums(float (&v)[16], int l31) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float keep = l31 & 1 ? v[8 + k] : v[k], give = l31 & 1 ? v[k] : v[8 + k];
+        v[k] = keep + dppf<0xB1>(give);                 // lane ^ 1
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float keep = l31 & 2 ? v[4 + k] : v[k], give = l31 & 2 ? v[k] : v[4 + k];
+        v[k] = keep + dppf<0x4E>(give);                 // lane ^ 2
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const float keep = l31 & 4 ? v[2 + k] : v[k], give = l31 & 4 ? v[k] : v[2 + k];
+        v[k] = keep + dppf<0x141>(dppf<0x1B>(give));    // lane ^ 7 of lane ^ 3
+    }
+    const float keep = l31 & 8 ? v[1] : v[0], give = l31 & 8 ? v[0] : v[1];
+    const float x = keep + dppf<0x128>(give);           // lane ^ 8
+    return x + __shfl_xor(x, 16);
+}
+
 template <bool DROP, bool SHORT>
 __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
     typedef bf16_t T;
@@ -876,17 +900,19 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
                         row_products<T>(sc, dp, sQ[buf] + ln.frag<T>(), kf, sO[buf] + ln.frag<T>(), vf);
                         Draws w;
                         if constexpr (DROP) w.keys(a.drop, key.k0, key.k1, bh, j, i0, h);
+                        float e[16];
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const bool in = counts && (!DROP || w.kept_k(r));
-                            float e = in ? exp2_(fmaf(sc[r], a.c2, -sL[buf][acc_row(r, h)])) * dp[r] * a.drop.scale : 0.0f;
-                            e += dppf<0xB1>(e);
-                            e += dppf<0x4E>(e);
-                            e += dppf<0x141>(e);
-                            e += dppf<0x140>(e);
-                            e += __shfl_xor(e, 16);
-                            if (l31 == 0) sE[wave & (SHORT ? 1 : 0)][acc_row(r, h)] = e;
+                        for (int g = 0; g < 4; ++g) {
+                            const float4 L4 = *reinterpret_cast<const float4*>(&sL[buf][8 * g + 4 * h]);
+                            const float lv[4] = {L4.x, L4.y, L4.z, L4.w};
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) {
+                                const int r = 4 * g + t;
+                                e[r] = counts && (!DROP || w.kept_k(r)) ? exp2_(fmaf(sc[r], a.c2, -lv[t])) * dp[r] * a.drop.scale : 0.0f;
+                            }
                         }
+                        const float d = lane_sums(e, l31);
+                        if (l31 < 16) sE[wave & (SHORT ? 1 : 0)][acc_row(lane_value(l31), h)] = d;
                     }
                     __syncthreads();
                     if (tid < FQ) sD[buf][tid] = sE[0][tid] + (kend > 32 ? sE[SHORT ? 1 : 0][tid] : 0.0f);

@@ -373,10 +373,11 @@ PyObject* attention_backward(PyObject* const* a) {
         for (int i = 0; i < 3 && good; ++i) {
             const Tensor* t = tensor(PySequence_Fast_GET_ITEM(seq, i));
             good = t && t->sizes() == s.q.sizes() && t->scalar_type() == s.q.scalar_type() && t->device() == s.q.device() && in_place(*t);
+            for (int64_t n = 0; n < 4 && good && n < t->dim(); ++n) good = t->size(n) <= 1 || t->stride(n) != 0;   // no expanded ones
             if (good) g[i] = *t;
         }
         Py_DECREF(seq);
-        TORCH_CHECK_VALUE(good, what, ": grads must be like q, their heads contiguous, data and strides multiples of 16 bytes");
+        TORCH_CHECK_VALUE(good, what, ": grads must be like q, their heads contiguous, data and strides multiples of 16 bytes, not expanded");
     }
     const int device = s.q.device().index();
     void* const stream = stream_of(device);

@@ -117,7 +117,7 @@ def attention_forward(q, k, v, mask=None, cu_seqlens=None, max_seqlen=None, drop
 def attention_backward(dout, q, k, v, out, lse, mask=None, cu_seqlens=None, max_seqlen=None, dropout_p=0.0, seed=None, call=0,
                        scale=None, grads=None):
     """Gradients (dq, dk, dv) of attention_forward, whose other arguments must be given again.  grads: three tensors to
-    write them to, for instance the views dqkv.unbind(-3) of one buffer."""
+    write them to, for instance the views dqkv.unbind(-3) of one buffer; they may not overlap each other or an operand."""
     return _lib.calls().attention_backward(dout, out, lse, grads, q, k, v, mask, cu_seqlens, _longest(cu_seqlens, max_seqlen),
                                            dropout_p, seed, call, scale)
 

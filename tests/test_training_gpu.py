@@ -874,3 +874,15 @@ def test_one_key_leaves_no_gradient(B, L, H, how, dtype):
     out, lse = T.attention_forward(q, k, v, **kw)
     dq, dk, dv = T.attention_backward(do, q, k, v, out, lse, **kw)
     assert (dq == 0).all() and (dk == 0).all() and (dv != 0).any()
+
+
+def test_expanded_gradient_buffers_are_refused():
+    from otter_amd import training as T
+    q = torch.randn(2, 8, 2, 64, device=_dev())
+    out, lse = T.attention_forward(q, q, q)
+    g = torch.zeros_like(q)
+    with pytest.raises(ValueError, match="grads"):
+        T.attention_backward(out, q, q, q, out, lse, grads=(g, g.clone(), g[:1].expand(2, 8, 2, 64)))
+    one = q[:1]                                                 # a dimension of one may have any stride
+    out, lse = T.attention_forward(one, one, one)
+    T.attention_backward(out, one, one, one, out, lse, grads=tuple(torch.zeros(8, 2, 64, device=_dev())[None] for _ in range(3)))
