@@ -172,7 +172,10 @@ __device__ __forceinline__ void clear(f32x16 (&acc)[BM / 64][BM / 64]) {
             for (int r = 0; r < 16; ++r) acc[i][n][r] = 0.0f;
 }
 
-// out(row, col, value) for every element of the tile
+// row of the tile that register r of an accumulator holds (of lane half 0; half 1 has the fourth after it)
+__device__ __forceinline__ constexpr int acc_row(int r) { return (r & 3) + 8 * (r >> 2); }
+
+// out(row, col, accumulator): register r is element (row + acc_row(r), col)
 template <int BM, typename F>
 __device__ __forceinline__ void each(const f32x16 (&acc)[BM / 64][BM / 64], int m0, int n0, const F& out) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, l31 = lane & 31;
@@ -180,10 +183,7 @@ __device__ __forceinline__ void each(const f32x16 (&acc)[BM / 64][BM / 64], int 
 #pragma unroll
     for (int i = 0; i < BM / 64; ++i)
 #pragma unroll
-        for (int n = 0; n < BM / 64; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                out(m0 + wm + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * h, n0 + wn + 32 * n + l31, acc[i][n][r]);
+        for (int n = 0; n < BM / 64; ++n) out(m0 + wm + 32 * i + 4 * h, n0 + wn + 32 * n + l31, acc[i][n]);
 }
 
 // S = q c^T; grid (tiles, splits of d).  float32 products, tiles of 64: the chip is filled by pieces of d (B = 64 d = 2304:
@@ -201,8 +201,10 @@ __global__ __launch_bounds__(256) void loss_scores_kernel(LossArgs a) {
     product<BM, true, true>(acc, Plain{a.q, a.B, a.d, a.d}, Plain{a.c, a.B, a.d, a.d}, m0, n0, ka, kb, lds);
     float* out = a.splits > 1 ? a.part + (size_t)blockIdx.y * a.B * a.B : a.scores;
     const long long ld = a.splits > 1 ? a.B : a.ld;
-    each<BM>(acc, m0, n0, [&](int i, int j, float v) {
-        if (i < a.B && j < a.B) out[(long long)i * ld + j] = v;
+    each<BM>(acc, m0, n0, [&](int i0, int j, const f32x16& v) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if (i0 + acc_row(r) < a.B && j < a.B) out[(long long)(i0 + acc_row(r)) * ld + j] = v[r];
     });
 }
 
@@ -321,25 +323,37 @@ __global__ __launch_bounds__(1024) void loss_mean_kernel(LossArgs a) {
     }
 }
 
-// Element (row, n) of dq (SECOND: of dc): a piece of its sum to its place, or, where there is one piece, the gradient
-// itself with the hard negative's share.
-__device__ __forceinline__ void put_grad(const LossArgs& a, bool second, int piece, float g, int row, int n, float v) {
-    if (row >= a.B || n >= a.d) return;
-    const long long at = (long long)row * a.d + n;
-    if (a.gsplits > 1) {
-        a.gpart[((long long)piece * 2 + second) * a.B * a.d + at] = v;
+// Elements (row0 + acc_row(r), n) of dq (second: of dc): a piece of their sums to its place, or, where there is one piece, the
+// gradients themselves with the hard negative's share.
+__device__ __forceinline__ void put_grad(const LossArgs& a, bool second, int piece, float g, int row0, int n, const f32x16& v) {
+    if (a.gsplits > 1 || second || !a.neg) {
+        float* out = a.gsplits > 1 ? a.gpart + ((long long)piece * 2 + second) * a.B * a.d : second ? a.dc : a.dq;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if (row0 + acc_row(r) < a.B && n < a.d) out[(long long)(row0 + acc_row(r)) * a.d + n] = v[r];
         return;
     }
-    if (second) {
-        a.dc[at] = v;
-        return;
+    const int nc = min(n, a.d - 1);
+#pragma unroll
+    for (int r0 = 0; r0 < 16; r0 += 8) {
+        float sn[8], lse[8], x[8], y[8];             // eight elements' loads before the first use
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int row = min(row0 + acc_row(r0 + r), a.B - 1);
+            sn[r] = a.scores[(long long)row * a.ld + a.B];
+            lse[r] = a.lse[row];
+            x[r] = a.neg[(long long)row * a.d + nc];
+            y[r] = a.q[(long long)row * a.d + nc];
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int row = row0 + acc_row(r0 + r);
+            if (row >= a.B || n >= a.d) continue;
+            const float gn = __expf(sn[r] - lse[r]) * g;
+            a.dq[(long long)row * a.d + n] = fmaf(gn, x[r], v[r0 + r]);
+            a.dneg[(long long)row * a.d + n] = gn * y[r];
+        }
     }
-    if (a.neg) {
-        const float gn = __expf(a.scores[(long long)row * a.ld + a.B] - a.lse[row]) * g;
-        v = fmaf(gn, a.neg[at], v);
-        a.dneg[at] = gn * a.q[at];
-    }
-    a.dq[at] = v;
 }
 
 // dq (blockIdx.y = 0) and dc from their pieces, summed in order; bound by reading them
@@ -374,7 +388,7 @@ __global__ __launch_bounds__(256) void loss_join_kernel(LossArgs a) {
 }
 
 // dq and dc, half the grid each; blockIdx.y: a piece of the contraction.  G is made from S where a tile of it is loaded (once for
-// every 64 columns of d).  B = 64 d = 2304: 9 us; 400 x 256 in 12 pieces: 33 -> 11 us with the join.
+// every 64 columns of d).  B = 64 d = 2304: 8 us; 400 x 256 in 12 pieces: 33 -> 11 us with the join.
 template <int BM>
 __global__ __launch_bounds__(256) void loss_grad_kernel(LossArgs a) {
     __shared__ __attribute__((aligned(16))) float lds[2 * BM * KB];
@@ -392,7 +406,7 @@ __global__ __launch_bounds__(256) void loss_grad_kernel(LossArgs a) {
         product<BM, false, false>(acc, G, Plain{a.q, a.B, a.d, a.d}, m0, n0, ka, kb, lds);
     else
         product<BM, true, false>(acc, G, Plain{a.c, a.B, a.d, a.d}, m0, n0, ka, kb, lds);
-    each<BM>(acc, m0, n0, [&](int i, int n, float v) { put_grad(a, second, blockIdx.y, g, i, n, v); });
+    each<BM>(acc, m0, n0, [&](int i0, int n, const f32x16& v) { put_grad(a, second, blockIdx.y, g, i0, n, v); });
 }
 
 // ------------------------------------------------------------------ two float16 planes
@@ -609,10 +623,7 @@ __device__ __forceinline__ void each16(const f32x16 (&acc)[2][BN / 64], int m0, 
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int n = 0; n < BN / 64; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                out(m0 + wm + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * h, n0 + wn + 32 * n + l31, acc[i][n][r]);
+        for (int n = 0; n < BN / 64; ++n) out(m0 + wm + 32 * i + 4 * h, n0 + wn + 32 * n + l31, acc[i][n]);
 }
 
 template <int NB>
@@ -636,13 +647,17 @@ __global__ __launch_bounds__(256, 2) void loss_scores16_kernel(LossArgs a, Split
     f32x16 acc[2][2];
     clear16<2>(acc);
     product16<128, true, true>(acc, s.plane[0], s.plane[1], s.dp, s.plane[2], s.plane[3], s.dp, m0, n0, ka, min(s.dp, ka + a.kchunk), lds);
-    each16<128>(acc, m0, n0, [&](int i, int j, float v) {
-        if (i < a.B && j < a.B) out[(long long)i * ld + j] = v * s.qs[i] * s.cs[j];
+    each16<128>(acc, m0, n0, [&](int i0, int j, const f32x16& v) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int i = i0 + acc_row(r);
+            if (i < a.B && j < a.B) out[(long long)i * ld + j] = v[r] * s.qs[i] * s.cs[j];
+        }
     });
 }
 
 // dq and dc, half the grid each; blockIdx.y: a piece of the contraction.  128 x 64 tiles, so that the 768 of B = 4096 d = 768 are
-// resident at once: 222 us, 0.7 PFLOP/s.
+// resident at once: 215 us, 0.7 PFLOP/s.
 __global__ __launch_bounds__(256, 2) void loss_grad16_kernel(LossArgs a, SplitArgs s, const unsigned short* ghi, const unsigned short* glo) {
     constexpr int LDS1 = 2 * Planes<128, true>::BYTES, LDS2 = 2 * Planes<128, false>::BYTES;
     __shared__ __attribute__((aligned(16))) char lds[(LDS1 > LDS2 ? LDS1 : LDS2) + 2 * Planes<64, false>::BYTES];
@@ -658,7 +673,11 @@ __global__ __launch_bounds__(256, 2) void loss_grad16_kernel(LossArgs a, SplitAr
         product16<64, false, false>(acc, ghi, glo, s.Bp, s.plane[0], s.plane[1], s.dp, m0, n0, ka, kb, lds);
     else
         product16<64, true, false>(acc, ghi, glo, s.Bp, s.plane[2], s.plane[3], s.dp, m0, n0, ka, kb, lds);
-    each16<64>(acc, m0, n0, [&](int i, int n, float v) { put_grad(a, second, blockIdx.y, g, i, n, v * back * gback); });
+    each16<64>(acc, m0, n0, [&](int i0, int n, f32x16 v) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[r] = v[r] * back * gback;
+        put_grad(a, second, blockIdx.y, g, i0, n, v);
+    });
 }
 
 // ------------------------------------------------------------------ host side
