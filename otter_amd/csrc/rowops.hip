@@ -10,6 +10,8 @@
 #include "otter_common.h"
 #include "otter_philox.h"
 
+#include <type_traits>
+
 namespace {
 using namespace otter;
 
@@ -162,17 +164,62 @@ struct NormArgs {
     DropArgs drop;
 };
 
-// 8 weights from c on, zeros past the row's end
-__device__ __forceinline__ void load_w(const void* p, int c, int cols, int bf, float v[8]) {
-    const int n = cols - c;
-    if (n <= 0) {
+// A lane holds the groups i LPR + l, i < NG, of a row.  Of NG groups of all lanes only the last can be cut or empty, so that one
+// alone is looked at, and without a branch: a group past the row's end is the row's last 8 elements again, and the one that
+// the end cuts is those, moved to their places.  (With a branch for every group and element of the cut one the kernel of odd
+// rows was 19 KB of code instead of 11: 4097 x 771 float32 11.3 -> 9.2 us forward, 20.8 -> 17.8 backward; 30000 x 771 bfloat16
+// 34 -> 24 and 62 -> 44.)
+template <bool VEC>
+__device__ __forceinline__ void move_cut(int c, int cols, float v[8]) {
+    const int s = c - (cols - 8);                     // 1 .. 7 in the cut group
+    if (VEC) return;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-    } else if (bf) {
-        load8<bf16_t, false>((const bf16_t*)p + c, n, v);
-    } else {
-        load8<float, false>((const float*)p + c, n, v);
+    for (int b = 1; b < 8; b <<= 1) {
+        const bool move = s > 0 && (s & b);
+#pragma unroll
+        for (int e = 0; e + b < 8; ++e) v[e] = move ? v[e + b] : v[e];
     }
+}
+
+// group c of a row p; LAST: it may be cut or empty (VEC: empty)
+template <typename T, bool VEC, bool LAST>
+__device__ __forceinline__ void load_group(const T* p, int c, int cols, Raw<T>& r) {
+    if (!LAST || VEC || cols >= 8) {
+        load_raw<T, VEC>(p + (LAST ? min(c, cols - 8) : c), 8, r);
+    } else {
+        T t[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = p[min(e, cols - 1)];
+        __builtin_memcpy(&r, t, sizeof(t));
+    }
+}
+
+template <typename T, bool VEC, bool LAST>
+__device__ __forceinline__ void unpack_group(const Raw<T>& r, int c, int cols, float v[8]) {
+    unpack<T>(r, v);
+    if (LAST && cols >= 8) move_cut<VEC>(c, cols, v);
+}
+
+// a group of weights; any of them past the row's end
+template <bool VEC, bool LAST>
+__device__ __forceinline__ void load_w(const void* p, int c, int cols, int bf, float v[8]) {
+    if (bf) {
+        Raw<bf16_t> r;
+        load_group<bf16_t, false, LAST>((const bf16_t*)p, c, cols, r);
+        unpack_group<bf16_t, VEC, LAST>(r, c, cols, v);
+    } else {
+        Raw<float> r;
+        load_group<float, false, LAST>((const float*)p, c, cols, r);
+        unpack_group<float, VEC, LAST>(r, c, cols, v);
+    }
+}
+
+// f(group, whether it is the last): the second is a constant
+template <int NG, typename F>
+__device__ __forceinline__ void groups(const F& f) {
+#pragma unroll
+    for (int i = 0; i < NG - 1; ++i) f(i, std::false_type{});
+    f(NG - 1, std::true_type{});
 }
 
 template <int CTRL>
@@ -214,15 +261,12 @@ template <typename T, bool VEC, int LPR, int NG>
 struct RowLoad {
     Raw<T> r[NG];
     __device__ __forceinline__ void load(const void* base, long long row, int cols, int l) {
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            const int c = (i * LPR + l) * 8;
-            // past the row's end: the row's first element again, whole groups only (a value nobody uses)
-            if (VEC)
-                load_raw<T, VEC>((const T*)base + row * cols + (c < cols ? c : 0), 8, r[i]);
-            else if (c < cols)
-                load_raw<T, VEC>((const T*)base + row * cols + c, cols - c, r[i]);
-        }
+        const T* p = (const T*)base + row * cols;
+        groups<NG>([&](int i, auto last) { load_group<T, VEC, last.value>(p, (i * LPR + l) * 8, cols, r[i]); });
+    }
+    template <bool LAST>
+    __device__ __forceinline__ void get(int i, int cols, int l, float v[8]) const {
+        unpack_group<T, VEC, LAST>(r[i], (i * LPR + l) * 8, cols, v);
     }
 };
 
@@ -230,10 +274,9 @@ struct RowLoad {
 template <typename T, bool VEC, int LPR, int NG>
 __device__ __forceinline__ void make_z(const NormArgs& a, const RowLoad<T, VEC, LPR, NG>& x, const RowLoad<T, VEC, LPR, NG>& res,
                                        long long row, int l, u32 k0, u32 k1, float z[NG][8], u32 keep[NG]) {
-#pragma unroll
-    for (int i = 0; i < NG; ++i) {
+    groups<NG>([&](int i, auto last) {
         const int c = (i * LPR + l) * 8;
-        unpack<T>(x.r[i], z[i]);
+        x.template get<last.value>(i, a.cols, l, z[i]);
         if (a.drop.thr) {
             keep[i] = keep8((u32)(c >> 3), (u32)row, a.drop, k0, k1);
 #pragma unroll
@@ -242,19 +285,28 @@ __device__ __forceinline__ void make_z(const NormArgs& a, const RowLoad<T, VEC, 
         // written out as one fma, as are the sums below: a row's bits do not depend on how it is aligned
         if (a.residual) {
             float r[8];
-            unpack<T>(res.r[i], r);
+            res.template get<last.value>(i, a.cols, l, r);
 #pragma unroll
             for (int e = 0; e < 8; ++e) z[i][e] = fmaf(z[i][e], a.drop.scale, r[e]);
         } else if (a.drop.thr) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) z[i][e] *= a.drop.scale;
         }
-        if (c + 8 > a.cols) {
+        if (last.value) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (c + e >= a.cols) z[i][e] = 0.0f;
+            for (int e = 0; e < 8; ++e) z[i][e] = c + (VEC ? 0 : e) < a.cols ? z[i][e] : 0.0f;
         }
-    }
+    });
+}
+
+// a group of a row to memory
+template <typename T, bool VEC, bool LAST>
+__device__ __forceinline__ void store_group(void* base, long long row, int c, int cols, const float v[8]) {
+    T* p = (T*)base + row * cols + c;
+    if (!LAST)
+        store8<T, VEC>(p, 8, v);
+    else if (c < cols)
+        store8<T, VEC>(p, cols - c, v);
 }
 
 struct Seed2 {
@@ -271,7 +323,7 @@ struct Seed2 {
 // mean, then the sum of (z - mean)^2 of the same registers (no cancellation of E z^2 - mean^2): one read of x and the residual,
 // one write, bound by memory.  A row is held by half a wave (up to 1024 columns: two rows a wave, no LDS) or by the workgroup;
 // weight and bias stay in registers over the rows and the next row is loaded while this one is summed.
-// 65536 x 768 bfloat16 with residual and dropout: 49 us = 6.1 TB/s; 4097 x 771 float32, one row a half-wave: 11 us (2.3 TB/s,
+// 65536 x 768 bfloat16 with residual and dropout: 49 us = 6.1 TB/s; 4097 x 771 float32, one row a half-wave: 9 us (2.7 TB/s,
 // the latency of one load, two sums and one store; 4097 x 768: 7).
 template <typename T, bool VEC, int LPR, int NG>
 __global__ __launch_bounds__(256) void ln_fwd_kernel(NormArgs a) {
@@ -286,11 +338,10 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(NormArgs a) {
     x.load(a.x, min(r0 + slot, a.rows - 1), a.cols, l);
     if (a.residual) res.load(a.residual, min(r0 + slot, a.rows - 1), a.cols, l);
     float w[NG][8], b[NG][8];
-#pragma unroll
-    for (int i = 0; i < NG; ++i) {
-        load_w(a.weight, (i * LPR + l) * 8, a.cols, a.wbf16, w[i]);
-        load_w(a.bias, (i * LPR + l) * 8, a.cols, a.wbf16, b[i]);
-    }
+    groups<NG>([&](int i, auto last) {
+        load_w<VEC, last.value>(a.weight, (i * LPR + l) * 8, a.cols, a.wbf16, w[i]);
+        load_w<VEC, last.value>(a.bias, (i * LPR + l) * 8, a.cols, a.wbf16, b[i]);
+    });
     for (; r0 < a.rows; r0 += step) {
         const bool in = r0 + slot < a.rows;       // a half-wave past the end repeats the last row and stores nothing
         const long long row = in ? r0 + slot : a.rows - 1;
@@ -310,16 +361,15 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(NormArgs a) {
         row_sum2<LPR>(s, dummy, lds);
         const float mean = s / (float)a.cols;
         float v = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
+        groups<NG>([&](int i, auto last) {
             const int c = (i * LPR + l) * 8;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float d = z[i][e] - mean;
                 z[i][e] = d;
-                v = fmaf(d, (VEC ? c < a.cols : c + e < a.cols) ? d : 0.0f, v);
+                v = fmaf(d, !last.value || c + (VEC ? 0 : e) < a.cols ? d : 0.0f, v);
             }
-        }
+        });
         row_sum2<LPR>(v, dummy, lds);
         const float rstd = 1.0f / sqrtf(fmaf(v, inv, a.eps));
         if (!in) continue;
@@ -327,15 +377,12 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(NormArgs a) {
             a.mean[row] = mean;
             a.rstd[row] = rstd;
         }
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            const int c = (i * LPR + l) * 8, n = min(8, a.cols - c);
-            if (n <= 0) continue;
+        groups<NG>([&](int i, auto last) {
             float o[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = fmaf(z[i][e] * rstd, w[i][e], b[i][e]);
-            store8<T, VEC>((T*)a.y + row * a.cols + c, n, o);
-        }
+            store_group<T, VEC, last.value>(a.y, row, (i * LPR + l) * 8, a.cols, o);
+        });
     }
 }
 
@@ -364,12 +411,11 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(NormArgs a) {
     };
     fetch(r0);
     float dw[NG][8], db[NG][8], w[NG][8];
-#pragma unroll
-    for (int i = 0; i < NG; ++i) {
-        load_w(a.weight, (i * LPR + l) * 8, a.cols, a.wbf16, w[i]);
+    groups<NG>([&](int i, auto last) {
+        load_w<VEC, last.value>(a.weight, (i * LPR + l) * 8, a.cols, a.wbf16, w[i]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) dw[i][e] = db[i][e] = 0.0f;
-    }
+    });
     for (; r0 < a.rows; r0 += step) {
         const bool in = r0 + slot < a.rows;
         const long long row = in ? r0 + slot : a.rows - 1;
@@ -378,16 +424,12 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(NormArgs a) {
         make_z<T, VEC, LPR, NG>(a, x, res, row, l, k.k0, k.k1, z, keep);
         const float mu = mean, rs = rstd;
         float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
+        groups<NG>([&](int i, auto last) {
             const int c = (i * LPR + l) * 8;
-            unpack<T>(g.r[i], dy[i]);
-            if (!in || c + 8 > a.cols) {
+            g.template get<last.value>(i, a.cols, l, dy[i]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (!in || c + e >= a.cols) dy[i][e] = 0.0f;
-            }
-        }
+            for (int e = 0; e < 8; ++e) dy[i][e] = in && (!last.value || c + (VEC ? 0 : e) < a.cols) ? dy[i][e] : 0.0f;
+        });
         if (r0 + step < a.rows) fetch(r0 + step);
 #pragma unroll
         for (int i = 0; i < NG; ++i)
@@ -404,17 +446,15 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(NormArgs a) {
         row_sum2<LPR>(s1, s2, lds);
         if (!in) continue;
         const float m1 = s1 * inv, m2 = s2 * inv;
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            const int c = (i * LPR + l) * 8, n = min(8, a.cols - c);
-            if (n <= 0) continue;
+        groups<NG>([&](int i, auto last) {
+            const int c = (i * LPR + l) * 8;
             float o[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = rs * fmaf(-z[i][e], m2, dy[i][e] - m1);
-            if (a.dresidual) store8<T, VEC>((T*)a.dresidual + row * a.cols + c, n, o);
+            if (a.dresidual) store_group<T, VEC, last.value>(a.dresidual, row, c, a.cols, o);
             if (a.drop.thr) apply_keep(o, keep[i], a.drop.scale);
-            store8<T, VEC>((T*)a.dx + row * a.cols + c, n, o);
-        }
+            store_group<T, VEC, last.value>(a.dx, row, c, a.cols, o);
+        });
     }
     // the workgroup's sums over its rows, in the order of its row slots
     float* out = a.part + (size_t)blockIdx.x * 2 * a.cols;

@@ -886,3 +886,46 @@ def test_expanded_gradient_buffers_are_refused():
     one = q[:1]                                                 # a dimension of one may have any stride
     out, lse = T.attention_forward(one, one, one)
     T.attention_backward(out, one, one, one, out, lse, grads=tuple(torch.zeros(8, 2, 64, device=_dev())[None] for _ in range(3)))
+
+
+@pytest.mark.parametrize("dtype,wdtype", [(F32, F32), (BF16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("cols", list(range(1, 18)) + [249, 250, 255, 257, 263, 505, 511, 513, 519, 1023, 1025, 1031, 2041, 2049, 4097, 8185, 8191])
+def test_layer_norm_rows_cut_anywhere(cols, dtype, wdtype):
+    """Rows whose last group of eight holds one to eight elements, in the first and the last group of a lane."""
+    from otter_amd import training as T
+    rows, p, dev = 5, 0.2, _dev()
+    x64, x = _rand(170, rows, cols, dtype=dtype)
+    r64, r = _rand(171, rows, cols, dtype=dtype)
+    d64, dy = _rand(172, rows, cols, dtype=dtype)
+    w64, w = _rand(173, cols, dtype=wdtype)
+    b64, b = _rand(174, cols, dtype=wdtype)
+    kw = dict(residual=r, dropout_p=p, seed=_seed(), call=3)
+    y, mean, rstd = T.layer_norm_forward(x, w, b, 1e-5, **kw)
+    dx, dres, dw, db = T.layer_norm_backward(dy, x, w, mean, rstd, **kw)
+    ref = R.layer_norm(x64, w64, b64, 1e-5, r64, p, SEED, 3, d64, dtype, wdtype)
+    for name, t in (("y", y), ("dx", dx), ("dresidual", dres), ("dweight", dw), ("dbias", db)):
+        _close(name, t, ref[name])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cols", [1, 3, 7, 9, 257, 771, 1029])
+def test_layer_norm_writes_nothing_behind_its_rows(cols, dtype):
+    from otter_amd import _lib
+    lib, dev, rows = _lib.load(), _dev(), 9
+    n, code = rows * cols, _lib.OTTER_F32 if dtype == F32 else _lib.OTTER_BF16
+    x, r, dy = (_rand(180 + i, rows, cols, dtype=dtype)[1] for i in range(3))
+    w, b = torch.ones(cols, device=dev), torch.zeros(cols, device=dev)
+    bufs = [torch.full((n + 64,), 7.0, device=dev, dtype=dtype) for _ in range(3)]
+    small = [torch.full((m + 64,), 7.0, device=dev) for m in (rows, rows, cols, cols)]
+    stream = torch.cuda.current_stream().cuda_stream
+    _lib.check(lib.otter_layernorm_forward(0, code, 0, x.data_ptr(), r.data_ptr(), w.data_ptr(), b.data_ptr(), rows, cols, 1e-5, 0.1,
+                                           _seed().data_ptr(), 0, bufs[0].data_ptr(), small[0].data_ptr(), small[1].data_ptr(), stream))
+    need = lib.otter_layernorm_backward_workspace(rows, cols)
+    ws = torch.full((need + 64,), 9, dtype=torch.uint8, device=dev)
+    seed = _seed()
+    _lib.check(lib.otter_layernorm_backward(0, code, 0, dy.data_ptr(), x.data_ptr(), r.data_ptr(), w.data_ptr(), small[0].data_ptr(),
+                                            small[1].data_ptr(), rows, cols, 0.1, seed.data_ptr(), 0, bufs[1].data_ptr(),
+                                            bufs[2].data_ptr(), small[2].data_ptr(), small[3].data_ptr(), ws.data_ptr(), need, stream))
+    for t, m in list(zip(bufs, (n,) * 3)) + list(zip(small, (rows, rows, cols, cols))):
+        assert (t[m:] == 7).all() and torch.isfinite(t).all()
+    assert (ws[need:] == 9).all()
