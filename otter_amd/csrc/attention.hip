@@ -756,7 +756,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
 // carried in a float32 buffer that the same thread writes and reads.  One barrier a tile; D comes out of the staging.
 // Bound by the workgroup that a CU holds: eight waves that meet at a barrier for every tile, where matrix and vector unit take
 // turns: 2.6 to 3.4 us a tile of 32 x 256, whose five products take 1.2 us at a large matrix product's rate.  128 packed sequences
-// of up to 512, 12 heads, dropout: 323 us (0.26 PFLOP/s), without dropout 289.  Tiles of 64 queries, half the barriers, measured
+// of up to 512, 12 heads, dropout: 318 us (0.26 PFLOP/s), without dropout 284.  Tiles of 64 queries, half the barriers, measured
 // no better (337 us), nor did orders of the instructions pinned by hand.
 // SHORT: batches of short sequences, see D below (in a batch of long ones it would cost 64 x 200 tokens 70 -> 96 us).
 constexpr int FK = 256, FQ = 32;      // keys at a time, rows of a streamed tile
@@ -815,11 +815,16 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
     // nothing is shared between workgroups here: an XCD takes the heads of a sequence together (packed, 128 sequences: 323 us,
     // 366 with the pairs going round)
     const Seq s = find_seq(a, blockIdx.x, xcd_remap(blockIdx.x, items));
+    if (s.len == 0) return;
+    const T *Q = head_ptr<T>(a, a.q, s), *K = head_ptr<T>(a, a.k, s), *V = head_ptr<T>(a, a.v, s);
+    const T *O = head_ptr<T>(a, a.o, s), *dO = head_ptr<T>(a, a.dout, s);
+    // the first keys are on their way before the mask is looked at, and the first queries before the keys are stored
+    float4 kf[X::NF], vf[X::NF];
+    load_own<T>(kf, K, a.k.st, min(wave * 32 + l31, s.len - 1), h);
+    load_own<T>(vf, V, a.v.st, min(wave * 32 + l31, s.len - 1), h);
     bool even;
     const int kend = key_end(a, s, even);
     const bool flat = even || kend == 1;
-    const T *Q = head_ptr<T>(a, a.q, s), *K = head_ptr<T>(a, a.k, s), *V = head_ptr<T>(a, a.v, s);
-    const T *O = head_ptr<T>(a, a.o, s), *dO = head_ptr<T>(a, a.dout, s);
     T *dQ = head_ptr<T>(a, a.dq, s), *dK = head_ptr<T>(a, a.dk, s), *dV = head_ptr<T>(a, a.dv, s);
     const u32 bh = (u32)(s.b * a.heads + s.h);
     const Key2 key(a.drop);
@@ -836,25 +841,17 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
     for (int n0 = 0; n0 < s.len; n0 += FK) {
         const int nk = min(FK, kend - n0);                 // keys that may count here
         const int j = n0 + wave * 32 + l31, jc = min(j, s.len - 1);
-        const bool counts = j < kend && (!mask || mask[jc] != 0);
+        bool counts = j < kend;
+        if (mask) counts &= mask[jc] != 0;
         const bool all = __all(counts);
         f32x16 ok[2] = {zero16(), zero16()}, ov[2] = {zero16(), zero16()};
         if (nk > 0) {
             const bool first = n0 == 0, last = n0 + FK >= kend, busy = wave * 32 < nk;
-            float4 kf[X::NF], vf[X::NF];
-            load_own<T>(kf, K, a.k.st, jc, h);
-            load_own<T>(vf, V, a.v.st, jc, h);
-            if (even) zero_frags<T>(kf);
-            // K^T: 16 elements x 256 keys, a lane one element and 8 keys of every 32
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = e * 64 + (tid >> 3), jj = n0 + r;
-                float4 v = *reinterpret_cast<const float4*>(K + (long long)min(jj, s.len - 1) * a.k.st + sc8 * X::EPC);
-                if (even || !(jj < kend && (!mask || mask[min(jj, s.len - 1)] != 0))) v = make_float4(0.f, 0.f, 0.f, 0.f);
-                *reinterpret_cast<float4*>(sK + r * X::PITCH + sc8 * 16) = v;
+            if (!first) {
+                load_own<T>(kf, K, a.k.st, jc, h);
+                load_own<T>(vf, V, a.v.st, jc, h);
             }
-            __syncthreads();
+            if (even) zero_frags<T>(kf);
             float4 rv, ro = make_float4(0.f, 0.f, 0.f, 0.f);
             float rl = 0.0f;
             auto fetch = [&](int i0) {
@@ -881,6 +878,21 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
                 if (tid < FQ) sL[buf][tid] = i0 + tid < s.len ? rl * 1.4426950408889634f : INFINITY;
             };
             fetch(0);
+            // K^T: 16 elements x 256 keys, a lane one element and 8 keys of every 32
+            __syncthreads();
+            float4 kt[4];
+            bool kc[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int jj = n0 + e * 64 + (tid >> 3), jr = min(jj, s.len - 1);
+                kt[e] = *reinterpret_cast<const float4*>(K + (long long)jr * a.k.st + sc8 * X::EPC);
+                kc[e] = !even && jj < kend;
+                if (mask) kc[e] &= mask[jr] != 0;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<float4*>(sK + (e * 64 + (tid >> 3)) * X::PITCH + sc8 * 16) = kc[e] ? kt[e] : make_float4(0.f, 0.f, 0.f, 0.f);
+            __syncthreads();
             store(0, 0);
             if (FQ < s.len) fetch(FQ);
             __syncthreads();                               // K^T is read, tile 0 is there
@@ -1075,7 +1087,7 @@ void launch_fwd(AttnTrainArgs& a, hipStream_t st) {
 //   up to OWN tokens        16 x 70: 19 and 21, 16 x 128: 17.5 and 20.6; 64 x 70: 53 and 39        -> while the CUs hold all pairs
 //   up to FK                16 x 200: 24.4 and 40, 40 x 200: 48 and 65, 8 x 200: 23.5 and 26.7; 4 x 256: 26 and 19.7, 1 x 256: 25
 //                           and 18 (two passes, two waves to a row) -> beyond a quarter of the CUs
-//   longer                  128 packed up to 512: 323 and 420, 16 x 512: 87 and 92, 40 packed: 139 and 143; but 32 x 512 (one and a
+//   longer                  128 packed up to 512: 318 and 420, 16 x 512: 82 and 92, 40 packed: 139 and 143; but 32 x 512 (one and a
 //                           half rounds of workgroups): 163 and 145, 2 x 4001: 626 and 502 -> where the last round is not mostly empty
 // Several workgroups a pair, whose parts of dQ another launch adds up, did not help (16 x 512: 97).
 bool one_pass(const AttnTrainArgs& a, int dtype) {
