@@ -41,6 +41,7 @@ struct AttnTrainArgs {
     const int* cu;             // packed: [B + 1] row offsets; null: dense
     long long T;               // packed: rows of the tensors
     int B, L, heads, nblk;     // L: tokens (dense) / longest sequence (packed); nblk: workgroups a (sequence, head)
+    int group;                 // (sequence, head) pairs whose workgroups are dealt out in turn
     float scale, c2;           // c2 = scale * log2 e
     DropArgs drop;
 };
@@ -54,12 +55,21 @@ struct Seq {
 
 // Workgroups b, b + 8, ... share an XCD and its L2.  The workgroups of one (sequence, head), which read the same rows, go to
 // one XCD; (sequence, head) pairs go round the XCDs one by one, so that every XCD gets its share of long and short sequences.
+// An XCD takes `group` pairs at a time, first every pair's first rows, then the next: the workgroups that have nothing to do (rows
+// past a short sequence's end) come after the others and not between them, where the round robin over the CUs would give
+// some CUs all the work (128 packed sequences of up to 512, forward: 132 -> 122 us).
 __device__ __forceinline__ Seq find_seq(const AttnTrainArgs& a, int bid, int pair = -1) {
     Seq s;
-    const int whole = (a.B * a.heads & ~7) * a.nblk;      // the last pairs, fewer than 8, as they come
-    const int idx = bid < whole ? bid >> 3 : bid - whole;
-    const int bh = pair >= 0 ? pair : bid < whole ? idx / a.nblk * 8 + (bid & 7) : whole / a.nblk + idx / a.nblk;
-    s.blk = pair >= 0 ? 0 : idx % a.nblk;
+    int bh = pair;
+    s.blk = 0;
+    if (pair < 0) {
+        const int pairs = a.B * a.heads, whole = pairs & ~7, end = whole * a.nblk;   // the last pairs, fewer than 8, as they come
+        const int idx = bid < end ? bid >> 3 : bid - end, n = bid < end ? whole >> 3 : pairs - whole;
+        const int first = idx / (a.group * a.nblk) * a.group, size = min(a.group, n - first), r = idx - first * a.nblk;
+        s.blk = r / size;
+        bh = first + r - s.blk * size;
+        bh = bid < end ? bh * 8 + (bid & 7) : whole + bh;
+    }
     s.h = bh % a.heads;
     s.b = bh / a.heads;
     if (a.cu) {
@@ -297,10 +307,16 @@ __device__ __forceinline__ int key_end(const AttnTrainArgs& a, const Seq& s, boo
     even = false;
     if (!a.mask || s.len == 0) return s.len;
     const long long* m = a.mask + (long long)s.b * a.L;
-    for (int c = (s.len - 1) >> 6; c >= 0; --c) {
-        const int j = c * 64 + (threadIdx.x & 63);
-        const u64 bal = __ballot(j < s.len && m[j] != 0);
-        if (bal) return c * 64 + 64 - __builtin_clzll(bal);
+    // four chunks of 64 at a time: a short sequence in a long row costs a latency for every 256 keys it leaves out
+    for (int c = (s.len - 1) >> 6; c >= 0; c -= 4) {
+        long long v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = m[min(max(c - e, 0) * 64 + (int)(threadIdx.x & 63), s.len - 1)];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const u64 bal = __ballot(c >= e && (c - e) * 64 + (int)(threadIdx.x & 63) < s.len && v[e] != 0);
+            if (bal) return (c - e) * 64 + 64 - __builtin_clzll(bal);
+        }
     }
     even = true;
     return s.len;
@@ -406,7 +422,7 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 // that the accumulators are rescaled once or twice a row and not at every tile.
 // Bound by the matrix unit and the vector unit together: of their times only about a third overlaps, with exp2, the draws and
 // the conversion to bfloat16 about as long as the products.  bfloat16: 2 x 4001 tokens, 12 heads, no dropout 131 us
-// = 0.75 PFLOP/s (a large matrix product: 1.15); 128 packed of up to 512 with dropout 131 us, without 96; 16 x 512 ragged 28 us.
+// = 0.75 PFLOP/s (a large matrix product: 1.15); 128 packed of up to 512 with dropout 124 us, without 91; 16 x 512 ragged 28 us.
 // float32, 8 x 512 ragged: 64 us, 57 TFLOP/s on the 32x32x2 products (a large product: 154).
 template <typename T, bool DROP, bool HALF>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnTrainArgs a) {
@@ -1050,6 +1066,8 @@ int fill(const char* what, const otter_attention_args* x, AttnTrainArgs* a, long
     a->scale = x->scale;
     a->c2 = x->scale * 1.4426950408889634f;
     a->lse = x->lse;
+    // K and V of a group stay in a quarter of an XCD's L2 (8 x 2000 tokens, 8 heads, in groups of 8: forward 98 -> 123 us)
+    a->group = 8ll * x->tokens * DH * 2 * (x->dtype == OTTER_BF16 ? 2 : 4) <= 1 << 20 ? 8 : 1;
     a->nblk = x->tokens > OWN ? (x->tokens + OWN - 1) / OWN : 1;     // own_half() may double it
     *rows = x->cu_seqlens ? x->total : (long long)x->batch * x->tokens;
     if ((long long)a->nblk * a->heads * a->B + a->heads > 0x7FFFFFFFll || (long long)a->B * a->heads > 0x7FFFFFFFll)
@@ -1082,20 +1100,24 @@ void launch_fwd(AttnTrainArgs& a, hipStream_t st) {
 }
 
 // One pass over the scores (bfloat16) or two, one for dQ and one for dK and dV.  One pass makes each score tile once and is one
-// launch, but it is one workgroup a (sequence, head) of which a CU holds one, and it needs FK keys to fill its waves.  Measured
-// (us, one pass and two, 12 heads, dropout):
+// launch, but it is one workgroup a (sequence, head) of which a CU holds one, it needs FK keys to fill its waves, and a long
+// sequence among short ones keeps one CU busy when the others are done.  Measured (us, one pass and two, 12 heads, dropout):
 //   up to OWN tokens        16 x 70: 19 and 21, 16 x 128: 17.5 and 20.6; 64 x 70: 53 and 39        -> while the CUs hold all pairs
-//   up to FK                16 x 200: 24.4 and 40, 40 x 200: 48 and 65, 8 x 200: 23.5 and 26.7; 4 x 256: 26 and 19.7, 1 x 256: 25
+//   up to FK                16 x 200: 25 and 38, 64 x 200: 69 and 84, 8 x 200: 23.7 and 24.9; 4 x 256: 26 and 19.7, 1 x 256: 25
 //                           and 18 (two passes, two waves to a row) -> beyond a quarter of the CUs
-//   longer                  128 packed up to 512: 318 and 420, 16 x 512: 82 and 92, 40 packed: 139 and 143; but 32 x 512 (one and a
-//                           half rounds of workgroups): 163 and 145, 2 x 4001: 626 and 502 -> where the last round is not mostly empty
+//   up to 2 FK              64 packed: 170 and 188, 128 packed: 318 and 379, 16 x 512 dense and ragged: 82 and 86, 20 x 512: 84 and
+//                           93; but 32 x 512 (one and a half rounds of workgroups): 163 and 145, one round of packed
+//                           sequences 16 x 512: 79 and 68 -> where the last round is not mostly empty, dense ones also in one
+//   longer, ragged          100 x 700: 625 and 662, 64 x 1000: 783 and 783, packed 552 and 563 (three rounds and more); 16 x 640: 130
+//                           and 106, 16 x 2000 packed: 1044 and 482, 40 x 1500: 1129 and 976 -> from three rounds on
 // Several workgroups a pair, whose parts of dQ another launch adds up, did not help (16 x 512: 97).
 bool one_pass(const AttnTrainArgs& a, int dtype) {
-    const long long pairs = (long long)a.B * a.heads;
+    const long long pairs = (long long)a.B * a.heads, rounds = (pairs + CUS - 1) / CUS;
     if (dtype != OTTER_BF16) return false;
-    if (a.L <= FK) return a.L > OWN ? pairs > CUS / 4 : pairs <= CUS;
-    const long long slots = (pairs + CUS - 1) / CUS * CUS;
-    return slots == CUS ? 4 * pairs >= 3 * slots : 5 * pairs >= 4 * slots;
+    if (a.L <= OWN) return pairs <= CUS;
+    if (a.L <= FK) return pairs > CUS / 4;
+    if (rounds == 1) return a.L <= 2 * FK && !a.cu && 4 * pairs >= 3 * CUS;
+    return (a.L <= 2 * FK || rounds >= 3) && 5 * pairs >= 4 * rounds * CUS;
 }
 
 template <bool DROP>

@@ -929,3 +929,23 @@ def test_layer_norm_writes_nothing_behind_its_rows(cols, dtype):
     for t, m in list(zip(bufs, (n,) * 3)) + list(zip(small, (rows, rows, cols, cols))):
         assert (t[m:] == 7).all() and torch.isfinite(t).all()
     assert (ws[need:] == 9).all()
+
+
+def test_attention_one_pass_three_key_blocks():
+    """Many pairs of more than 512 keys: the carried dQ is written, read and added to, and read and finished."""
+    B, H, L, p = 10, 64, 520, 0.1
+    m = _mask("prefix", B, L)
+    x = [_rand(190 + i, B, L, H, 64, dtype=BF16) for i in range(4)]
+    _check_attention(*x, dict(mask=m.to(_dev()), dropout_p=p, seed=_seed(), call=6), mask=m, p=p)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,L,H", [(1, 700, 3), (3, 300, 5), (9, 130, 9), (17, 257, 7)])
+def test_every_pair_is_dealt_out(B, L, H, dtype):
+    """Numbers of (sequence, head) pairs that are no multiples of anything: every row of every pair, dense and packed."""
+    m = _mask("prefix", B, L)
+    x = [_rand(200 + i, B, L, H, 64, dtype=dtype) for i in range(4)]
+    _check_attention(*x, dict(mask=m.to(_dev()), dropout_p=0.0, seed=None, call=6), mask=m)
+    cu = [L * b for b in range(B + 1)]
+    y = [(t64.flatten(0, 1), t.flatten(0, 1)) for t64, t in x]
+    _check_attention(*y, dict(cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=_dev()), max_seqlen=L), cu=cu)
