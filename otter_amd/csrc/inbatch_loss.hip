@@ -208,8 +208,12 @@ __global__ __launch_bounds__(256) void loss_scores_kernel(LossArgs a) {
     });
 }
 
+// the larger one, a NaN if there is one (fmaxf would drop it, and a row whose scores are not numbers would have a finite loss)
+__device__ __forceinline__ float max_(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+
+// maximum and sum of two parts of a row; parts without weight (no scores, or -inf throughout) have the sum 0
 __device__ __forceinline__ void online(float& m, float& l, float m2, float l2) {
-    const float n = fmaxf(m, m2);
+    const float n = max_(m, m2);
     if (n == -INFINITY) return;
     l = l * __expf(m - n) + l2 * __expf(m2 - n);
     m = n;
@@ -245,7 +249,7 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (j + e == i) v[e] = -INFINITY;
-            const float top = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), n = fmaxf(m, top), base = n == -INFINITY ? 0.0f : n;
+            const float top = max_(max_(v[0], v[1]), max_(v[2], v[3])), n = max_(m, top), base = n == -INFINITY ? 0.0f : n;
             l = l * __expf(m - base) + ((__expf(v[0] - base) + __expf(v[1] - base)) + (__expf(v[2] - base) + __expf(v[3] - base)));
             m = n;
         }
@@ -277,7 +281,7 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(LossArgs a) {
         const float t = row[i];
         float lse, rest, loss;
         if (m <= t) {
-            const float u = l * __expf(m - t);
+            const float u = l * __expf(m - t) + (t - t);   // the last: 0, and NaN for a target's score of +inf (inf - inf)
             loss = log1pf(u);
             lse = t + loss;
             rest = u / (1.0f + u);
