@@ -9,9 +9,13 @@
 // u = sum_(j != i) exp(S_ij - S_ii), the row's loss is log1p(u) and G_ii = -u / (1 + u) dloss / B, good to float32's last bits.
 // Little work: the three products run on v_mfma_f32_32x32x2_f32 (an fma chain: no operand is rounded), G is made from S and
 // lse where a product's tile is loaded.  Much work: every operand is split into two float16 planes, x = (hi + lo) 2^-e with
-// hi + lo good to 22 bits, and hi hi' + hi lo' + lo hi' run on v_mfma_f32_32x32x16_f16, sixteen times float32's rate for
-// three times its products.  What that leaves out is at most 3 2^-22 of each |term|, less than the float32 sums' own rounding
-// over a row of 64 and more.  S is kept (4 B^2 bytes) instead of multiplied out again in the backward pass (2 B^2 d flops).
+// one e for the elements that a sum runs over, and hi hi' + hi lo' + lo hi' run on v_mfma_f32_32x32x16_f16, sixteen times
+// float32's rate for three times its products.  hi + lo is good to 22 bits of an element, or to 2^-39 of the largest one of its e
+// where that is more (elements below 2^-17 of it): what a term loses is at most 3 2^-22 of it or 2^-38 of the largest one a sum
+// could have, less than the float32 sums' own rounding over a row of 64 and more.  So that rows of very different weight in
+// a batch (a confident row's gradient is e^-margin of a hard one's) and of very different size keep that, S has an e for every row
+// of q and of c, dq one for every row of G weighted by the sizes of c's rows, dc one for every COLUMN of G weighted by q's: two
+// pairs of planes of G.  S is kept (4 B^2 bytes) instead of multiplied out again in the backward pass (2 B^2 d flops).
 #include "otter_common.h"
 #include "otter_device.h"
 
@@ -418,15 +422,16 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef u32 u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int SB = 32;             // contraction depth of a staged tile
-constexpr int NMAX = 256;          // workgroups of the pass for the largest element
 
 struct SplitArgs {
     const float *q, *c;            // [B][d]
     unsigned short* plane[4];      // q hi, q lo, c hi, c lo: [Bp][dp], zeros outside [B][d]
-    float *qs, *cs;                // [Bp]: what a row of the planes is to be multiplied by (forward)
-    float* top;                    // [3][NMAX] largest elements of q, c and G (backward: one scale a matrix)
-    const float* rest;             // [B]: a row of G has no larger element
+    float *qs, *cs;                // [Bp]: what a row of the planes is to be multiplied by, 2^-14 of its largest element's power of two
+    unsigned short* gplane[4];     // backward, of G: hi and lo for dq, hi and lo for dc; [Bp][Bp], zeros outside [B][B]
+    float *gq, *gc;                // [Bp]: the scale of a row of the first pair, of a column of the second
+    float *rowtop, *coltop;        // [4 colblocks][Bp], [strips][Bp]: parts of the largest weighted elements of rows and columns
     int B, d, Bp, dp;
+    int strip;                     // rows of a part of coltop; Bp is a multiple of it
 };
 
 // 2^(14 - exponent of top): the largest element then lies in [2^14, 2^15), the smallest half step of a float16 (2^-25) is
@@ -443,48 +448,13 @@ __device__ __forceinline__ void split1(float x, unsigned short& hi, unsigned sho
     lo = __builtin_bit_cast(unsigned short, l);
 }
 
-// the largest elements' parts, one a workgroup: q and c of 4096 x 768 in 5.6 us (4.5 TB/s)
-__global__ __launch_bounds__(256) void loss_top_kernel(SplitArgs a) {
-    __shared__ float red[4];
-    const float* x = blockIdx.y == 2 ? a.rest : blockIdx.y ? a.c : a.q;
-    const long long n = blockIdx.y == 2 ? a.B : (long long)a.B * a.d;
-    float t = 0.0f;
-    // four elements a load, four loads in flight; the last n % 4 by the first threads
-    const long long n4 = n / 4, step = (long long)gridDim.x * 256;
-    const long long first = (long long)blockIdx.x * 256 + threadIdx.x;
-#pragma unroll 4
-    for (long long i = first; i < n4; i += step) {
-        const f4u v = *reinterpret_cast<const f4u*>(x + 4 * i);
-        t = fmaxf(t, fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
-    }
-    if (4 * n4 + first < n) t = fmaxf(t, fabsf(x[4 * n4 + first]));
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = t;
-    __syncthreads();
-    if (threadIdx.x == 0) a.top[blockIdx.y * NMAX + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-}
-
-// the largest element of matrix m, in every lane
-__device__ __forceinline__ float matrix_top(const float* top, int m) {
-    float t = 0.0f;
-    for (int i = threadIdx.x & 63; i < NMAX; i += 64) t = fmaxf(t, top[m * NMAX + i]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o));
-    return t;
-}
-
-// one wave a row of one matrix; WHOLE: the scale of the whole matrix, otherwise the row's own.  The scores' planes have a scale a
-// row (S_ij only needs its two rows'), the gradients' one a matrix, because their sums run over rows.  4096 x 768: 12 and 9 us.
-template <bool WHOLE>
+// One wave a row of one matrix, which has its own scale.  4096 x 768: 12 us.
 __global__ __launch_bounds__(256) void loss_split_kernel(SplitArgs a) {
     const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, m = blockIdx.y;
     if (row >= a.Bp) return;
     const float* x = (m ? a.c : a.q) + (long long)row * a.d;
     float t = 0.0f;
-    if (WHOLE) {
-        t = matrix_top(a.top, m);
-    } else if (row < a.B) {
+    if (row < a.B) {
         for (int i = lane; i < a.d; i += 64) t = fmaxf(t, fabsf(x[i]));
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o));
@@ -499,22 +469,88 @@ __global__ __launch_bounds__(256) void loss_split_kernel(SplitArgs a) {
         __builtin_memcpy(hi + 4 * i, h, 8);
         __builtin_memcpy(lo + 4 * i, l, 8);
     }
-    if (lane == 0 && !WHOLE) (m ? a.cs : a.qs)[row] = 1.0f / f;
+    if (lane == 0) (m ? a.cs : a.qs)[row] = 1.0f / f;
 }
 
-// G without dloss / B as two planes [Bp][Bp], zeros outside [B][B]: one read and one write of B^2 float32, B = 4096 27 us
-// (5 TB/s).  Made where the products load it, it would be made again for every 64 of d.
-__global__ __launch_bounds__(256) void loss_gplanes_kernel(LossArgs a, const float* top, unsigned short* hi, unsigned short* lo, int Bp) {
-    const int nb = (Bp + 1023) / 1024, i = blockIdx.x / nb, j = (blockIdx.x % nb * 256 + threadIdx.x) * 4;
-    const float f = plane_scale(matrix_top(top, 2));
-    if (j >= Bp) return;
-    const Grad G{a.scores, a.lse, a.rest, a.ld, a.B, f};
+// a row's size as a power of two, from what its planes are multiplied by
+__device__ __forceinline__ float row_size(float s) { return s * 16384.0f; }
+
+// Parts of max_j |G_ij| size(c_j) for every row and max_i |G_ij| size(q_i) for every column: a workgroup takes `strip` rows x 1024
+// columns, a thread four columns, four rows at a time and the next four on their way.  One read of S: B = 4096 25 us (2.7 TB/s).
+__global__ __launch_bounds__(256) void loss_gtop_kernel(LossArgs a, SplitArgs s) {
+    const int j = blockIdx.y * 1024 + threadIdx.x * 4, i0 = blockIdx.x * s.strip, last = i0 + s.strip - 1;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    float* rowtop = s.rowtop + (long long)(blockIdx.y * 4 + wave) * s.Bp;
+    float size[4], col[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) size[e] = row_size(s.cs[min(j, s.Bp - 4) + e]);
+    f4u next[4];
+    auto fetch = [&](int i) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) next[r] = load4(a.scores, a.ld, a.B, a.B, min(i + r, last), j);   // past the strip's end its last row again
+    };
+    fetch(i0);
+    for (int i = i0; i <= last; i += 4) {
+        float t[4];
+        f4u v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = next[r];
+        if (i + 4 <= last) fetch(i + 4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = min(i + r, last);
+            const float size_q = row_size(s.qs[row]), l = row < a.B ? a.lse[row] : 0.0f, rest = row < a.B ? a.rest[row] : 0.0f;
+            t[r] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float g = row < a.B && j + e < a.B ? (j + e == row ? rest : __expf(v[r][e] - l)) : 0.0f;
+                t[r] = fmaxf(t[r], g * size[e]);
+                col[e] = fmaxf(col[e], g * size_q);
+            }
+        }
+        // four maxima over 64 lanes: two steps halve the values and the lanes that hold each, lane l keeps row 2 (l & 1) + (l >> 1 & 1)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) t[r] = fmaxf(lane & 1 ? t[2 + r] : t[r], __shfl_xor(lane & 1 ? t[r] : t[2 + r], 1));
+        float top = fmaxf(lane & 2 ? t[1] : t[0], __shfl_xor(lane & 2 ? t[0] : t[1], 2));
+#pragma unroll
+        for (int o = 4; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const int row = i + 2 * (lane & 1) + (lane >> 1);
+        if (lane < 4 && row <= last) rowtop[row] = top;
+    }
+    if (j < s.Bp) *reinterpret_cast<float4*>(s.coltop + (long long)blockIdx.x * s.Bp + j) = make_float4(col[0], col[1], col[2], col[3]);
+}
+
+// blockIdx.y = 0: the rows' scales, 1: the columns'; 64 of them a workgroup, a quarter of the parts a wave
+__global__ __launch_bounds__(256) void loss_gscale_kernel(SplitArgs s, int nrow, int ncol) {
+    __shared__ float top[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.x * 64 + lane, parts = blockIdx.y ? ncol : nrow;
+    const float* p = (blockIdx.y ? s.coltop : s.rowtop) + n;
+    float t = 0.0f;
+#pragma unroll 8
+    for (int k = wave; k < parts; k += 4) t = fmaxf(t, p[(long long)k * s.Bp]);
+    top[wave][lane] = t;
+    __syncthreads();
+    if (wave == 0) (blockIdx.y ? s.gc : s.gq)[n] = plane_scale(fmaxf(fmaxf(top[0][lane], top[1][lane]), fmaxf(top[2][lane], top[3][lane])));
+}
+
+// G without dloss / B as the two pairs of planes: one read of B^2 float32 and a write of twice as much, B = 4096
+// 33 us (6.1 TB/s).  Made where the products load it, it would be made again for every 64 of d.
+__global__ __launch_bounds__(256) void loss_gplanes_kernel(LossArgs a, SplitArgs s) {
+    const int nb = (s.Bp + 1023) / 1024, i = blockIdx.x / nb, j = (blockIdx.x % nb * 256 + threadIdx.x) * 4;
+    if (j >= s.Bp) return;
+    const Grad G{a.scores, a.lse, a.rest, a.ld, a.B, 1.0f};
     const f4u v = G(i, j);
+    const float size_q = row_size(s.qs[i]), f = s.gq[i];
+    const long long at = (long long)i * s.Bp + j;
     unsigned short h[4], l[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) split1(v[e], h[e], l[e]);
-    __builtin_memcpy(hi + (long long)i * Bp + j, h, 8);
-    __builtin_memcpy(lo + (long long)i * Bp + j, l, 8);
+    for (int e = 0; e < 4; ++e) split1(v[e] * row_size(s.cs[j + e]) * f, h[e], l[e]);
+    __builtin_memcpy(s.gplane[0] + at, h, 8);
+    __builtin_memcpy(s.gplane[1] + at, l, 8);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split1(v[e] * size_q * s.gc[j + e], h[e], l[e]);
+    __builtin_memcpy(s.gplane[2] + at, h, 8);
+    __builtin_memcpy(s.gplane[3] + at, l, 8);
 }
 
 // A tile of one operand, both planes, on its way to LDS.  KC: SB contiguous k of W rows (80 bytes a row in LDS); otherwise W
@@ -661,25 +697,25 @@ __global__ __launch_bounds__(256, 2) void loss_scores16_kernel(LossArgs a, Split
 }
 
 // dq and dc, half the grid each; blockIdx.y: a piece of the contraction.  128 x 64 tiles, so that the 768 of B = 4096 d = 768 are
-// resident at once: 215 us, 0.7 PFLOP/s.
-__global__ __launch_bounds__(256, 2) void loss_grad16_kernel(LossArgs a, SplitArgs s, const unsigned short* ghi, const unsigned short* glo) {
+// resident at once: 240 us, 0.64 PFLOP/s.
+__global__ __launch_bounds__(256, 2) void loss_grad16_kernel(LossArgs a, SplitArgs s) {
     constexpr int LDS1 = 2 * Planes<128, true>::BYTES, LDS2 = 2 * Planes<128, false>::BYTES;
     __shared__ __attribute__((aligned(16))) char lds[(LDS1 > LDS2 ? LDS1 : LDS2) + 2 * Planes<64, false>::BYTES];
     const int nt = (a.d + 63) / 64, half = gridDim.x / 2, id = xcd_remap(blockIdx.x, gridDim.x);
     const bool second = id >= half;
     const int t = second ? id - half : id, m0 = (t / nt) * 128, n0 = (t % nt) * 64;
     const float g = *a.dloss / (float)a.B;
-    const float back = 1.0f / plane_scale(matrix_top(s.top, second ? 0 : 1)), gback = g / plane_scale(matrix_top(s.top, 2));
+    const float* scale = second ? s.gc : s.gq;
     const int ka = blockIdx.y * a.gchunk, kb = min(s.Bp, ka + a.gchunk);
     f32x16 acc[2][1];
     clear16<1>(acc);
     if (second)
-        product16<64, false, false>(acc, ghi, glo, s.Bp, s.plane[0], s.plane[1], s.dp, m0, n0, ka, kb, lds);
+        product16<64, false, false>(acc, s.gplane[2], s.gplane[3], s.Bp, s.plane[0], s.plane[1], s.dp, m0, n0, ka, kb, lds);
     else
-        product16<64, true, false>(acc, ghi, glo, s.Bp, s.plane[2], s.plane[3], s.dp, m0, n0, ka, kb, lds);
+        product16<64, true, false>(acc, s.gplane[0], s.gplane[1], s.Bp, s.plane[2], s.plane[3], s.dp, m0, n0, ka, kb, lds);
     each16<64>(acc, m0, n0, [&](int i0, int n, f32x16 v) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) v[r] = v[r] * back * gback;
+        for (int r = 0; r < 16; ++r) v[r] = v[r] * 0x1p-14f / scale[i0 + acc_row(r)] * g;   // a power of two, and the sizes' 2^14
         put_grad(a, second, blockIdx.y, g, i0, n, v);
     });
 }
@@ -698,14 +734,16 @@ int pieces(long long tiles, int k, int want, int least) {
     return max(1, min(s, most));
 }
 
-// Two float16 planes or float32, by B^2 d with d in whole tiles.  The planes cost passes over the operands, and over G in the
-// backward pass.  float32 -> planes, us: forward B = 600 d = 768 30 -> 40, 400 x 2304 44 -> 47, 500 x 2304 50 -> 47, 800 x 768
-// 51 -> 43, 1500 x 256 33 -> 35, 2000 x 256 42 -> 40; backward 800 x 256 27 -> 33, 1000 x 256 33 -> 34, 600 x 768 36 -> 36,
-// 1500 x 256 75 -> 43, 500 x 2304 64 -> 49.  Of short sums what the planes leave out would show beside float32's own rounding:
-// scores of less than 64 elements stay float32 (and take the same time: 38 and 36 us of B = 4096).
+// Two float16 planes or float32, by B^2 d with d in whole tiles.  The planes cost passes over the operands, and in the
+// backward pass two over S and one over G.  float32 -> planes, us: forward B = 600 d = 768 30 -> 40, 400 x 2304 44 -> 47, 500 x
+// 2304 50 -> 47, 800 x 768 51 -> 43, 1500 x 256 33 -> 35, 2000 x 256 42 -> 40; backward 600 x 768 37 -> 45, 700 x 768 58 -> 49,
+// 1000 x 768 90 -> 57, 1000 x 256 33 -> 40, 1200 x 256 49 -> 49, 1500 x 256 76 -> 54, 1500 x 128 41 -> 46, 2000 x 128 58 -> 57,
+// 400 x 2304 45 -> 60, 500 x 2304 61 -> 61, 600 x 2304 71 -> 68, 400 x 4608 61 -> 79; of less than 128 columns the passes over
+// G are as long as the products, 3000 x 64 68 -> 77, 4096 x 64 103 -> 106.  Of short sums what the planes leave out would show
+// beside float32's own rounding: scores of less than 64 elements stay float32 (and take the same time: 38 and 36 us of B = 4096).
 double loss_work(int B, int d) { return (double)B * B * round_up(d, 64); }
 bool score_planes(int B, int d) { return B > 256 && d >= 64 && loss_work(B, d) > 4e8; }
-bool grad_planes(int B, int d) { return B > 256 && loss_work(B, d) > 2.7e8; }
+bool grad_planes(int B, int d) { return B > 500 && loss_work(B, d) > (d < 128 ? 1e9 : 3.6e8); }
 
 // Pieces of the scores' contraction (d) and of the gradients' (B) where there are few tiles, each piece `chunk` deep.  Fewer or
 // shallower pieces and more or deeper ones measured 0 to 20 % slower; without pieces: scores of B = 600 d = 768 54 -> 40 us
@@ -741,6 +779,8 @@ struct Take {                      // pieces of a workspace, 16-byte aligned
 };
 
 void take_planes(Take& t, SplitArgs& s) {
+    s.qs = t.template operator()<float>(s.Bp);
+    s.cs = t.template operator()<float>(s.Bp);
     for (auto& x : s.plane) x = t.template operator()<unsigned short>((int64_t)s.Bp * s.dp);
 }
 
@@ -752,6 +792,7 @@ SplitArgs split_args(const float* q, const float* c, int B, int d) {
     s.d = d;
     s.Bp = round_up(B, 128);
     s.dp = round_up(d, 64);
+    s.strip = max(4, s.Bp / 128);
     return s;
 }
 
@@ -760,23 +801,23 @@ int64_t lay_forward(void* ws, LossArgs& a, SplitArgs& s) {
     Take t{(char*)ws};
     a.rowloss = t.template operator()<float>(a.B);
     a.done = t.template operator()<unsigned>(1);
-    if (score_planes(a.B, a.d)) {
-        s.qs = t.template operator()<float>(s.Bp);
-        s.cs = t.template operator()<float>(s.Bp);
-        take_planes(t, s);
-    }
+    if (score_planes(a.B, a.d)) take_planes(t, s);
     if (a.splits > 1) a.part = t.template operator()<float>((int64_t)a.splits * a.B * a.B);
     return t.used;
 }
 
-int64_t lay_backward(void* ws, LossArgs& a, SplitArgs& s, unsigned short** g) {
+int col_blocks(const SplitArgs& s) { return (s.Bp + 1023) / 1024; }
+
+int64_t lay_backward(void* ws, LossArgs& a, SplitArgs& s) {
     Take t{(char*)ws};
     if (a.gsplits > 1) a.gpart = t.template operator()<float>((int64_t)a.gsplits * 2 * s.B * s.d);
     if (!grad_planes(s.B, s.d)) return t.used;
-    s.top = t.template operator()<float>(3 * NMAX);
     take_planes(t, s);
-    g[0] = t.template operator()<unsigned short>((int64_t)s.Bp * s.Bp);
-    g[1] = t.template operator()<unsigned short>((int64_t)s.Bp * s.Bp);
+    for (auto& x : s.gplane) x = t.template operator()<unsigned short>((int64_t)s.Bp * s.Bp);
+    s.gq = t.template operator()<float>(s.Bp);
+    s.gc = t.template operator()<float>(s.Bp);
+    s.rowtop = t.template operator()<float>(4ll * col_blocks(s) * s.Bp);
+    s.coltop = t.template operator()<float>((int64_t)(s.Bp / s.strip) * s.Bp);
     return t.used;
 }
 
@@ -825,7 +866,7 @@ int otter_inbatch_loss_forward(int device, const float* q, const float* c, const
     lay_forward(workspace, a, s);
     hipStream_t st = (hipStream_t)stream;
     if (score_planes(B, d)) {
-        loss_split_kernel<false><<<dim3((unsigned)(s.Bp / 4), 2), 256, 0, st>>>(s);
+        loss_split_kernel<<<dim3((unsigned)(s.Bp / 4), 2), 256, 0, st>>>(s);
         loss_scores16_kernel<<<dim3((unsigned)((s.Bp / 128) * (s.Bp / 128)), (unsigned)a.splits), 256, 0, st>>>(a, s);
     } else {
         const unsigned nt = (unsigned)(B + 63) / 64;
@@ -853,8 +894,7 @@ int64_t otter_inbatch_loss_backward_workspace(int B, int d) {
     LossArgs a = {};
     a.gsplits = grad_splits(B, d, &a.gchunk);
     SplitArgs s = split_args(nullptr, nullptr, B, d);
-    unsigned short* g[2];
-    return lay_backward(nullptr, a, s, g);
+    return lay_backward(nullptr, a, s);
 }
 
 int otter_inbatch_loss_backward(int device, const float* dloss, const float* q, const float* c, const float* neg_c, int B, int d,
@@ -885,15 +925,15 @@ int otter_inbatch_loss_backward(int device, const float* dloss, const float* q, 
     a.ld = ld;
     a.gsplits = grad_splits(B, d, &a.gchunk);
     SplitArgs s = split_args(q, c, B, d);
-    unsigned short* gp[2];
-    lay_backward(workspace, a, s, gp);
+    lay_backward(workspace, a, s);
     hipStream_t st = (hipStream_t)stream;
     if (grad_planes(B, d)) {
-        s.rest = a.rest;
-        loss_top_kernel<<<dim3(NMAX, 3), 256, 0, st>>>(s);
-        loss_split_kernel<true><<<dim3((unsigned)(s.Bp / 4), 2), 256, 0, st>>>(s);
-        loss_gplanes_kernel<<<(unsigned)s.Bp * ((unsigned)(s.Bp + 1023) / 1024), 256, 0, st>>>(a, s.top, gp[0], gp[1], s.Bp);
-        loss_grad16_kernel<<<dim3((unsigned)(2 * (s.Bp / 128) * ((d + 63) / 64)), (unsigned)a.gsplits), 256, 0, st>>>(a, s, gp[0], gp[1]);
+        const unsigned nb = (unsigned)col_blocks(s), strips = (unsigned)(s.Bp / s.strip);
+        loss_split_kernel<<<dim3((unsigned)(s.Bp / 4), 2), 256, 0, st>>>(s);
+        loss_gtop_kernel<<<dim3(strips, nb), 256, 0, st>>>(a, s);
+        loss_gscale_kernel<<<dim3((unsigned)(s.Bp / 64), 2), 256, 0, st>>>(s, (int)(4 * nb), (int)strips);
+        loss_gplanes_kernel<<<(unsigned)s.Bp * nb, 256, 0, st>>>(a, s);
+        loss_grad16_kernel<<<dim3((unsigned)(2 * (s.Bp / 128) * ((d + 63) / 64)), (unsigned)a.gsplits), 256, 0, st>>>(a, s);
     } else {
         loss_grad_kernel<64><<<dim3((unsigned)(2 * tiles), (unsigned)a.gsplits), 256, 0, st>>>(a);
     }

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import training_ref as R
-from tests.test_training_gpu import _dev, _rand, _same
+from tests.test_training_gpu import _close, _dev, _rand, _same
 
 pytestmark = pytest.mark.gpu
 NAN, INF = float("nan"), float("inf")
@@ -70,3 +70,50 @@ def test_an_infinity_in_a_block_is_not_hidden(B, d, sign):
         assert not torch.isfinite(loss), float(loss)
         if sign > 0:
             assert torch.isnan(loss) and torch.isnan(stats[1, i])
+
+
+def _margins(B, d, seed, margin):
+    """float32 inputs: row i's target lies margin[i] above the others, whose scores are a few margins / sqrt(d)."""
+    c = torch.nn.functional.normalize(_rand(seed, B, d)[0], dim=1).float().double()
+    return (margin[:, None] * c).float().double(), c
+
+
+def _close_loss(q64, c64, names=("loss", "rest", "dq", "dc")):
+    ref = R.inbatch_loss(q64, c64, None, 1.0)
+    loss, _, stats, dq, dc, _ = _loss_step(q64.float().to(_dev()), c64.float().to(_dev()), None)
+    got = {"loss": loss, "rest": stats[1], "lse": stats[0], "dq": dq, "dc": dc}
+    for name in names:
+        _close(name, got[name], ref[name])
+
+
+# float32 products, float16 planes in one and in several pieces
+MIXED = [(200, 128), (640, 768), (700, 768), (2000, 128), (1100, 300), (4096, 64), (600, 2304)]
+
+
+@pytest.mark.parametrize("B,d", MIXED)
+@pytest.mark.parametrize("margin", [12.0, 25.0, 60.0])
+@pytest.mark.parametrize("hard", ["spread", "confused"])
+def test_loss_of_confident_rows_beside_one_that_is_not(B, d, margin, hard):
+    """The other rows' gradients are e^-margin of the hard one's and as exact; a confused row has its weight on one wrong column,
+    so that the other columns' gradients are as small."""
+    m = torch.full((B,), margin, dtype=torch.float64)
+    q, c = _margins(B, d, 330, m)
+    i = B // 3
+    q[i] = 0.01 * c[i] if hard == "spread" else margin * c[(i + 7) % B]
+    _close_loss(q.float().double(), c)
+
+
+@pytest.mark.parametrize("B,d", MIXED)
+def test_loss_of_rows_of_every_confidence(B, d):
+    m = torch.linspace(0.0, 40.0, B, dtype=torch.float64)[torch.randperm(B, generator=torch.Generator().manual_seed(7))]
+    _close_loss(*_margins(B, d, 340, m))
+
+
+@pytest.mark.parametrize("B,d", MIXED)
+def test_loss_of_blocks_of_very_different_sizes(B, d):
+    """Blocks whose sizes span twelve decades, met by questions that point away from the large ones."""
+    size = torch.logspace(-6, 6, B, dtype=torch.float64)[torch.randperm(B, generator=torch.Generator().manual_seed(8))][:, None]
+    u = torch.nn.functional.normalize(_rand(350, B, d)[0].abs(), dim=1)
+    c = (size * u).float().double()
+    q = _rand(351, B, d)[0].abs() * torch.where(torch.arange(B)[:, None] % 2 == 0, -1e-3, 1e-9)
+    _close_loss(q.float().double(), c, ("loss", "lse", "dq", "dc"))
