@@ -302,12 +302,16 @@ __device__ __forceinline__ void store_own(T* dst, const f32x16 (&o)[2], float f,
 }
 
 // ------------------------------------------------------------------ keys that count
-// How far keys count in this sequence (last one + 1), and whether none does (then all do, evenly).
-__device__ __forceinline__ int key_end(const AttnTrainArgs& a, const Seq& s, bool& even) {
+// How far keys count in this sequence (last one + 1), whether none does (`even`: then all do, evenly), and whether the
+// probabilities are what they are whatever q and k hold (`flat`: evenly, or one key has them all): no gradient reaches those.
+__device__ __forceinline__ int key_end(const AttnTrainArgs& a, const Seq& s, bool& even, bool& flat) {
     even = false;
+    flat = s.len == 1;
     if (!a.mask || s.len == 0) return s.len;
     const long long* m = a.mask + (long long)s.b * a.L;
-    // four chunks of 64 at a time: a short sequence in a long row costs a latency for every 256 keys it leaves out
+    int end = 0;
+    // four chunks of 64 at a time: a short sequence in a long row costs a latency for every 256 keys it leaves out; past the
+    // last key that counts the walk goes on only as long as no other is found
     for (int c = (s.len - 1) >> 6; c >= 0; c -= 4) {
         long long v[4];
 #pragma unroll
@@ -315,11 +319,17 @@ __device__ __forceinline__ int key_end(const AttnTrainArgs& a, const Seq& s, boo
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const u64 bal = __ballot(c >= e && (c - e) * 64 + (int)(threadIdx.x & 63) < s.len && v[e] != 0);
-            if (bal) return (c - e) * 64 + 64 - __builtin_clzll(bal);
+            if (!bal) continue;
+            if (end || (bal & (bal - 1))) {            // a second key
+                flat = false;
+                return end ? end : (c - e) * 64 + 64 - __builtin_clzll(bal);
+            }
+            end = (c - e) * 64 + 64 - __builtin_clzll(bal);
         }
     }
-    even = true;
-    return s.len;
+    even = end == 0;
+    flat = true;
+    return even ? s.len : end;
 }
 
 // bit r: key j0 + r counts.  The mask's value of this lane's key is loaded a tile before it is needed.
@@ -435,8 +445,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnTrainArgs a) {
     const int items = a.nblk * a.heads * a.B;
     if ((int)blockIdx.x >= items) return zero_outside<T>(a, blockIdx.x - items, a.o, a.lse);
     const Seq s = find_seq(a, blockIdx.x);
-    bool even;
-    const int kend = key_end(a, s, even);
+    bool even, flat;
+    const int kend = key_end(a, s, even, flat);
     const T *Q = head_ptr<T>(a, a.q, s), *K = head_ptr<T>(a, a.k, s), *V = head_ptr<T>(a, a.v, s);
     T* O = head_ptr<T>(a, a.o, s);
     const u32 bh = (u32)(s.b * a.heads + s.h);
@@ -554,8 +564,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
     const int items = a.nblk * a.heads * a.B;
     if ((int)blockIdx.x >= items) return zero_outside<T>(a, blockIdx.x - items, a.dq, nullptr);
     const Seq s = find_seq(a, blockIdx.x);
-    bool even;
-    const int kend = key_end(a, s, even);
+    bool even, flat;
+    const int kend = key_end(a, s, even, flat);
     const T *Q = head_ptr<T>(a, a.q, s), *K = head_ptr<T>(a, a.k, s), *V = head_ptr<T>(a, a.v, s);
     const T *O = head_ptr<T>(a, a.o, s), *dO = head_ptr<T>(a, a.dout, s);
     T* dQ = head_ptr<T>(a, a.dq, s);
@@ -577,7 +587,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnTrainArgs a) {
         load_own<T>(qf, Q, a.q.st, ic, h);
         const float lse2 = a.lse[s.stat + ic] * 1.4426950408889634f;
         f32x16 o[2] = {zero16(), zero16()};
-        if (!even && kend > 1) {                    // even, and with one key: dS = 0
+        if (!flat) {                                // dS = 0 otherwise, not what is left of P (Z dP - D)
             KeyBits kb(a, s, even);
             Stage<T> rk(K, a.k.st, s.len), rv(V, a.v.st, s.len);
             kb.fetch(0);
@@ -672,10 +682,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
         return zero_outside<T>(a, blockIdx.x - items, a.dv, nullptr);
     }
     const Seq s = find_seq(a, blockIdx.x);
-    bool even;
-    const int kend = key_end(a, s, even);
+    bool even, flat;
+    const int kend = key_end(a, s, even, flat);
     const T *Q = head_ptr<T>(a, a.q, s), *K = head_ptr<T>(a, a.k, s), *V = head_ptr<T>(a, a.v, s);
-    const bool flat = even || kend == 1;       // one key: dS = 0, not what is left of P dO V^T - D
     const T* dO = head_ptr<T>(a, a.dout, s);
     T *dK = head_ptr<T>(a, a.dk, s), *dV = head_ptr<T>(a, a.dv, s);
     const u32 bh = (u32)(s.b * a.heads + s.h);
@@ -838,9 +847,8 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
     float4 kf[X::NF], vf[X::NF];
     load_own<T>(kf, K, a.k.st, min(wave * 32 + l31, s.len - 1), h);
     load_own<T>(vf, V, a.v.st, min(wave * 32 + l31, s.len - 1), h);
-    bool even;
-    const int kend = key_end(a, s, even);
-    const bool flat = even || kend == 1;
+    bool even, flat;
+    const int kend = key_end(a, s, even, flat);
     T *dQ = head_ptr<T>(a, a.dq, s), *dK = head_ptr<T>(a, a.dk, s), *dV = head_ptr<T>(a, a.dv, s);
     const u32 bh = (u32)(s.b * a.heads + s.h);
     const Key2 key(a.drop);

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import training_ref as R
-from tests.test_training_gpu import _close, _dev, _rand, _same
+from tests.test_training_gpu import BF16, F32, _check_attention, _close, _dev, _rand, _same, _seed
 
 pytestmark = pytest.mark.gpu
 NAN, INF = float("nan"), float("inf")
@@ -117,3 +117,33 @@ def test_loss_of_blocks_of_very_different_sizes(B, d):
     c = (size * u).float().double()
     q = _rand(351, B, d)[0].abs() * torch.where(torch.arange(B)[:, None] % 2 == 0, -1e-3, 1e-9)
     _close_loss(q.float().double(), c, ("loss", "lse", "dq", "dc"))
+
+
+# ---------------------------------------------------------------------------------------------------------- attention
+# one pass over the scores (bfloat16) with rows of one, two and three blocks of 256 keys; two passes, with one and two waves to 32 rows
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,L,H", [(4, 40, 2), (3, 70, 2), (130, 70, 2), (3, 128, 3), (5, 200, 64), (4, 300, 64), (13, 520, 64), (3, 530, 2), (5, 150, 64)])
+@pytest.mark.parametrize("at", ["middle", "last", "each"])
+def test_one_key_anywhere_leaves_no_gradient(B, L, H, at, dtype):
+    """With one key the probabilities are 1 whatever q and k are, wherever the key stands."""
+    from otter_amd import training as T
+    q, k, v, do = (_rand(360 + i, B, L, H, 64, dtype=dtype)[1] * 3 for i in range(4))
+    where = torch.tensor([L // 2 if at == "middle" else L - 1 if at == "last" else (37 * b + 1) % L for b in range(B)], device=_dev())
+    mask = (torch.arange(L, device=_dev())[None, :] == where[:, None]).long()
+    kw = dict(mask=mask, dropout_p=0.1, seed=_seed(), call=6)
+    out, lse = T.attention_forward(q, k, v, **kw)
+    dq, dk, dv = T.attention_backward(do, q, k, v, out, lse, **kw)
+    assert (dq == 0).all() and (dk == 0).all(), (float(dq.abs().max()), float(dk.abs().max()))
+    assert (dv[mask == 0] == 0).all() and (dv[mask != 0] != 0).any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("L,keys", [(70, (0, 69)), (70, (3, 4)), (200, (0, 199)), (300, (63, 64)), (600, (0, 599)), (600, (1, 320))])
+def test_two_keys_far_apart(L, keys, dtype):
+    """Two keys that count, in one chunk of the mask's 64 and in chunks that are looked at one after the other."""
+    B, H = 3, 2
+    m = torch.zeros(B, L, dtype=torch.int64)
+    m[:, list(keys)] = 1
+    m[1, keys[0]] = 0                                           # and a sequence with one beside them
+    x = [_rand(370 + i, B, L, H, 64, dtype=dtype) for i in range(4)]
+    _check_attention(*x, dict(mask=m.to(_dev()), dropout_p=0.1, seed=_seed(), call=6), mask=m, p=0.1)
