@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <dlfcn.h>
@@ -515,6 +516,7 @@ PyObject* entry(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK_TYPE(n == N, "expected ", N, " arguments, got ", n);
     if (F != load) TORCH_CHECK(lib.check, "otter_amd._calls.load() has not been called");
+    at::NoGradGuard no_grad;               // copies and casts made here are no part of a caller's graph
     return F(a);
     END_HANDLE_TH_ERRORS
 }

@@ -147,3 +147,21 @@ def test_two_keys_far_apart(L, keys, dtype):
     m[1, keys[0]] = 0                                           # and a sequence with one beside them
     x = [_rand(370 + i, B, L, H, 64, dtype=dtype) for i in range(4)]
     _check_attention(*x, dict(mask=m.to(_dev()), dropout_p=0.1, seed=_seed(), call=6), mask=m, p=0.1)
+
+
+# ------------------------------------------------------------------------------------------------- autograd's own records
+def test_explicit_halves_have_no_history():
+    """Whatever p is and whatever has to be copied or cast on the way."""
+    from otter_amd import inbatch as IB, training as T
+    x = torch.randn(6, 8, device=_dev(), requires_grad=True)
+    w = torch.ones(8, device=_dev(), requires_grad=True)
+    for p in (0.0, 0.3):
+        for t in (x, x.t(), x * 1.0):
+            assert not T.dropout_forward(t, p, _seed()).requires_grad
+        out = torch.empty(6, 8, device=_dev())
+        assert T.dropout_forward(x, p, _seed(), out=out) is out and not out.requires_grad
+        assert not any(t.requires_grad for t in T.layer_norm_forward(x.bfloat16(), w, w, dropout_p=p, seed=_seed()))
+    assert not any(t.requires_grad for t in IB.inbatch_loss_forward(x.bfloat16(), x * 2.0))
+    # the differentiable call keeps it
+    g, = torch.autograd.grad(T.dropout(x, 0.0, None).sum(), x)
+    assert (g == 1).all()
