@@ -148,6 +148,8 @@ PyObject* results(const Ts&... ts) {
 
 const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* out_ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+// a caller's tensor is written: whoever saved it for a backward pass is to find out
+void written(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
 
 // ------------------------------------------------------------------ dropout
 PyObject* dropout(const char* what, PyObject* ox, PyObject* op, PyObject* oseed, PyObject* ocall, PyObject* oout) {
@@ -168,6 +170,7 @@ PyObject* dropout(const char* what, PyObject* ox, PyObject* op, PyObject* oseed,
         } else {
             const Tensor in = x.contiguous();
             out = to ? *to : at::empty_like(in);
+            if (to) written(out);
             const int64_t cols = in.dim() ? in.sizes().back() : 1;
             rc = lib.otter_dropout(x.device().index(), dtype_code(x), ptr(in), out_ptr(out), cols ? in.numel() / cols : 0, cols,
                                    (float)d.p, d.seed, d.call, stream);
@@ -389,8 +392,10 @@ PyObject* attention_backward(PyObject* const* a) {
         s.operands();
         Attention::place(dout);
         Attention::place(out);
-        for (Tensor& t : g)
-            if (!t.defined()) t = make(s.q.sizes(), s.q);
+        for (Tensor& t : g) {
+            if (t.defined()) written(t);
+            else t = make(s.q.sizes(), s.q);
+        }
         s.args.out = view(out), s.args.dout = view(dout);
         s.args.dq = view(g[0]), s.args.dk = view(g[1]), s.args.dv = view(g[2]);
         bytes = lib.otter_attention_backward_workspace(&s.args);

@@ -165,3 +165,21 @@ def test_explicit_halves_have_no_history():
     # the differentiable call keeps it
     g, = torch.autograd.grad(T.dropout(x, 0.0, None).sum(), x)
     assert (g == 1).all()
+
+
+def test_tensors_that_are_written_say_so():
+    """A tensor saved for a backward pass and then written by a call: the backward pass refuses instead of using the new values."""
+    from otter_amd import training as T
+    for p in (0.0, 0.3):
+        x = torch.randn(6, 8, device=_dev(), requires_grad=True)
+        y = x.exp()                                             # its backward pass needs y
+        T.dropout_forward(y.detach(), p, _seed(), out=y.detach())
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    q = torch.randn(2, 8, 2, 64, device=_dev())
+    out, lse = T.attention_forward(q, q, q)
+    buf = torch.randn(2, 8, 3, 2, 64, device=_dev(), requires_grad=True)
+    y = buf.exp()
+    T.attention_backward(out, q, q, q, out, lse, grads=y.detach().unbind(2))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
