@@ -724,6 +724,9 @@ __global__ __launch_bounds__(256, 2) void loss_grad16_kernel(LossArgs a, SplitAr
 int check_loss(const char* what, int B, int d, int ld, int ncol) {
     if (B < 1 || d < 1) return set_err(OTTER_EINVAL, "%s: bad B=%d d=%d (the mean over no rows is undefined)", what, B, d);
     if (B > LOSS_MAX_B) return set_err(OTTER_EINVAL, "%s: B=%d exceeds %d", what, B, LOSS_MAX_B);
+    // the gradients' grid: two halves of 64 x 64 tiles, 256 threads each, fewer than 2^32 threads; it also keeps columns in an int
+    if ((int64_t)((B + 63) / 64) * ((d - 1) / 64 + 1) > 0x7FFFFF)
+        return set_err(OTTER_EINVAL, "%s: B=%d x d=%d is too large for one launch", what, B, d);
     if (ld < ncol) return set_err(OTTER_EINVAL, "%s: ld=%d is less than the %d columns of the scores", what, ld, ncol);
     return OTTER_OK;
 }
@@ -906,7 +909,6 @@ int otter_inbatch_loss_backward(int device, const float* dloss, const float* q, 
         return set_err(OTTER_EINVAL, "inbatch_loss_backward: NULL buffer");
     if ((rc = check_workspace("inbatch_loss_backward", workspace, workspace_bytes, otter_inbatch_loss_backward_workspace(B, d)))) return rc;
     const long long tiles = (long long)((B + 63) / 64) * ((d + 63) / 64);
-    if (tiles > 0x3FFFFFFF) return set_err(OTTER_EINVAL, "inbatch_loss_backward: B=%d x d=%d is too large for one launch", B, d);
     DeviceGuard g(device);
     if (!g.ok) return set_err(OTTER_EHIP, "inbatch_loss_backward: hipSetDevice(%d) failed", device);
     LossArgs a = {};
