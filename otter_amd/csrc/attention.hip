@@ -1078,7 +1078,8 @@ int fill(const char* what, const otter_attention_args* x, AttnTrainArgs* a, long
     a->group = 8ll * x->tokens * DH * 2 * (x->dtype == OTTER_BF16 ? 2 : 4) <= 1 << 20 ? 8 : 1;
     a->nblk = x->tokens > OWN ? (x->tokens + OWN - 1) / OWN : 1;     // own_half() may double it
     *rows = x->cu_seqlens ? x->total : (long long)x->batch * x->tokens;
-    if ((long long)a->nblk * a->heads * a->B + a->heads > 0x7FFFFFFFll || (long long)a->B * a->heads > 0x7FFFFFFFll)
+    // a launch has fewer than 2^32 threads: 256 an item, 512 where the backward pass takes a pair of two items and more at once
+    if ((long long)a->B * a->heads > 0xFFFFFF || (long long)a->nblk * a->heads * a->B + 2ll * a->heads > 0xFFFFFF)
         return set_err(OTTER_EINVAL, "%s: batch x heads x tokens is too large for one launch", what);
     return OTTER_OK;
 }
