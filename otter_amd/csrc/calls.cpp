@@ -159,13 +159,18 @@ PyObject* dropout(const char* what, PyObject* ox, PyObject* op, PyObject* oseed,
     TORCH_CHECK_VALUE(oout == Py_None || (to && to->sizes() == x.sizes() && to->scalar_type() == x.scalar_type() &&
                                           to->device() == x.device() && to->is_contiguous()),
                       what, ": out must be a contiguous ", x.scalar_type(), " tensor of shape ", x.sizes(), " on ", x.device());
+    if (to && x.is_contiguous()) {         // otherwise a copy of x is read
+        const char *a = (const char*)x.const_data_ptr(), *b = (const char*)to->const_data_ptr();
+        const int64_t bytes = x.numel() * (int64_t)x.element_size();
+        TORCH_CHECK_VALUE(a == b || a >= b + bytes || b >= a + bytes, what, ": out overlaps x (it may be x itself)");
+    }
     void* const stream = stream_of(x.device().index());
     int rc = 0;
     Tensor out;
     {
         NoGil no_gil;
         if (d.p == 0.0) {
-            if (to) to->copy_(x);
+            if (to) to->copy_(x.contiguous());      // copied first where out is another view of it
             else out = x.clone();
         } else {
             const Tensor in = x.contiguous();
@@ -382,6 +387,11 @@ PyObject* attention_backward(PyObject* const* a) {
         }
         Py_DECREF(seq);
         TORCH_CHECK_VALUE(good, what, ": grads must be like q, their heads contiguous, data and strides multiples of 16 bytes, not expanded");
+        const Tensor* const all[] = {&g[0], &g[1], &g[2], &s.q, &s.k, &s.v, &dout, &out};
+        for (int i = 0; i < 3; ++i)
+            for (int j = i + 1; j < 8; ++j)
+                TORCH_CHECK_VALUE(s.q.numel() == 0 || g[i].const_data_ptr() != all[j]->const_data_ptr(), what,
+                                  ": grads may not be one another or an operand");
     }
     const int device = s.q.device().index();
     void* const stream = stream_of(device);

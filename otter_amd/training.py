@@ -32,7 +32,7 @@ def new_seed(device=None, generator=None):
 # ------------------------------------------------------------------------------------------------------------ dropout
 def dropout_forward(x, p, seed, call=0, out=None):
     """y = x * keep / (1 - p); the draws are counted along x's last dimension, the others together are its rows.
-    A dropped value is zero whatever it was.  out may be x itself."""
+    A dropped value is zero whatever it was.  out may be x itself but not overlap it otherwise."""
     return _lib.calls().dropout_forward(x, p, seed, call, out)
 
 

@@ -183,3 +183,27 @@ def test_tensors_that_are_written_say_so():
     T.attention_backward(out, q, q, q, out, lse, grads=y.detach().unbind(2))
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+# -------------------------------------------------------------------------------------------------------- shared memory
+def test_overlapping_outputs_are_refused():
+    from otter_amd import training as T
+    buf = torch.randn(100, device=_dev())
+    for p in (0.0, 0.3):
+        for x, out in ((buf[:64], buf[1:65]), (buf[32:96], buf[:64]), (buf[:64].view(8, 8), buf[8:72].view(8, 8))):
+            with pytest.raises(ValueError, match="overlaps"):
+                T.dropout_forward(x, p, _seed(), out=out)
+        x = torch.randn(8, 8, device=_dev())                    # a view that has to be copied first may be overwritten
+        exp = T.dropout_forward(x.t(), p, _seed())
+        assert torch.equal(T.dropout_forward(x.t(), p, _seed(), out=x), exp)
+        T.dropout_forward(buf[:32], p, _seed(), out=buf[32:64])
+    q, k, v, do = (torch.randn(2, 8, 2, 64, device=_dev()) for _ in range(4))
+    out, lse = T.attention_forward(q, k, v)
+    a, b, c = (torch.empty_like(q) for _ in range(3))
+    for grads in ((a, a, c), (a, b, a), (a, b, b), (q, b, c), (a, k, c), (a, b, v), (do, b, c), (a, out, c), (k, b, c)):
+        with pytest.raises(ValueError, match="one another or an operand"):
+            T.attention_backward(do, q, k, v, out, lse, grads=grads)
+    ref = T.attention_backward(do, q, k, v, out, lse)
+    _same(T.attention_backward(do, q, k, v, out, lse, grads=(a, b, c)), ref)
+    empty = torch.empty(0, 8, 2, 64, device=_dev())
+    T.attention_backward(empty, empty, empty, empty, empty, torch.empty(0, 2, 8, device=_dev()), grads=(empty,) * 3)
