@@ -404,7 +404,8 @@ typedef struct otter_attention_args {
     float* lse;
     otter_view dout, dq, dk, dv;      /* backward only */
     void* workspace;                  /* backward only: otter_attention_backward_workspace() bytes, 16-byte
-                                       * aligned (may be 0) */
+                                       * aligned (may be 0).  The size depends on the sizes, on whether there is a
+                                       * mask or cu_seqlens and on total: ask with the call's own arguments */
     int64_t workspace_bytes;
 } otter_attention_args;
 

@@ -1110,23 +1110,35 @@ void launch_fwd(AttnTrainArgs& a, hipStream_t st) {
 
 // One pass over the scores (bfloat16) or two, one for dQ and one for dK and dV.  One pass makes each score tile once and is one
 // launch, but it is one workgroup a (sequence, head) of which a CU holds one, it needs FK keys to fill its waves, and a long
-// sequence among short ones keeps one CU busy when the others are done.  Measured (us, one pass and two, 12 heads, dropout):
-//   up to OWN tokens        16 x 70: 19 and 21, 16 x 128: 17.5 and 20.6; 64 x 70: 53 and 39        -> while the CUs hold all pairs
-//   up to FK                16 x 200: 25 and 38, 64 x 200: 69 and 84, 8 x 200: 23.7 and 24.9; 4 x 256: 26 and 19.7, 1 x 256: 25
-//                           and 18 (two passes, two waves to a row) -> beyond a quarter of the CUs
-//   up to 2 FK              64 packed: 170 and 188, 128 packed: 318 and 379, 16 x 512 dense and ragged: 82 and 86, 20 x 512: 84 and
-//                           93; but 32 x 512 (one and a half rounds of workgroups): 163 and 145, one round of packed
-//                           sequences 16 x 512: 79 and 68 -> where the last round is not mostly empty, dense ones also in one
-//   longer, ragged          100 x 700: 625 and 662, 64 x 1000: 783 and 783, packed 552 and 563 (three rounds and more); 16 x 640: 130
-//                           and 106, 16 x 2000 packed: 1044 and 482, 40 x 1500: 1129 and 976 -> from three rounds on
+// sequence among short ones keeps one CU busy when the others are done: how full a batch is, rows over batch x longest, decides with
+// the number of rounds of workgroups.  The host knows it of a packed batch and of a dense one without a mask; dense ones with
+// a mask count as ragged.  Measured (kernels alone, us, one pass and two, 12 heads, dropout; ragged: lengths from an eighth on):
+//   up to OWN tokens  16 x 70: 15 and 18, 21 x 128: 16.4 and 21, ragged 20.5 and 21.7; 32 x 70: 20.5 and 23, ragged 28 and 24, 32 x 33: 19
+//                     and 17 -> while the CUs hold all pairs
+//   up to FK          16 x 200: 25 and 41, 64 x 200: 73 and 97, ragged 72 and 87, 6 x 200: 23 and 26, ragged 24 and 25; 4 x 256: 26 and
+//                     20, 4 x 129: 17 and 17 -> beyond a quarter of the CUs
+//   up to 2 FK        full: 10 x 512 81 and 63, 12 x 512 81 and 85, 20 x 512 89 and 109, 14 x 300 47 and 46, 16 x 300 48 and 57 -> when
+//   (one round)       two passes no longer hold all their workgroups at once; with a mask 13 x 512 82 and 79, 14 x 512 83 and 85, 20 x
+//                     512 84 and 98, 14 x 300 49 and 44, 18 x 300 50 and 53 -> from three quarters of the CUs on; packed ragged 16 x
+//                     512 80 and 80, 20 x 300 46 and 42 -> two passes
+//   (more rounds)     22 x 512 159 and 132, 32 x 512 163 and 163, 36 x 512 170 and 181, ragged 161 and 157, 42 x 512 181 and 210, ragged
+//                     170 and 174, packed 151 and 140, 128 packed 318 and 379 -> where the last round is not mostly empty
+//   longer            full: 21 x 700 169 and 211, 40 x 1500 1307 and 1447, 64 x 2000 3675 and 3998; 16 x 1500 615 and 578; with a mask 40 x 700
+//                     305 and 279, 40 x 1500 1219 and 995, 64 x 700 413 and 450, 64 x 1000 738 and 793, 64 x 1500 1555 and 1554, 64 x 2000 2858
+//                     and 2574 -> full ones where the last round is not mostly empty, with a mask from three rounds on and
+//                     up to 6 FK; packed by how full, 40 x 700: 0.70 299 and 253, 0.80 303 and 297, 0.90 313 and 349; 64 x 1000: 0.56 601
+//                     and 577, 0.70 674 and 729; 64 x 1500: 0.56 1274 and 1102, 0.70 1441 and 1446, 0.80 1632 and 1744
 // Several workgroups a pair, whose parts of dQ another launch adds up, did not help (16 x 512: 97).
 bool one_pass(const AttnTrainArgs& a, int dtype) {
     const long long pairs = (long long)a.B * a.heads, rounds = (pairs + CUS - 1) / CUS;
     if (dtype != OTTER_BF16) return false;
     if (a.L <= OWN) return pairs <= CUS;
     if (a.L <= FK) return pairs > CUS / 4;
-    if (rounds == 1) return a.L <= 2 * FK && !a.cu && 4 * pairs >= 3 * CUS;
-    return (a.L <= 2 * FK || rounds >= 3) && 5 * pairs >= 4 * rounds * CUS;
+    const bool last = 5 * pairs >= 4 * rounds * CUS;           // the last round is not mostly empty
+    const bool full = a.cu ? 15 * a.T >= (rounds >= 3 ? 10 : 12) * (long long)a.B * a.L : !a.mask;
+    if (a.L > 2 * FK) return last && (full || (!a.cu && rounds >= 3 && a.L <= 6 * FK));
+    if (rounds > 1) return last;
+    return full ? a.nblk * pairs > 2 * CUS : !a.cu && 4 * pairs >= 3 * CUS;
 }
 
 template <bool DROP>
