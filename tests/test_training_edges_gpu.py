@@ -4,7 +4,8 @@ import pytest
 import torch
 
 from oracle import training_ref as R
-from tests.test_training_gpu import BF16, F32, _check_attention, _close, _dev, _rand, _same, _seed
+from tests.test_training_gpu import BF16, F32, _check_attention, _close, _dev, _mask, _rand, _same, _seed
+from tests.test_training_paths import takes_one_pass
 
 pytestmark = pytest.mark.gpu
 NAN, INF = float("nan"), float("inf")
@@ -147,6 +148,40 @@ def test_two_keys_far_apart(L, keys, dtype):
     m[1, keys[0]] = 0                                           # and a sequence with one beside them
     x = [_rand(370 + i, B, L, H, 64, dtype=dtype) for i in range(4)]
     _check_attention(*x, dict(mask=m.to(_dev()), dropout_p=0.1, seed=_seed(), call=6), mask=m, p=0.1)
+
+
+# The backward pass in one pass and in two on either side of the rules that choose; the path is asserted, so that a rule that
+# moves does not leave one of them untested
+@pytest.mark.parametrize("p", [0.0, 0.1])
+@pytest.mark.parametrize("lens,lead,tail,H,one", [([300, 20, 1, 256, 400, 0, 130], 3, 70, 64, True), ([512, 257, 33, 290, 511, 64, 500], 0, 0, 64, True),
+                                                  ([520] * 4, 0, 0, 64, True), ([520, 500, 516, 513], 2, 30, 64, True), ([600, 450, 500, 1, 530], 0, 5, 150, True),
+                                                  ([600, 20, 130, 0, 257], 0, 5, 150, False), ([300, 20, 1, 256], 0, 9, 64, False)])
+def test_attention_packed_either_way(lens, lead, tail, H, one, p):
+    cu = [lead]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    total = cu[-1] + tail
+    assert takes_one_pass(len(lens), max(lens), H, total=total) == one
+    x = [_rand(380 + i, total, H, 64, dtype=BF16) for i in range(4)]
+    for t64, t in x:
+        for rows in (slice(0, lead), slice(cu[-1], total)):
+            t64[rows] = 0
+            t[rows] = NAN
+    cut = torch.tensor(cu, dtype=torch.int32, device=_dev())
+    _check_attention(*x, dict(cu_seqlens=cut, max_seqlen=max(lens), dropout_p=p, seed=_seed(), call=6), cu=cu, p=p)
+
+
+@pytest.mark.parametrize("p", [0.0, 0.1])
+@pytest.mark.parametrize("B,L,H,kind,one", [(4, 520, 64, None, True), (4, 777, 60, None, True), (3, 300, 60, None, True), (3, 300, 64, "holes", True),
+                                            (2, 300, 64, None, False), (4, 520, 64, "prefix", False), (11, 530, 64, "alternate", True), (3, 260, 40, "tile", False)])
+def test_attention_dense_either_way(B, L, H, kind, one, p):
+    assert takes_one_pass(B, L, H, mask=kind is not None) == one
+    m = None if kind is None else _mask(kind, B, L)
+    x = [_rand(390 + i, B, L, H, 64, dtype=BF16) for i in range(4)]
+    kw = dict(dropout_p=p, seed=_seed() if p else None, call=6)
+    if m is not None:
+        kw["mask"] = m.to(_dev())
+    _check_attention(*x, kw, mask=m, p=p)
 
 
 # ------------------------------------------------------------------------------------------------- autograd's own records
