@@ -57,7 +57,7 @@ struct Seq {
 // one XCD; (sequence, head) pairs go round the XCDs one by one, so that every XCD gets its share of long and short sequences.
 // An XCD takes `group` pairs at a time, first every pair's first rows, then the next: the workgroups that have nothing to do (rows
 // past a short sequence's end) come after the others and not between them, where the round robin over the CUs would give
-// some CUs all the work (128 packed sequences of up to 512, forward: 132 -> 122 us).
+// some CUs all the work if a pair's workgroups divide their number.
 __device__ __forceinline__ Seq find_seq(const AttnTrainArgs& a, int bid, int pair = -1) {
     Seq s;
     int bh = pair;
@@ -1074,9 +1074,12 @@ int fill(const char* what, const otter_attention_args* x, AttnTrainArgs* a, long
     a->scale = x->scale;
     a->c2 = x->scale * 1.4426950408889634f;
     a->lse = x->lse;
-    // K and V of a group stay in a quarter of an XCD's L2 (8 x 2000 tokens, 8 heads, in groups of 8: forward 98 -> 123 us)
-    a->group = 8ll * x->tokens * DH * 2 * (x->dtype == OTTER_BF16 ? 2 : 4) <= 1 << 20 ? 8 : 1;
     a->nblk = x->tokens > OWN ? (x->tokens + OWN - 1) / OWN : 1;     // own_half() may double it
+    // Pairs one by one or eight at a time (find_seq), us, lengths from an eighth on, forward / two-pass backward.  Packed bfloat16:
+    // two workgroups a pair 256 x 256 92 / 295 -> 81 / 263, four 128 x 512 134 / 420 -> 117 / 364, 64 x 512 with 8 heads 54 / 148 -> 48 / 137;
+    // but three 170 x 384 100 / 306 -> 106 / 321, five 102 x 640 137 / 398 -> 151 / 449, eight 20 x 1024 77 / 200 -> 80 / 215, sixteen 16 x
+    // 2048 188 / 496 -> 244 / 656.  float32, four: packed 128 x 512 622 / 1974 -> 550 / 1723, with a mask 642 / 2520 -> 675 / 2178
+    a->group = a->nblk == 2 || a->nblk == 4 ? 8 : 1;
     *rows = x->cu_seqlens ? x->total : (long long)x->batch * x->tokens;
     // a launch has fewer than 2^32 threads: 256 an item, 512 where the backward pass takes a pair of two items and more at once
     if ((long long)a->B * a->heads > 0xFFFFFF || (long long)a->nblk * a->heads * a->B + 2ll * a->heads > 0xFFFFFF)

@@ -184,6 +184,20 @@ def test_attention_dense_either_way(B, L, H, kind, one, p):
     _check_attention(*x, kw, mask=m, p=p)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,L,H", [(13, 140, 9), (5, 400, 7), (3, 512, 11), (7, 260, 3)])
+def test_every_pair_of_several_workgroups(B, L, H, dtype):
+    """Pairs dealt out one by one and eight at a time, whole eights and a rest: every row of every pair, dense and packed."""
+    m = _mask("prefix", B, L)
+    x = [_rand(400 + i, B, L, H, 64, dtype=dtype) for i in range(4)]
+    _check_attention(*x, dict(mask=m.to(_dev()), dropout_p=0.1, seed=_seed(), call=6), mask=m, p=0.1)
+    cu = [0]
+    for n in m.sum(1).tolist():
+        cu.append(cu[-1] + n)
+    y = [(t64[m != 0], t[m.to(_dev()) != 0]) for t64, t in x]
+    _check_attention(*y, dict(cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=_dev()), max_seqlen=L), cu=cu)
+
+
 # ------------------------------------------------------------------------------------------------- autograd's own records
 def test_explicit_halves_have_no_history():
     """Whatever p is and whatever has to be copied or cast on the way."""
