@@ -1089,11 +1089,13 @@ int fill(const char* what, const otter_attention_args* x, AttnTrainArgs* a, long
 
 // Two waves share their rows (HALF): twice the workgroups, each half as long, for twice the staging of tiles.  Sequences of up
 // to 64 rows leave no wave idle that way and stage no more (64 x 64 tokens, 12 heads, float32: 22.8 -> 17.7 us forward, 75 -> 59
-// backward).  Longer ones take it where there are few workgroups, us forward / backward, 12 heads, dropout:
-//   bfloat16  1 x 1024 26 / 62 -> 20 / 44, 8 x 300 16 / 39 -> 12 / 30, 1 x 4096 136 / 321 -> 115 / 300
-//   float32   1 x 1024 87 / 265 -> 51 / 149, 8 x 512 87 / 257 -> 77 / 218
-// and no longer with 432 (12 x 300: 16 / 40 -> 15 / 44) and 480 workgroups (20 x 256 forward: 15 -> 17).  Between 65 and 128 rows
-// it gains nothing (16 x 128 float32 15.8 / 50 -> 16.7 / 52).
+// backward).  Longer ones take it where there are few workgroups; us forward / backward in two passes, 12 heads, dropout, no mask:
+//   bfloat16  192 workgroups (1 x 2048) 50 / 117 -> 46 / 108, 288 (6 x 512) 23 / 57 -> 21 / 57, 384 (8 x 512) 23.5 / 57.6 -> 21.3 / 57.4,
+//             4 x 1024 40 / 95 -> 35 / 94, 2 x 2048 72 / 171 -> 64 / 161; but 396 (11 x 300) 16.7 / 41 -> 15.2 / 45, 432 (9 x 512)
+//             23.6 / 58 -> 26.4 / 68, 480 (5 x 1024) 41 / 98 -> 45 / 114
+//   float32   288 (6 x 512) 82 / 257 -> 73 / 212, 384 (8 x 512) 83 / 258 -> 75 / 214, 4 x 1024 157 / 491 -> 136 / 400; 432 (12 x 300) 56 / 171 ->
+//             49 / 143 but 9 x 512 82 / 260 -> 91 / 274, 504 (14 x 300) 57 / 174 -> 62 / 181
+// Between 65 and 128 rows it gains nothing (16 x 128 float32 15.8 / 50 -> 16.7 / 52).
 bool own_half(AttnTrainArgs& a) {
     if (a.L > OWN / 2 && (a.L <= OWN || (long long)a.nblk * a.heads * a.B > CUS * 3 / 2)) return false;
     a.nblk = a.L > OWN / 2 ? (a.L + OWN / 2 - 1) / (OWN / 2) : 1;

@@ -23,7 +23,7 @@ namespace {
 using namespace otter;
 
 constexpr int LOSS_MAX_B = 65536;
-constexpr int MEAN_B = 64;         // up to here the rows' launch takes the mean as well
+constexpr int MEAN_B = 48;         // up to here the rows' launch takes the mean as well
 constexpr int KB = 32;             // contraction depth of a staged tile
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // 16-byte load at any 4-byte address
 
@@ -224,8 +224,10 @@ __device__ __forceinline__ void online(float& m, float& l, float m2, float l2) {
 }
 
 // one workgroup a row: the pieces of S summed in order (PIECES), the hard negative's score, lse and the row's loss; of a
-// small batch the last workgroup takes the mean as well (MEAN; B = 64: 19.6 -> 16.5 us without the launch for it; the fence in
-// front of the count is dear where there are many rows, B = 200: 13.7 -> 14.5, B = 4096: 160 -> 240)
+// small batch the last workgroup takes the mean as well (MEAN).  That saves the host a launch and costs the GPU a fence for
+// every row: forward and backward calls back to back, us, own launch and here, d = 768: B = 4 22.5 and 17.9, 32 22.8 and 19.0, 48 22.5 and
+// 21.7, 64 22.2 and 23.1, 128 25.3 and 28.1; d = 2304: 48 23.0 and 22.6, 64 23.1 and 23.2, 96 24.6 and 26.7 (the kernels alone, d =
+// 768: B = 4 11.2 and 11.2, 32 11.3 and 12.2, 64 11.9 and 13.6, 200 12.7 and 16.9).
 template <bool PIECES, bool MEAN>
 __global__ __launch_bounds__(256) void loss_rows_kernel(LossArgs a) {
     __shared__ float sm[4], sl[4], sd[4];
