@@ -198,6 +198,33 @@ def test_every_pair_of_several_workgroups(B, L, H, dtype):
     _check_attention(*y, dict(cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=_dev()), max_seqlen=L), cu=cu)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lens,lead,tail,H", [([30, 0, 5], 900, 6000, 12), ([300], 0, 3001, 1), ([70] * 6, 1, 2000, 40), ([], 0, 500, 3), ([129, 1], 5000, 0, 5)])
+def test_packed_buffers_with_many_unused_rows(lens, lead, tail, H, dtype):
+    """A buffer of a fixed size: rows of no sequence come out as zeros, whatever the outputs' views, and nothing else of them is written."""
+    from otter_amd import training as T
+    n, dev = sum(lens), _dev()
+    total = lead + n + tail
+    cu = torch.tensor([lead] + [lead + sum(lens[:i + 1]) for i in range(len(lens))], dtype=torch.int32, device=dev)
+    q, k, v, do = (_rand(410 + i, total, H, 64, dtype=dtype)[1] for i in range(4))
+    kw = dict(max_seqlen=max(lens, default=0), dropout_p=0.1, seed=_seed(), call=6)
+    used = slice(lead, lead + n)
+    out, lse = T.attention_forward(q, k, v, cu_seqlens=cu, **kw)
+    buf = torch.full((total + 8, 5, H, 64), 7.0, device=dev, dtype=dtype)       # three of its five columns are the gradients
+    grads = buf[4:4 + total, 1:4].unbind(1)
+    T.attention_backward(do, q, k, v, out, lse, cu_seqlens=cu, grads=grads, **kw)
+    if n:
+        tight = tuple(t[used].contiguous() for t in (q, k, v))
+        out2, lse2 = T.attention_forward(*tight, cu_seqlens=cu - lead, **kw)
+        g2 = T.attention_backward(do[used].contiguous(), *tight, out2, lse2, cu_seqlens=cu - lead, **kw)
+        _same((out[used], lse[:, used]), (out2, lse2))
+        for a, b in zip(grads, g2):                             # the way may be another one: a half step of each
+            assert ((a[used].double() - b.double()).abs() <= 4 * R.half_step(dtype) * b.double().abs().amax()).all()
+    for t in (out, lse.t(), *grads):
+        assert (t[:lead] == 0).all() and (t[lead + n:] == 0).all()
+    assert (buf[:4] == 7).all() and (buf[4 + total:] == 7).all() and (buf[:, 0] == 7).all() and (buf[:, 4] == 7).all()
+
+
 # ------------------------------------------------------------------------------------------------- autograd's own records
 def test_explicit_halves_have_no_history():
     """Whatever p is and whatever has to be copied or cast on the way."""
