@@ -213,7 +213,11 @@ int otter_inbatch_scores(int device, const float* q, const float* c, const float
                          float* product, int32_t* rank, void* stream);
 
 /* The loss of the fine-tuning script over that matrix and its gradient (reference retrieval/criterions.py:10-27:
- * cross entropy of [q c^T | q . neg_c] against the diagonal, mean over the batch), float32 throughout:
+ * cross entropy of [q c^T | q . neg_c] against the diagonal, mean over the batch), float32 in and out, sums in float32.
+ * The products of small batches are float32's.  Those of large ones (B > 256 and B^2 d > 4e8, the gradients' B > 500 and
+ * B^2 d > 3.6e8) take each operand as two float16 parts: 22 bits of every element, or 2^-39 of the largest one that a sum
+ * runs over (a row of q or c; a row of G weighted by the sizes of c's rows, a column weighted by q's) where that is more.
+ * A score that is NaN, or a target's score of +inf, makes its row's loss and gradients NaN.
  *   S = [q c^T | q . neg_c],  lse_i = log sum_j exp S_ij,  *loss = mean_i (lse_i - S_ii)
  *   G = (exp(S - lse) - 1[j = i]) * *dloss / B,  dq = G c + G_neg neg_c,  dc = G^T q,  dneg = G_neg q
  * All pointers are device pointers: q, c, neg_c (may be NULL) float32 [B, d]; scores float32 [B, ld] with
@@ -221,7 +225,8 @@ int otter_inbatch_scores(int device, const float* q, const float* c, const float
  * stats float32 [2, B]: lse, and 1 - the target's probability (what G's diagonal is made of: exp(S_ii - lse_i) - 1 itself
  * would be all rounding where a row's loss is small); loss, dloss float32 [1].  1 <= B <= 65536.  Each call needs a workspace of
  * otter_inbatch_loss_workspace(B, d) / otter_inbatch_loss_backward_workspace(B, d) bytes (may be 0), 16-byte aligned,
- * for its time (stream order).  Both calls only enqueue; the same inputs give the same bits (no atomics). */
+ * for its time (stream order).  ceil(B / 64) ceil(d / 64) <= 2^23 - 1.  Both calls only enqueue; the same inputs give the same
+ * bits (no atomics on data; of up to 48 rows a counter in the workspace finds the workgroup that takes the mean). */
 int64_t otter_inbatch_loss_workspace(int B, int d);
 int64_t otter_inbatch_loss_backward_workspace(int B, int d);
 int otter_inbatch_loss_forward(int device, const float* q, const float* c, const float* neg_c, int B, int d,
@@ -344,8 +349,9 @@ void otter_encoder_destroy(otter_encoder* enc);
 
 /* Layer operators of a fine-tuning step (the reference trains the encoder of retrieval/models/tb_retriever.py with
  * torch autograd, scripts/train_1hop_tb_retrieval.py:196-262).  dtype = element type of the activations and their
- * gradients: OTTER_F32 or OTTER_BF16; sums, statistics and probabilities are float32.  Every call only enqueues,
- * allocates nothing and uses no atomics: the same inputs give the same bits.
+ * gradients: OTTER_F32 or OTTER_BF16; sums, statistics and norms are float32.  Every call only enqueues, allocates
+ * nothing and uses no atomics: the same inputs give the same bits.  Attention in bfloat16 rounds dropped-out probabilities
+ * and dS to bfloat16 in front of the products that take them, and takes D = sum dO O from the stored out (see there).
  *
  * Dropout: value e is dropped where its 16-bit draw is below T = round(65536 p), kept values are scaled by
  * 65536 / (65536 - T); 0 <= p < 1.  The draws are Philox4x32 with 7 rounds under the 64-bit key *seed (DEVICE
@@ -382,10 +388,13 @@ int otter_layernorm_backward(int device, int dtype, int wdtype, const void* dy, 
  * contiguous.  Data pointers and strides are multiples of 16 bytes.
  *   dense   cu_seqlens NULL: [batch, tokens, heads, 64]; mask int64 [batch, tokens] (non-zero = attend, as input_mask of
  *           the encoder) or NULL for every key.  Keys left out reach nothing, whatever they hold.  A sequence whose mask
- *           leaves nothing attends to all its keys evenly, as in the encoder; no gradient reaches its q and k.
+ *           leaves nothing attends to all its keys evenly, as in the encoder; no gradient reaches its q and k, nor
+ *           those of a sequence with one key, whichever it is.
  *   packed  cu_seqlens int32 [batch + 1], non-decreasing: sequence b is rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of
  *           [total, heads, 64] tensors (stride_batch unused); tokens = the longest sequence (sizes the launch; a
- *           longer one is still computed).  Rows of no sequence are set to zero in the outputs.
+ *           longer one is still computed, for which the backward pass in one pass takes 256 bytes a row and head of
+ *           workspace whatever tokens says).  Rows of no sequence are set to zero in the outputs.
+ * batch x heads x ceil(tokens / 128) < 2^24.  The outputs overlap neither each other nor an operand.
  * lse: float32 [batch, heads, tokens] / [heads, total], log sum_j exp(scale q k^T), written by the forward pass. */
 typedef struct otter_view {
     void* data;

@@ -13,6 +13,12 @@
 // operand needs ("accumulator tile as the next operand").  So the tile is made with the QUERY on the lane where the
 // contraction runs over keys (O, dQ) and with the KEY on the lane where it runs over queries (dK, dV): no probability
 // ever goes through memory.
+//
+// Roundings.  float32: none but float32's own.  bfloat16: scores, softmax, their sums and all accumulators are float32, but the
+// matrix unit takes bfloat16, so that P Z (in front of P V and of dV) and dS (in front of dQ and dK) are rounded to it, half a step
+// (2^-8) of each weight; and D comes from the stored, rounded O, except where 64 keys hold a whole sequence (two passes; one
+// pass of batches up to 128 tokens), whose O is as large as its terms.  Off from 64 bits by 2.4e-3 of the outputs' size, where
+// rounding the outputs alone costs 1.7e-3; splitting P and dS in two parts would double those products.
 #include "otter_common.h"
 #include "otter_philox.h"
 
@@ -440,8 +446,8 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 // The running maximum is let stand while no score passes it by more than 2^8 (in base 2 exponents: the sums and the
 // probabilities then stay below 2^8 times their final size, harmless in float32 and for bfloat16's relative rounding), so
 // that the accumulators are rescaled once or twice a row and not at every tile.
-// Bound by the matrix unit and the vector unit together: of their times only about a third overlaps, with exp2, the draws and
-// the conversion to bfloat16 about as long as the products.  bfloat16: 2 x 4001 tokens, 12 heads, no dropout 131 us
+// Bound by the vector unit beside the matrix unit: 2 x 4001 tokens keep a SIMD's vector unit busy 58 % of its cycles (exp2, the
+// conversion to bfloat16) and the matrix unit 32 %, one after the other within a wave; packed with dropout 60 % and 15 %.  bfloat16: 2 x 4001 tokens, 12 heads, no dropout 131 us
 // = 0.75 PFLOP/s (a large matrix product: 1.15); 128 packed of up to 512 with dropout 124 us, without 91; 16 x 512 ragged 28 us.
 // float32, 8 x 512 ragged: 64 us, 57 TFLOP/s on the 32x32x2 products (a large product: 154).
 template <typename T, bool DROP, bool HALF>
@@ -787,11 +793,12 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnTrainArgs a) {
 // bfloat16.  A workgroup of 8 waves owns a (sequence, head); it takes its keys 256 at a time, a wave 32 (one on each lane of a
 // half), and streams the queries in tiles of 32.  Every score tile is made ONCE: probabilities and dS go from the registers
 // into dV and dK as in attn_dkv_kernel, dS also goes to LDS (64 bytes a key), from where all waves together make the tile's
-// dQ, a block of 16 queries x 16 elements each, with their 16 columns of K^T in registers.  dQ of more than 256 keys is
+// dQ, a block of 16 queries x 16 elements each, K read transposed from LDS.  dQ of more than 256 keys is
 // carried in a float32 buffer that the same thread writes and reads.  One barrier a tile; D comes out of the staging.
-// Bound by the workgroup that a CU holds: eight waves that meet at a barrier for every tile, where matrix and vector unit take
-// turns: 2.6 to 3.4 us a tile of 32 x 256, whose five products take 1.2 us at a large matrix product's rate.  128 packed sequences
-// of up to 512, 12 heads, dropout: 318 us (0.26 PFLOP/s), without dropout 284.  Tiles of 64 queries, half the barriers, measured
+// Bound by the workgroup that a CU holds (93 KB of LDS): eight waves that meet at a barrier for every tile, 2.6 to 3.4 us a tile of
+// 32 x 256, whose five products take 1.2 us at a large matrix product's rate.  128 packed sequences of up to 512, 12 heads, dropout: 318
+// to 365 us by the order of their lengths (0.26 PFLOP/s), without dropout 285; of a SIMD's cycles the matrix unit is busy 14 %, the
+// vector unit 32 %, neither for the rest.  Tiles of 64 queries, half the barriers, measured
 // no better (337 us), nor did orders of the instructions pinned by hand.
 // SHORT: batches of short sequences, see D below (in a batch of long ones it would cost 64 x 200 tokens 70 -> 96 us).
 constexpr int FK = 256, FQ = 32;      // keys at a time, rows of a streamed tile
@@ -835,7 +842,7 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
     typedef float f32x4 __attribute__((ext_vector_type(4)));
     __shared__ __attribute__((aligned(16))) char sQ[2][FQ * X::PITCH];
     __shared__ __attribute__((aligned(16))) char sO[2][FQ * X::PITCH];
-    __shared__ __attribute__((aligned(16))) char sS[2][FK * SPITCH];        // first K's 256 rows, then dS^T of a tile
+    __shared__ __attribute__((aligned(16))) char sS[2][FK * SPITCH];        // dS^T of a tile, two of them in turn
     __shared__ __attribute__((aligned(16))) float sL[2][FQ], sD[2][FQ];
     __shared__ __attribute__((aligned(16))) char sK[FK * X::PITCH];
     __shared__ float sE[SHORT ? 2 : 1][FQ];
@@ -912,8 +919,7 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
                 if (tid < FQ) sL[buf][tid] = i0 + tid < s.len ? rl * 1.4426950408889634f : INFINITY;
             };
             fetch(0);
-            // K^T: 16 elements x 256 keys, a lane one element and 8 keys of every 32
-            __syncthreads();
+            __syncthreads();                               // the keys before these are done with
             float4 kt[4];
             bool kc[4];
 #pragma unroll
@@ -929,7 +935,7 @@ __global__ __launch_bounds__(512, 2) void attn_bwd_kernel(AttnTrainArgs a) {
             __syncthreads();
             store(0, 0);
             if (FQ < s.len) fetch(FQ);
-            __syncthreads();                               // K^T is read, tile 0 is there
+            __syncthreads();                               // K and tile 0 are there
             if (!busy)                                     // keys nobody has: their dS is zero once and for all
                 for (int e = lane; e < 32 * SPITCH / 4; e += 64) {
                     reinterpret_cast<u32*>(sS[0] + wave * 32 * SPITCH)[e] = 0;

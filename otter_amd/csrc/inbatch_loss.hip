@@ -12,7 +12,8 @@
 // one e for the elements that a sum runs over, and hi hi' + hi lo' + lo hi' run on v_mfma_f32_32x32x16_f16, sixteen times
 // float32's rate for three times its products.  hi + lo is good to 22 bits of an element, or to 2^-39 of the largest one of its e
 // where that is more (elements below 2^-17 of it): what a term loses is at most 3 2^-22 of it or 2^-38 of the largest one a sum
-// could have, less than the float32 sums' own rounding over a row of 64 and more.  So that rows of very different weight in
+// could have, less than the float32 sums' own rounding over a row of 64 and more.  (An infinity in q or c has no second plane: its
+// scores come out as NaN.)  So that rows of very different weight in
 // a batch (a confident row's gradient is e^-margin of a hard one's) and of very different size keep that, S has an e for every row
 // of q and of c, dq one for every row of G weighted by the sizes of c's rows, dc one for every COLUMN of G weighted by q's: two
 // pairs of planes of G.  S is kept (4 B^2 bytes) instead of multiplied out again in the backward pass (2 B^2 d flops).

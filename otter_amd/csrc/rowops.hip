@@ -515,8 +515,10 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // rows a workgroup of 256 handles at a time: half a wave a row up to 1024 columns, the workgroup a row above
 int rows_per_block(int cols) { return cols <= 1024 ? 8 : 1; }
 
-// workgroups: as many as are resident together (65536 x 768 bf16: the forward pass 50.6 us with 768, 52.5 with 1024; the
-// backward pass, whose every workgroup leaves a row of partial sums, 101.5 with 512, 102.7 with 1024)
+// workgroups: as many as are resident together at 768 columns of bfloat16 (65536 rows: the forward pass 50.6 us with 768, 52.5
+// with 1024; the backward pass, whose every workgroup leaves a row of partial sums, 101.5 with 512, 102.7 with 1024).  Where a lane
+// holds more (backward: four groups, from 769 columns on, and three of float32, from 513) the registers leave one wave a SIMD and
+// half of these run at a time: float32 with the weights' sums 2000 x 771 12 us, 4097 x 771 20, 8192 x 771 28.
 int norm_grid(long long rows, int cols, bool bwd) {
     const long long need = (rows + rows_per_block(cols) - 1) / rows_per_block(cols), most = bwd ? 512 : 768;
     return (int)(need < most ? need : most);

@@ -8,7 +8,8 @@ Each operator comes in two forms:
   * attention / layer_norm / dropout            one differentiable call (torch autograd, first order)
   * *_forward / *_backward                      the two halves as plain calls, for loops that keep their own tape and for
                                                 captured graphs
-Activations are float32 or bfloat16; sums, softmax statistics and probabilities are float32.  There is no CPU path.
+Activations are float32 or bfloat16; sums, softmax statistics and norms are float32.  bfloat16 attention rounds the dropped-out
+probabilities and the scores' gradients to bfloat16 in front of the matrix products that take them.  There is no CPU path.
 
 Dropout stores no mask.  Its random numbers are drawn from `seed`, an int64 tensor with one element ON THE GPU (a captured
 graph reads the value it holds at replay), and `call`, a number that tells apart the calls sharing that seed: give every

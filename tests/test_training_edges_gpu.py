@@ -283,3 +283,15 @@ def test_overlapping_outputs_are_refused():
     _same(T.attention_backward(do, q, k, v, out, lse, grads=(a, b, c)), ref)
     empty = torch.empty(0, 8, 2, 64, device=_dev())
     T.attention_backward(empty, empty, empty, empty, empty, torch.empty(0, 2, 8, device=_dev()), grads=(empty,) * 3)
+
+
+def test_mixed_types_are_refused():
+    """What autocast makes of a layer: a product in bfloat16 beside a residual in float32."""
+    from otter_amd import training as T
+    x = torch.randn(4, 8, device=_dev())
+    w = torch.ones(8, device=_dev())
+    with pytest.raises(ValueError, match="residual must be like"):
+        T.layer_norm(x.bfloat16(), w, w, residual=x)
+    with pytest.raises(ValueError, match="float32 or bfloat16"):
+        T.layer_norm(x.half(), w, w)
+    assert T.layer_norm(x.bfloat16(), w, w, residual=x.bfloat16()).dtype == BF16
