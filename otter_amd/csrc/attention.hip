@@ -1147,7 +1147,8 @@ void launch_fwd(AttnTrainArgs& a, hipStream_t st) {
 //                     512 80 and 80, 20 x 300 46 and 42 -> two passes
 //   (more rounds)     22 x 512 159 and 132, 32 x 512 163 and 163, 36 x 512 170 and 181, ragged 161 and 157, 42 x 512 181 and 210, ragged
 //                     170 and 174, packed 151 and 140, 128 packed 318 and 379 -> where the last round is not mostly empty
-//   longer            full: 21 x 700 169 and 211, 40 x 1500 1307 and 1447, 64 x 2000 3675 and 3998; 16 x 1500 615 and 578; with a mask 40 x 700
+//   longer            full: 21 x 700 169 and 211, 40 x 1500 1307 and 1447, 64 x 2000 3675 and 3998; 16 x 1500 615 and 578; beyond 8 FK the
+//                     carried dQ, 64 times the workspace, brings no more: 64 x 3000 8695 and 8766, 21 x 4096 5255 and 5298; with a mask 40 x 700
 //                     305 and 279, 40 x 1500 1219 and 995, 64 x 700 413 and 450, 64 x 1000 738 and 793, 64 x 1500 1555 and 1554, 64 x 2000 2858
 //                     and 2574 -> full ones where the last round is not mostly empty, with a mask from three rounds on and
 //                     up to 6 FK; packed by how full, 40 x 700: 0.70 299 and 253, 0.80 303 and 297, 0.90 313 and 349; 64 x 1000: 0.56 601
@@ -1160,7 +1161,7 @@ bool one_pass(const AttnTrainArgs& a, int dtype) {
     if (a.L <= FK) return pairs > CUS / 4;
     const bool last = 5 * pairs >= 4 * rounds * CUS;           // the last round is not mostly empty
     const bool full = a.cu ? 15 * a.T >= (rounds >= 3 ? 10 : 12) * (long long)a.B * a.L : !a.mask;
-    if (a.L > 2 * FK) return last && (full || (!a.cu && rounds >= 3 && a.L <= 6 * FK));
+    if (a.L > 2 * FK) return last && (full ? a.L <= 8 * FK : !a.cu && rounds >= 3 && a.L <= 6 * FK);
     if (rounds > 1) return last;
     return full ? a.nblk * pairs > 2 * CUS : !a.cu && 4 * pairs >= 3 * CUS;
 }

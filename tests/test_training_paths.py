@@ -27,7 +27,7 @@ def test_full_batches_take_one_pass_where_it_is_faster(batch, tokens):
     assert takes_one_pass(batch, tokens, 12, total=batch * tokens)
 
 
-@pytest.mark.parametrize("batch,tokens", [(10, 512), (14, 300), (16, 1500), (22, 512)])
+@pytest.mark.parametrize("batch,tokens", [(10, 512), (14, 300), (16, 1500), (22, 512), (64, 3000), (42, 8192)])
 def test_full_batches_take_two_passes_where_those_are_faster(batch, tokens):
     assert not takes_one_pass(batch, tokens, 12)
 
