@@ -295,3 +295,85 @@ def test_mixed_types_are_refused():
     with pytest.raises(ValueError, match="float32 or bfloat16"):
         T.layer_norm(x.half(), w, w)
     assert T.layer_norm(x.bfloat16(), w, w, residual=x.bfloat16()).dtype == BF16
+
+
+# ------------------------------------------------------------------------------------------------------ graphs and streams
+@pytest.mark.parametrize("dtype,total,longest", [(F32, 700, 300), (BF16, 700, 300), (BF16, 3000, 512)])
+def test_captured_packed_step_follows_its_lengths(dtype, total, longest):
+    """A buffer of a fixed size in a graph: every replay has other sequences in it, and other rows of no sequence."""
+    from otter_amd import training as T
+    H, B, dev = 12, 8, _dev()
+    q, k, v, do = (_rand(420 + i, total, H, 64, dtype=dtype)[1] for i in range(4))
+    cu, seed = torch.zeros(B + 1, dtype=torch.int32, device=dev), _seed(1)
+
+    def step():
+        kw = dict(cu_seqlens=cu, max_seqlen=longest, dropout_p=0.1, seed=seed, call=2)
+        out, lse = T.attention_forward(q, k, v, **kw)
+        return (out, lse, *T.attention_backward(do, q, k, v, out, lse, **kw))
+
+    with torch.cuda.stream(torch.cuda.Stream()):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    g = torch.Generator().manual_seed(9)
+    for i in range(5):
+        lens = torch.randint(0, min(longest, total // B) + 1, (B,), generator=g)
+        lead = int(torch.randint(0, total - int(lens.sum()) + 1, (1,), generator=g))
+        cu.copy_(lead + torch.cat((torch.zeros(1, dtype=torch.int64), lens.cumsum(0))).int())
+        seed.fill_(50 + i)
+        q.copy_(torch.randn_like(q))
+        exp = [t.clone() for t in step()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        _same(got, exp)
+        n = int(lens.sum())
+        assert all((t[:lead] == 0).all() and (t[lead + n:] == 0).all() for t in (got[0], *got[2:]))
+
+
+@pytest.mark.parametrize("B,d", [(40, 768), (64, 2304), (300, 100), (700, 768), (1300, 256)])
+def test_captured_loss_follows_its_inputs(B, d):
+    q, c, n = (_rand(430 + i, B, d, scale=d ** -0.25)[1] for i in range(3))
+    with torch.cuda.stream(torch.cuda.Stream()):
+        _loss_step(q, c, n)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    one = torch.ones((), device=_dev())
+    from otter_amd import inbatch as IB
+    with torch.cuda.graph(graph):
+        loss, product, stats = IB.inbatch_loss_forward(q, c, n)
+        got = (loss, product, stats, *IB.inbatch_loss_backward(one, q, c, n, product, stats))
+    for i in range(4):
+        for t in (q, c, n):
+            t.copy_(torch.randn_like(t) * (0.5 + i) * d ** -0.25)
+        exp = [t.clone() for t in _loss_step(q, c, n)]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        _same(got, exp)
+
+
+def test_two_losses_at_once_on_two_streams():
+    x = [[_rand(440 + 3 * s + i, 900, 768, scale=768 ** -0.25)[1] for i in range(3)] for s in range(2)]
+    exp = [_loss_step(*t) for t in x]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for t in x:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got.append(_loss_step(*t))
+        torch.cuda.synchronize()
+        for a, b in zip(got, exp):
+            _same(a, b)
+
+
+@pytest.mark.parametrize("B,d", [(40, 96), (700, 640)])
+def test_loss_of_strided_and_mixed_inputs(B, d):
+    """Transposed, sliced and half-width inputs give what their float32 copies give."""
+    q, c, n = (_rand(450 + i, B, d, scale=d ** -0.25)[1] for i in range(3))
+    exp = _loss_step(q, c.bfloat16().float(), n)
+    wide = torch.zeros(B, 2 * d + 1, device=_dev())
+    wide[:, 1:d + 1] = n
+    _same(_loss_step(q.t().contiguous().t(), c.bfloat16(), wide[:, 1:d + 1]), exp)
